@@ -255,3 +255,19 @@ def test_backward_edges(bw, dev, native_sdp, Sq, Sk, H, Hkv, causal):
             assert (ab - bb).norm() <= 8 * 2.0 ** -9 * bb.norm(), (name, i, float((ab - bb).norm() / bb.norm()))
     bw.synchronize()
     assert bw._C._gemm_status(False) == 0
+
+
+def test_first_call_of_a_new_thread_runs_the_native_kernel(bw, dev, native_sdp):
+    """A fresh thread has no context of the device until a runtime call gives it one; memory from the cache makes none.  The tensor
+    maps of the kernel could not be encoded there, and the call went to the library."""
+    import threading
+
+    q = torch.randn(1, 2, 128, 128, device=dev, dtype=torch.bfloat16)
+    want = F.scaled_dot_product_attention(q, q, q, is_causal=True)
+    del want          # its blocks are in the cache now
+    before, got = bw._C._native_sdp_forward_calls(), []
+    thread = threading.Thread(target=lambda: got.append(F.scaled_dot_product_attention(q, q, q, is_causal=True)))
+    thread.start()
+    thread.join()
+    assert bw._C._native_sdp_forward_calls() == before + 1
+    assert torch.equal(got[0], F.scaled_dot_product_attention(q, q, q, is_causal=True))

@@ -93,7 +93,13 @@ void set_device(c10::DeviceIndex d) {
 c10::DeviceIndex exchange_device(c10::DeviceIndex d) {
   int cur = -1;
   B200_CUDA_CHECK(cudaGetDevice(&cur));
-  if (d >= 0 && d != cur) B200_CUDA_CHECK(cudaSetDevice(d));
+  // A thread that has made no runtime call yet names device 0 without having its context, and driver calls (the encoding of a
+  // tensor map) fail there: the first switch of a thread binds the context even when the number is the same.
+  static thread_local bool bound = false;
+  if (d >= 0 && (d != cur || !bound)) {
+    B200_CUDA_CHECK(cudaSetDevice(d));
+    bound = true;
+  }
   if (d >= 0 && d < kMaxDevices) g_ctx_touched[d] = true;
   return static_cast<c10::DeviceIndex>(cur);
 }
