@@ -1,0 +1,235 @@
+"""Causal attention with a sliding window and sinks on the tensor-core kernels, dense and packed, against the formulas in 64 bits.
+
+Tolerances are bounds, not guesses.  With u = eps / 2 of the type, the kernels round P (and in the backward P and dS) to the type
+before a product and every result once; sums are 32-bit.  So |o - o'| <= u (sum p |v| + |o|), |dV - dV'| <= u (sum p |dO| + |dV|),
+and dS carries u |dS| and scale p e with e = sum_d (error of o_d) |dO_d|, the error of the row sums that the backward forms from
+the rounded o.  Beside them stands 2^-14 of the same sums for the 32-bit parts, and 2^-25 for each value below fp16's normal range (its steps there are 2^-24): per term of a sum, and once for the result."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+D = 128
+
+
+def visible(sq, sk, window, sinks):
+    i, j = torch.arange(sq)[:, None], torch.arange(sk)[None, :]
+    m = j <= i
+    return m if window is None else m & ((i - j < window) | (j < sinks))
+
+
+def formula(q, k, v, do, window, sinks, scale=None):
+    """One sequence: q [Sq, H, D], k / v [Sk, Hkv, D] in any type.  Returns {name: (value, bound)} in 64 bits."""
+    u = torch.finfo(q.dtype).eps / 2
+    tiny = 2.0 ** -25
+    c = u + 2.0 ** -14
+    H, Hkv = q.shape[1], k.shape[1]
+    G, scale = H // Hkv, scale if scale is not None else 1 / math.sqrt(D)
+    seen = visible(q.shape[0], k.shape[0], window, sinks)
+    q, k, v, do = (t.double() for t in (q, k, v, do))
+    r = {n: [torch.zeros_like(t), torch.zeros_like(t)] for n, t in (("o", q), ("dq", q), ("dk", k), ("dv", v))}
+    for h in range(H):
+        qh, kh, vh, gh = q[:, h], k[:, h // G], v[:, h // G], do[:, h]
+        s = (qh @ kh.T * scale).masked_fill(~seen, -math.inf)
+        top = s.amax(1, keepdim=True) if s.shape[1] else s.new_zeros(s.shape[0], 1)
+        p = torch.exp(s - top.masked_fill(top == -math.inf, 0))
+        p = p / p.sum(1, keepdim=True).clamp_min(1e-300)
+        o = p @ vh
+        e_o = c * (p @ vh.abs() + o.abs()) + tiny * (seen.double() @ vh.abs())
+        ds = p * (gh @ vh.T - (gh * o).sum(1, keepdim=True)) * scale
+        e_ds = c * ds.abs() + scale * p * (e_o * gh.abs()).sum(1, keepdim=True) + 2.0 ** -14 * scale * p * (gh.abs() @ vh.abs().T) + tiny * seen.double()
+        dq, dk, dv = ds @ kh, ds.T @ qh, p.T @ gh
+        for n, at, val, err in (("o", h, o, e_o), ("dq", h, dq, e_ds @ kh.abs() + u * dq.abs()), ("dk", h // G, dk, e_ds.T @ qh.abs()),
+                                ("dv", h // G, dv, c * (p.T @ gh.abs()) + tiny * (seen.double().T @ gh.abs()))):
+            r[n][0][:, at] += val
+            r[n][1][:, at] += err
+    for n in ("dk", "dv"):
+        r[n][1] += u * r[n][0].abs()
+    return r
+
+
+def check(got, want, what):
+    value, bound = want
+    over = (got.double().cpu() - value).abs() - bound - 2.0 ** -25
+    assert bool((over <= 0).all()), f"{what}: {float(over.max())} over the bound, at {tuple(int(x) for x in torch.nonzero(over == over.max())[0])}"
+
+
+def inputs(dt, q_shape, k_shape, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    mk = lambda s: torch.randn(*s, generator=g).to(dt)  # noqa: E731
+    return mk(q_shape), mk(k_shape), mk(k_shape), mk(q_shape)
+
+
+DENSE = [  # B, Sq, Sk, H, Hkv, window, sinks
+    (1, 1, 1, 1, 1, 1, 0), (1, 5, 5, 2, 1, 1, 0), (2, 128, 128, 2, 2, 128, 0), (1, 129, 129, 2, 1, 128, 1), (1, 300, 300, 4, 2, 1, 4),
+    (2, 511, 511, 2, 2, 64, 0), (1, 640, 640, 4, 1, 130, 130), (1, 777, 777, 2, 1, 257, 3), (1, 1024, 1024, 2, 2, 256, 300),
+    (1, 1400, 1400, 2, 1, 100, 5), (1, 400, 400, 2, 2, 100000, 7), (1, 700, 200, 2, 1, 64, 0), (1, 700, 200, 2, 1, 64, 2), (1, 130, 600, 2, 2, 50, 129),
+]
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("B,Sq,Sk,H,Hkv,window,sinks", DENSE)
+def test_dense_forward_and_gradients(bw, dev, dt, B, Sq, Sk, H, Hkv, window, sinks):
+    from torch_musa_b200.ops import window_attention
+
+    q, k, v, do = inputs(dt, (B, Sq, H, D), (B, Sk, Hkv, D))
+    leaves = [t.to(dev).requires_grad_() for t in (q, k, v)]
+    before = bw._C._native_sdp_forward_calls(), bw._C._native_sdp_backward_calls()
+    out = window_attention(*leaves, window, sinks)
+    grads = torch.autograd.grad(out, leaves, do.to(dev))
+    assert (bw._C._native_sdp_forward_calls(), bw._C._native_sdp_backward_calls()) == (before[0] + 1, before[1] + 1)
+    bw.synchronize()
+    assert bw._C._gemm_status(False) == 0
+    for b in range(B):
+        want = formula(q[b], k[b], v[b], do[b], window, sinks)
+        for n, got in zip(("o", "dq", "dk", "dv"), (out, *grads)):
+            check(got.detach()[b], want[n], n)
+
+
+PACKED = [  # lengths of the queries, lengths of the keys, H, Hkv, window, sinks, rows past the last sequence
+    ([1], None, 2, 1, 3, 0, 0), ([300, 1, 129, 64], None, 4, 2, 100, 3, 0), ([200, 333], None, 2, 2, 257, 130, 70), ([0, 260, 0, 5], None, 2, 1, 32, 1, 3),
+    ([900, 17], None, 2, 1, 64, 4, 200), ([400, 100], [90, 500], 2, 1, 40, 0, 1), ([64, 30], [0, 30], 2, 1, 40, 2, 0),
+]
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lens,klens,H,Hkv,window,sinks,extra", PACKED)
+def test_packed_sequences(bw, dev, dt, lens, klens, H, Hkv, window, sinks, extra):
+    """Rows past the last sequence hold NaN: they reach nobody, and get zeros."""
+    from torch_musa_b200.ops import flash_attn_varlen_func
+
+    klens = klens or lens
+    q, k, v, do = inputs(dt, (sum(lens) + extra, H, D), (sum(klens) + extra, Hkv, D))
+    for t, n in ((q, lens), (k, klens), (v, klens), (do, lens)):
+        t[sum(n):] = float("nan")
+    cq = torch.tensor([0] + lens).cumsum(0).to(torch.int32)
+    ck = torch.tensor([0] + klens).cumsum(0).to(torch.int32)
+    leaves = [t.to(dev).requires_grad_() for t in (q, k, v)]
+    out = flash_attn_varlen_func(*leaves, cq.to(dev), ck.to(dev), max(lens), max(klens), causal=True, window=window, sinks=sinks)
+    grads = torch.autograd.grad(out, leaves, do.to(dev))
+    bw.synchronize()
+    assert bw._C._gemm_status(False) == 0
+    got = [t.detach().cpu() for t in (out, *grads)]
+    for i in range(len(lens)):
+        a, b = slice(cq[i], cq[i + 1]), slice(ck[i], ck[i + 1])
+        want = formula(q[a], k[b], v[b], do[a], window, sinks)
+        for n, t, rows in zip(("o", "dq", "dk", "dv"), got, (a, a, b, b)):
+            check(t[rows], want[n], f"sequence {i}, {n}")
+    for t, n in zip(got, (lens, lens, klens, klens)):
+        assert bool((t[sum(n):] == 0).all())
+
+
+def test_a_window_longer_than_the_sequence_is_the_causal_mask(bw, dev):
+    """Bit for bit: the same blocks in the same order."""
+    import torch.nn.functional as F
+    from torch_musa_b200.ops import flash_attn_varlen_func, window_attention
+
+    q, k, v, _ = (t.to(dev) for t in inputs(torch.bfloat16, (2, 515, 4, D), (2, 515, 2, D)))
+    want = F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), is_causal=True, enable_gqa=True).transpose(1, 2)
+    assert torch.equal(window_attention(q, k, v, 515), want)
+    cu = torch.tensor([0, 515, 1030], dtype=torch.int32).to(dev)
+    flat = [t.reshape(1030, -1, D) for t in (q, k, v)]
+    assert torch.equal(flash_attn_varlen_func(*flat, cu, cu, 515, 515, causal=True, window=600).view_as(want), want)
+    assert torch.equal(flash_attn_varlen_func(*flat, cu, cu, 515, 515, causal=True).view_as(want), want)
+
+
+def test_strided_broadcast_and_odd_operands(bw, dev):
+    """Views of one fused projection, an expanded head, and rows that do not start on 16 bytes."""
+    from torch_musa_b200.ops import window_attention
+
+    g = torch.Generator().manual_seed(3)
+    qkv = torch.randn(2, 260, 8, D, generator=g).to(torch.bfloat16)
+    q, k, v = qkv.split([4, 2, 2], 2)
+    plain = window_attention(*(t.contiguous().to(dev) for t in (q, k, v)), 70, 2)
+    dq, dk, dv = qkv.to(dev).split([4, 2, 2], 2)
+    assert torch.equal(window_attention(dq, dk, dv, 70, 2), plain)
+    one = k[:, :, :1].contiguous().to(dev)
+    assert torch.equal(window_attention(dq, one.expand(-1, -1, 2, -1), dv, 70, 2), window_attention(dq, one.repeat(1, 1, 2, 1), dv, 70, 2))
+    odd = torch.zeros(q.numel() + 1, dtype=torch.bfloat16)
+    odd[1:] = q.flatten()
+    assert torch.equal(window_attention(odd.to(dev)[1:].view(q.shape), dk, dv, 70, 2), plain)
+    leaf = one.clone().requires_grad_()          # the gradient of a broadcast head is the sum over its copies
+    grad = torch.autograd.grad(window_attention(dq, leaf.expand(-1, -1, 2, -1), dv, 70, 2), leaf, torch.ones_like(plain))[0]
+    assert grad.shape == one.shape
+
+
+def test_gradients_against_differences(bw, dev):
+    """Along a random direction, the change of a weighted output over a step of 2^-4 (exact in bf16 for inputs that are
+    multiples of 2^-3): the formula's curvature and the rounding of the outputs bound what differs."""
+    from torch_musa_b200.ops import window_attention
+
+    g = torch.Generator().manual_seed(5)
+    S, window, sinks, h = 200, 60, 2, 2.0 ** -4
+    x = [(torch.randint(-8, 9, (1, S, n, D), generator=g) / 8.0) for n in (2, 1, 1)]
+    w = torch.randn(1, S, 2, D, generator=g).to(torch.bfloat16)
+    leaves = [t.to(torch.bfloat16).to(dev).requires_grad_() for t in x]
+    grads = torch.autograd.grad(window_attention(*leaves, window, sinks), leaves, w.to(dev))
+    bound = formula(*(t[0].to(torch.bfloat16) for t in x), w[0], window, sinks)
+    for i, n in enumerate(("dq", "dk", "dv")):
+        d = torch.randint(0, 2, x[i].shape, generator=g) * 2.0 - 1
+        ends = []
+        for sign in (1, -1):
+            moved = [t.clone() for t in x]
+            moved[i] = moved[i] + sign * h * d
+            ends.append([t[0].double() for t in moved])
+        f = [float((formula(*e, w[0].double(), window, sinks)["o"][0] * w[0].double()).sum()) for e in ends]
+        third = [float((formula(*[t[0].double() + s * 2 * h * d[0].double() * (j == i) for j, t in enumerate(x)], w[0].double(), window, sinks)["o"][0] * w[0].double()).sum()) for s in (1, -1)]
+        slope = (f[0] - f[1]) / (2 * h)
+        coarse = (third[0] - third[1]) / (4 * h)
+        got = float((grads[i].double().cpu()[0] * d[0].double()).sum())
+        # the error of a central difference is a quarter of the step-2h one's, so it is at most the distance of the two
+        allowed = abs(slope - coarse) + float((bound[n][1] * d[0].abs().double()).sum())
+        assert abs(got - slope) <= allowed, (n, got, slope, allowed)
+
+
+def test_captured_forward_and_backward_replay(bw, dev):
+    from torch_musa_b200.ops import window_attention
+
+    q, k, v, do = (t.to(dev) for t in inputs(torch.bfloat16, (1, 300, 2, D), (1, 300, 1, D)))
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    step = lambda: (lambda o: [o.detach(), *torch.autograd.grad(o, leaves, do)])(window_attention(*leaves, 64, 3))  # noqa: E731
+    side = bw.Stream()
+    side.wait_stream(bw.current_stream())
+    with bw.stream(side):
+        step()
+    bw.current_stream().wait_stream(side)
+    graph = bw.BlackwellGraph()
+    with bw.graph(graph):
+        held = step()
+    for seed in (1, 2):
+        new = [t.to(dev) for t in inputs(torch.bfloat16, (1, 300, 2, D), (1, 300, 1, D), seed)]
+        with torch.no_grad():
+            for leaf, t in zip(leaves, new):
+                leaf.copy_(t)
+        do.copy_(new[3])
+        graph.replay()
+        bw.synchronize()
+        got = [t.clone() for t in held]
+        want = step()
+        for n, (a, b) in enumerate(zip(got, want)):
+            if n == 1:       # dq: 32-bit sums in the order of arrival, rounded once
+                assert float((a.double() - b.double()).abs().max()) <= float(2 ** -8 * b.double().abs().max())
+            else:
+                assert torch.equal(a, b)
+
+
+def test_llama_with_a_window_trains_like_the_plain_model(bw, dev):
+    """The model's attention goes through the operator; logits follow the same model on the CPU in 32 bits."""
+    from torch_musa_b200.models import Llama, LlamaConfig
+
+    cfg = LlamaConfig(vocab_size=64, dim=256, n_layers=2, n_heads=2, n_kv_heads=1, ffn_dim=256, max_seq_len=256, window=40, attention_sinks=2)
+    torch.manual_seed(0)
+    model = Llama(cfg).to(torch.bfloat16)
+    tokens = torch.randint(0, 64, (2, 200), generator=torch.Generator().manual_seed(1))
+    cpu = Llama(cfg)
+    cpu.load_state_dict(model.state_dict())
+    want = cpu(tokens)
+    before = bw._C._native_sdp_forward_calls()
+    loss = model.to(dev)(tokens.to(dev), tokens.to(dev))
+    loss.backward()
+    assert bw._C._native_sdp_forward_calls() == before + cfg.n_layers
+    got = model(tokens.to(dev)).float().cpu()
+    # 16 roundings of 2^-8 along the way (norms, projections, residuals of two layers), each at most the values' own size
+    assert float((got - want).abs().max()) <= 16 * 2 ** -8 * float(want.abs().max())
+    assert all(p.grad is not None and bool(torch.isfinite(p.grad).all()) for p in model.parameters())

@@ -18,7 +18,9 @@
 #include <ATen/native/transformers/attention.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <atomic>
+#include <climits>
 #include <cstdlib>
 #include <cmath>
 
@@ -223,8 +225,18 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> sdpa_fused_bwd(
 // device.  ONE launch of the tcgen05 forward (and of the backward) covers every sequence: a CTA reads its sequence's
 // bounds from cu_seqlens and offsets its tile coordinates; nothing is read on the host.  lse is [H, total_q].
 // Parity: reference torch_musa/csrc/aten/ops/attention/mudnn/SDP.cpp:678-845 (varlen entry of the vendor flash kernel).
+void window_desc(b200_attn_t& a, const char* op, bool causal, std::optional<int64_t> window, int64_t sinks) {
+  TORCH_CHECK(sinks >= 0, op, ": sinks must not be negative, got ", sinks);
+  if (!window.has_value()) return;
+  TORCH_CHECK(*window > 0, op, ": window must be positive, got ", *window);
+  TORCH_CHECK(causal, op, ": a window needs a causal mask");
+  a.window = (int)std::min<int64_t>(*window, 1 << 30);     // longer than any sequence
+  a.sinks = (int)std::min<int64_t>(sinks, 1 << 30);
+}
+
 void varlen_desc(b200_attn_t& a, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& cu_q,
-                 const at::Tensor& cu_k, int64_t max_q, int64_t max_k, bool causal, std::optional<double> scale) {
+                 const at::Tensor& cu_k, int64_t max_q, int64_t max_k, bool causal, std::optional<double> scale,
+                 std::optional<int64_t> window, int64_t sinks) {
   TORCH_CHECK(q.dim() == 3 && k.dim() == 3 && v.dim() == 3 && q.size(2) == 128 && k.size(2) == 128 && v.sizes() == k.sizes(),
               "varlen_attention: q [total_q, H, 128], k / v [total_k, Hkv, 128]");
   TORCH_CHECK((q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf) && k.scalar_type() == q.scalar_type() &&
@@ -245,16 +257,34 @@ void varlen_desc(b200_attn_t& a, const at::Tensor& q, const at::Tensor& k, const
   a.cu_seqlens_k = cu_k.const_data_ptr<int>();
   a.total_q = (int)q.size(0);
   a.total_k = (int)k.size(0);
+  window_desc(a, "varlen_attention", causal, window, sinks);
+}
+
+// With a window there is an answer where nobody has a key or a query: zeros, and an lse of -inf.
+bool empty_window(const at::Tensor& q, const at::Tensor& k, std::optional<int64_t> window) {
+  return window.has_value() && (q.numel() == 0 || k.numel() == 0);
+}
+
+// The scratch of a windowed backward, kept alive by the caller until its kernels are launched.
+at::Tensor bwd_workspace(b200_attn_t& a, const at::Tensor& q) {
+  const int64_t n = b200_flash_attn_bwd_workspace(&a);
+  if (n == 0) return {};
+  at::Tensor ws = at::empty({n}, q.options().dtype(at::kFloat));
+  a.workspace = ws.mutable_data_ptr<float>();
+  return ws;
 }
 
 std::tuple<at::Tensor, at::Tensor> varlen_attention(const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_,
                                                     const at::Tensor& cu_q, const at::Tensor& cu_k, int64_t max_q,
-                                                    int64_t max_k, bool causal, std::optional<double> scale) {
+                                                    int64_t max_k, bool causal, std::optional<double> scale,
+                                                    std::optional<int64_t> window, int64_t sinks) {
   check_devices("varlen_attention", q_, k_, v_, cu_q, cu_k);
+  if (q_.dim() == 3 && empty_window(q_, k_, window))
+    return {at::zeros(q_.sizes(), q_.options()), at::full({q_.size(1), q_.size(0)}, -INFINITY, q_.options().dtype(at::kFloat))};
   at::Tensor q = q_.stride(2) == 1 ? q_ : q_.contiguous(), k = k_.stride(2) == 1 ? k_ : k_.contiguous(),
              v = v_.stride(2) == 1 ? v_ : v_.contiguous();
   b200_attn_t a{};
-  varlen_desc(a, q, k, v, cu_q, cu_k, max_q, max_k, causal, scale);
+  varlen_desc(a, q, k, v, cu_q, cu_k, max_q, max_k, causal, scale, window, sinks);
   at::Tensor o = at::empty({q.size(0), q.size(1), 128}, q.options());
   at::Tensor lse = at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat));
   a.o_ss = o.stride(0); a.o_sh = o.stride(1);
@@ -270,17 +300,20 @@ std::tuple<at::Tensor, at::Tensor> varlen_attention(const at::Tensor& q_, const 
 std::tuple<at::Tensor, at::Tensor, at::Tensor> varlen_attention_backward(
     const at::Tensor& grad_out, const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_, const at::Tensor& out,
     const at::Tensor& lse, const at::Tensor& cu_q, const at::Tensor& cu_k, int64_t max_q, int64_t max_k, bool causal,
-    std::optional<double> scale) {
+    std::optional<double> scale, std::optional<int64_t> window, int64_t sinks) {
+  if (q_.dim() == 3 && empty_window(q_, k_, window))
+    return {at::zeros(q_.sizes(), q_.options()), at::zeros(k_.sizes(), k_.options()), at::zeros(v_.sizes(), v_.options())};
   check_devices("varlen_attention_backward", grad_out, q_, k_, v_, out, lse, cu_q, cu_k);
   at::Tensor q = q_.contiguous(), k = k_.contiguous(), v = v_.contiguous(), go = grad_out.contiguous(), o = out.contiguous(),
              l = lse.contiguous();
   b200_attn_t a{};
-  varlen_desc(a, q, k, v, cu_q, cu_k, max_q, max_k, causal, scale);
+  varlen_desc(a, q, k, v, cu_q, cu_k, max_q, max_k, causal, scale, window, sinks);
   TORCH_CHECK(l.scalar_type() == at::kFloat && l.numel() == q.size(0) * q.size(1), "varlen_attention_backward: lse must be [H, total_q]");
   a.o_ss = o.stride(0); a.o_sh = o.stride(1);
   at::Tensor dq32 = at::empty({q.size(1), q.size(0), 128}, q.options().dtype(at::kFloat));
   at::Tensor delta = at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat));
   at::Tensor gk = at::empty_like(k), gv = at::empty_like(v);
+  const at::Tensor ws = bwd_workspace(a, q);
   const int64_t extra[9] = {0, go.stride(1), go.stride(0), 0, gk.stride(1), gk.stride(0), 0, gv.stride(1), gv.stride(0)};
   DeviceSwitch sw(q.device().index());
   int e = b200_flash_attn_bwd(&a, dq32.data_ptr<float>(), gk.mutable_data_ptr(), gv.mutable_data_ptr(),
@@ -292,6 +325,98 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> varlen_attention_backward(
   g_native_bwd_calls.fetch_add(1, std::memory_order_relaxed);
   at::Tensor gq = at::empty_like(q);
   gq.copy_(dq32.transpose(0, 1));       // fp32 [H, total, 128] accumulator -> [total, H, 128] in the input type
+  return {gq, gk, gv};
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Sliding window with sinks over a dense batch: q [B, Sq, H, 128], k / v [B, Sk, Hkv, 128], the layout in which the projections
+// leave them; lse is [B, H, Sq].  The same two kernels, which leave out the blocks of keys that nobody sees.
+// Parity: no counterpart in the reference (its vendor flash kernel takes a causal flag only: reference
+// torch_musa/csrc/aten/ops/attention/mudnn/SDP.cpp:470-673).
+at::Tensor attn_operand(const at::Tensor& t) {
+  bool ok = t.stride(3) == 1 && (reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15) == 0 && t.stride(1) != 0;
+  for (int d = 0; d < 3; ++d) ok = ok && t.stride(d) % 8 == 0 && (t.size(d) == 1 || t.stride(d) != 0);
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+void dense_window_desc(b200_attn_t& a, const char* op, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, int64_t window,
+                       int64_t sinks, std::optional<double> scale) {
+  a.B = (int)q.size(0); a.H = (int)q.size(2); a.Hkv = (int)k.size(2);
+  a.Sq = (int)q.size(1); a.Sk = (int)k.size(1); a.head_dim = 128;
+  a.dtype = kdtype(q.scalar_type());
+  a.causal = 1;
+  a.scale = (float)scale.value_or(1.0 / std::sqrt(128.0));
+  a.q_sb = q.stride(0); a.q_sh = q.stride(2); a.q_ss = q.stride(1);
+  a.k_sb = k.stride(0); a.k_sh = k.stride(2); a.k_ss = k.stride(1);
+  a.v_sb = v.stride(0); a.v_sh = v.stride(2); a.v_ss = v.stride(1);
+  window_desc(a, op, true, window, sinks);
+}
+
+void check_window_operands(const char* op, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v) {
+  TORCH_CHECK(on_device(q), op, ": expected a blackwell tensor, got ", q.device());
+  TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && v.sizes() == k.sizes() && q.size(0) == k.size(0) && q.size(3) == 128 && k.size(3) == 128 &&
+                  k.size(2) > 0 && q.size(2) % k.size(2) == 0, op, ": q [B, Sq, H, 128], k / v [B, Sk, Hkv, 128] with Hkv a divisor of H, got ",
+              q.sizes(), ", ", k.sizes(), " and ", v.sizes());
+  TORCH_CHECK((q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf) && k.scalar_type() == q.scalar_type() &&
+                  v.scalar_type() == q.scalar_type(), op, ": bf16 / fp16 only");
+  for (const at::Tensor* t : {&q, &k})
+    TORCH_CHECK(t->size(0) <= INT_MAX && t->size(1) <= (1 << 30) && t->size(2) <= INT_MAX, op, ": a size of ", t->sizes(), " is not supported");
+}
+
+std::tuple<at::Tensor, at::Tensor> window_attention(const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_, int64_t window,
+                                                    int64_t sinks, std::optional<double> scale) {
+  const char* op = "window_attention";
+  check_window_operands(op, q_, k_, v_);
+  check_devices(op, q_, k_, v_);
+  b200_attn_t a{};
+  window_desc(a, op, true, window, sinks);
+  if (q_.numel() == 0 || k_.numel() == 0)
+    return {at::zeros(q_.sizes(), q_.options()), at::full({q_.size(0), q_.size(2), q_.size(1)}, -INFINITY, q_.options().dtype(at::kFloat))};
+  const at::Tensor q = attn_operand(q_), k = attn_operand(k_), v = attn_operand(v_);
+  at::Tensor o = at::empty(q.sizes(), q.options());
+  at::Tensor lse = at::empty({q.size(0), q.size(2), q.size(1)}, q.options().dtype(at::kFloat));
+  dense_window_desc(a, op, q, k, v, window, sinks, scale);
+  a.o_sb = o.stride(0); a.o_sh = o.stride(2); a.o_ss = o.stride(1);
+  DeviceSwitch sw(q.device().index());
+  const int e = b200_flash_attn_fwd(&a, o.mutable_data_ptr(), lse.data_ptr<float>(), q.const_data_ptr(), k.const_data_ptr(),
+                                    v.const_data_ptr(), current_raw_stream(q));
+  TORCH_CHECK(e != (int)cudaErrorNotSupported, op, ": unsupported sizes or strides");
+  B200_KERNEL_CALL(e);
+  g_native_fwd_calls.fetch_add(1, std::memory_order_relaxed);
+  return {o, lse};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> window_attention_backward(const at::Tensor& grad_out, const at::Tensor& q_, const at::Tensor& k_,
+                                                                         const at::Tensor& v_, const at::Tensor& out, const at::Tensor& lse,
+                                                                         int64_t window, int64_t sinks, std::optional<double> scale) {
+  const char* op = "window_attention_backward";
+  check_window_operands(op, q_, k_, v_);
+  check_devices(op, q_, k_, v_, grad_out, out, lse);
+  TORCH_CHECK(grad_out.sizes() == q_.sizes() && out.sizes() == q_.sizes() && grad_out.scalar_type() == q_.scalar_type() &&
+                  out.scalar_type() == q_.scalar_type() && lse.scalar_type() == at::kFloat && lse.numel() == q_.size(0) * q_.size(1) * q_.size(2),
+              op, ": grad_out and out must be like q, lse float32 [B, H, Sq]");
+  if (q_.numel() == 0 || k_.numel() == 0)
+    return {at::zeros(q_.sizes(), q_.options()), at::zeros(k_.sizes(), k_.options()), at::zeros(v_.sizes(), v_.options())};
+  const at::Tensor q = attn_operand(q_), k = attn_operand(k_), v = attn_operand(v_), go = attn_operand(grad_out), o = attn_operand(out);
+  const at::Tensor l = lse.contiguous();
+  const int64_t B = q.size(0), Sq = q.size(1), H = q.size(2);
+  b200_attn_t a{};
+  dense_window_desc(a, op, q, k, v, window, sinks, scale);
+  a.o_sb = o.stride(0); a.o_sh = o.stride(2); a.o_ss = o.stride(1);
+  at::Tensor dq32 = at::empty({B, H, Sq, 128}, q.options().dtype(at::kFloat));
+  at::Tensor delta = at::empty({B, H, Sq}, q.options().dtype(at::kFloat));
+  at::Tensor gq = at::empty(q.sizes(), q.options()), gk = at::empty(k.sizes(), k.options()), gv = at::empty(v.sizes(), v.options());
+  const at::Tensor ws = bwd_workspace(a, q);
+  const int64_t extra[9] = {go.stride(0), go.stride(2), go.stride(1), gk.stride(0), gk.stride(2), gk.stride(1),
+                            gv.stride(0), gv.stride(2), gv.stride(1)};
+  DeviceSwitch sw(q.device().index());
+  const int e = b200_flash_attn_bwd(&a, dq32.data_ptr<float>(), gk.mutable_data_ptr(), gv.mutable_data_ptr(), delta.data_ptr<float>(),
+                                    q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), o.const_data_ptr(), go.const_data_ptr(),
+                                    l.const_data_ptr<float>(), extra, current_raw_stream(q));
+  TORCH_CHECK(e != (int)cudaErrorNotSupported, op, ": unsupported sizes or strides");
+  B200_KERNEL_CALL(e);
+  g_native_bwd_calls.fetch_add(1, std::memory_order_relaxed);
+  gq.copy_(dq32.transpose(1, 2));       // fp32 [B, H, Sq, 128] sums -> [B, Sq, H, 128] in the input type
   return {gq, gk, gv};
 }
 
@@ -316,13 +441,17 @@ namespace b200 {
 namespace ops {
 
 TORCH_LIBRARY_FRAGMENT(blackwell, m) {
-  m.def("varlen_attention(Tensor q, Tensor k, Tensor v, Tensor cu_seqlens_q, Tensor cu_seqlens_k, int max_seqlen_q, int max_seqlen_k, bool causal=False, float? scale=None) -> (Tensor, Tensor)");
-  m.def("varlen_attention_backward(Tensor grad_out, Tensor q, Tensor k, Tensor v, Tensor out, Tensor lse, Tensor cu_seqlens_q, Tensor cu_seqlens_k, int max_seqlen_q, int max_seqlen_k, bool causal=False, float? scale=None) -> (Tensor, Tensor, Tensor)");
+  m.def("varlen_attention(Tensor q, Tensor k, Tensor v, Tensor cu_seqlens_q, Tensor cu_seqlens_k, int max_seqlen_q, int max_seqlen_k, bool causal=False, float? scale=None, int? window=None, int sinks=0) -> (Tensor, Tensor)");
+  m.def("varlen_attention_backward(Tensor grad_out, Tensor q, Tensor k, Tensor v, Tensor out, Tensor lse, Tensor cu_seqlens_q, Tensor cu_seqlens_k, int max_seqlen_q, int max_seqlen_k, bool causal=False, float? scale=None, int? window=None, int sinks=0) -> (Tensor, Tensor, Tensor)");
+  m.def("window_attention(Tensor q, Tensor k, Tensor v, int window, int sinks=0, float? scale=None) -> (Tensor, Tensor)");
+  m.def("window_attention_backward(Tensor grad_out, Tensor q, Tensor k, Tensor v, Tensor out, Tensor lse, int window, int sinks=0, float? scale=None) -> (Tensor, Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(blackwell, PrivateUse1, m) {
   m.impl("varlen_attention", TORCH_FN(varlen_attention));
   m.impl("varlen_attention_backward", TORCH_FN(varlen_attention_backward));
+  m.impl("window_attention", TORCH_FN(window_attention));
+  m.impl("window_attention_backward", TORCH_FN(window_attention_backward));
 }
 
 TORCH_LIBRARY_IMPL(aten, PrivateUse1, m) {

@@ -1,5 +1,5 @@
-// Flash-attention backward on the 5th-generation tensor cores (head_dim 128, bf16 / fp16, optional causal mask,
-// grouped-query heads).
+// Flash-attention backward on the 5th-generation tensor cores (head_dim 128, bf16 / fp16, optional causal mask or
+// sliding window with sinks, grouped-query heads).
 //
 // One CTA owns one block of 128 keys of one (batch, kv head); K and V stay resident in shared memory, dK and dV
 // accumulate in TMEM over every query block (and every query head of the group) that sees the keys.  Everything is
@@ -66,6 +66,10 @@ struct BwdParams {
   const int* cu_q;
   const int* cu_k;
   int total_q;
+  // kWin: key j is visible when j <= i and (i - j < window or j < sinks)
+  int window, sinks, total_k;
+  int sink_blocks, sink_chunks;   // key blocks with sinks, CTAs that share the query blocks of one of them
+  float* sink_ws;                 // sink_chunks > 1: fp32 [B * Hkv][sink_blocks][sink_chunks][dV, dK][128][128]
 };
 
 // adds a [128 rows x 32 floats] box of shared memory (128B-swizzled) into global memory at (x, y) of the tensor map
@@ -75,7 +79,30 @@ __device__ __forceinline__ void tma_reduce_add_2d(const CUtensorMap* map, const 
                : "memory");
 }
 
-template <typename T>
+// kWin: the queries that see a block of keys are a contiguous range, window + 127 long behind the block's first key, or all that
+// follow when it holds sinks.  A block with sinks meets many more query blocks than the others (at 4096 tokens and a window of
+// 1024: 32 against 9, times the heads of a group), so its range is cut into chunks of about the others' length that CTAs of their
+// own work off; their dV and dK go to fp32 buffers that a small kernel adds up in order.
+// The query blocks [first, end) that see key block kb.
+__device__ __forceinline__ void window_queries(const BwdParams& p, int kb, int Sq, int Sk, int q_blocks, int& first, int& end) {
+  const int k0 = kb * BK;
+  first = min(q_blocks, k0 / BQ);
+  end = k0 < p.sinks ? q_blocks : min(q_blocks, (min(k0 + BK, Sk) - 1 + p.window - 1) / BQ + 1);
+  if (k0 >= Sk || end < first) end = first;
+}
+
+// Rows [rows, 128) of a tile that a copy brought into shared memory become zero (called by a converged warp, before its products
+// read the tile): they belong to another sequence, or to nobody.
+__device__ __forceinline__ void zero_tail(uint8_t* tile, int rows, int lane) {
+  for (int x = rows * 8 + lane; x < 128 * 8; x += 32) {
+    *reinterpret_cast<uint4*>(tile + x * 16) = make_uint4(0, 0, 0, 0);
+    *reinterpret_cast<uint4*>(tile + kTile / 2 + x * 16) = make_uint4(0, 0, 0, 0);
+  }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncwarp();
+}
+
+template <typename T, bool kWin>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 attn_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
                 const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ CUtensorMap tmap_do,
@@ -115,7 +142,16 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // all (batch, head) instances of the earliest key block first: under a causal mask it meets the most query blocks
   const int n_bh = p.B * p.Hkv;
-  const int kb = (int)(blockIdx.x / n_bh);
+  int kb = (int)(blockIdx.x / n_bh), chunk = 0;
+  if constexpr (kWin) {              // kb counts (block with sinks, chunk) pairs first
+    const int pairs = p.sink_blocks * p.sink_chunks;
+    if (kb < pairs) {
+      chunk = kb % p.sink_chunks;
+      kb /= p.sink_chunks;
+    } else {
+      kb -= pairs - p.sink_blocks;
+    }
+  }
   const int bh = (int)(blockIdx.x % n_bh);
   const int b = bh / p.Hkv, hk = bh - b * p.Hkv;
   const int G = p.H / p.Hkv;
@@ -131,9 +167,25 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
     bt = 0;
     q_blocks = (Sq + BQ - 1) / BQ;
   }
-  const int i0 = p.causal ? min(q_blocks, k0 / BQ) : 0;   // first query block that sees these keys
-  const int n_i = k0 < Sk ? q_blocks - i0 : 0;            // a key block past the sequence's end has nothing to do
-  const int n_it = n_i * G;
+  int i0 = p.causal ? min(q_blocks, k0 / BQ) : 0;   // first query block that sees these keys
+  int n_i = k0 < Sk ? q_blocks - i0 : 0;            // a key block past the sequence's end has nothing to do
+  int n_it = n_i * G, h0 = hk * G, istart = 0;
+  bool partial = false;
+  if constexpr (kWin) {
+    int end;
+    window_queries(p, kb, Sq, Sk, q_blocks, i0, end);
+    n_i = end - i0;
+    n_it = n_i * G;
+    if (kb < p.sink_blocks && p.sink_chunks > 1) {     // pairs [chunk * per, (chunk + 1) * per) of this block's
+      partial = true;
+      const int per = (n_it + p.sink_chunks - 1) / p.sink_chunks, from = min(n_it, chunk * per);
+      n_it = min(n_it, from + per) - from;
+      if (n_i > 0) {
+        h0 += from / n_i;
+        istart = from % n_i;
+      }
+    }
+  }
 
   if (threadIdx.x == 0) {
     *abort_flag = 0;
@@ -180,7 +232,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
         tma_load_4d(sK + kTile / 2, &tmap_k, kv_full, 64, koff + k0, hk, bt);
         tma_load_4d(sV, &tmap_v, kv_full, 0, koff + k0, hk, bt);
         tma_load_4d(sV + kTile / 2, &tmap_v, kv_full, 64, koff + k0, hk, bt);
-        int h = hk * G, i = 0;
+        int h = h0, i = istart;
         for (int it = 0; it < n_it; ++it) {
           const int q0 = (i0 + i) * BQ, st = it & 1;
           if (!mbar_wait(&q_empty[st], (uint32_t)(((it >> 1) & 1) ^ 1), abort_flag)) break;
@@ -210,6 +262,16 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
       auto koff16 = [](int kk) { return (uint32_t)(((kk >> 2) * (kTile / 2) + (kk & 3) * 32) >> 4); };   // K-major: two 64-column atoms
       auto mnoff16 = [](int kk) { return (uint32_t)((kk * 2048) >> 4); };                                // MN-major: 16 rows of 128 bytes
       bool ok = n_it > 0 && wait(kv_full, 0) && wait(&q_full[0], 0);
+      // kWin: the rows of the current and the next query block that are the sequence's own (128 or more: all)
+      int mi = istart;
+      auto own_rows = [&]() { return Sq - (i0 + mi) * BQ; };
+      if (kWin && ok && p.cu_q) {
+        if (k0 + BK > Sk) {
+          zero_tail(sK, Sk - k0, lane);
+          zero_tail(sV, Sk - k0, lane);
+        }
+        if (own_rows() < BQ) zero_tail(sQ, own_rows(), lane);
+      }
       if (ok) {
         tc_fence_after();
         if (issuer) {
@@ -221,6 +283,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
       for (int it = 0; it < n_it && ok; ++it) {
         const uint32_t tq = (uint32_t)((it & 1) * (kTile >> 4)), tq_next = (uint32_t)(((it + 1) & 1) * (kTile >> 4));
         if (!wait(do_full, it)) { ok = false; break; }
+        if (kWin && p.cu_q && own_rows() < BQ) zero_tail(sdO, own_rows(), lane);
         if (it > 0 && !wait(dq_drained, it - 1)) { ok = false; break; }
         tc_fence_after();
         if (issuer) {
@@ -239,6 +302,10 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
         }
         if (it + 1 < n_it) {
           if (!wait(&q_full[(it + 1) & 1], (it + 1) >> 1)) { ok = false; break; }
+          if constexpr (kWin) {
+            if (++mi == n_i) mi = 0;
+            if (p.cu_q && own_rows() < BQ) zero_tail(sQ + ((it + 1) & 1) * kTile, own_rows(), lane);
+          }
           tc_fence_after();
           if (issuer) {
 #pragma unroll
@@ -266,7 +333,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
       // ------------------------------------------------------------ lse (log2 domain, negated: an addend of the exponent) and
       // delta (times the softmax scale, negated) of every query block; an lse of -inf switches a row off
       // (read one block ahead, all eight loads in flight at once)
-      int h = hk * G, i = 0;
+      int h = h0, i = istart;
       float l[4], d[4];
       auto fetch = [&]() {
         const int64_t base = p.cu_q ? (int64_t)h * p.total_q + qoff : ((int64_t)b * p.H + h) * p.Sq;
@@ -298,7 +365,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
     const int qw = warp & 3;
     const int r = qw * 32 + lane;                 // query row inside the block = TMEM lane
     const uint32_t addr = tmem_base + ((uint32_t)(qw * 32) << 16) + kColDP;
-    int h = hk * G, i = 0;
+    int h = h0, i = istart;
     for (int it = 0; it < n_it; ++it) {
       const int q0 = (i0 + i) * BQ;
       bool ok = mbar_wait_warp(dq_full, (uint32_t)(it & 1), abort_flag);
@@ -346,16 +413,17 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
     uint8_t* srow = sS + (size_t)wg * (kTile / 2) + (size_t)r * 128;   // this warpgroup's 64 query columns = atom `wg`
     const bool key_off = kj >= Sk;
     const bool block_off = k0 + BK > Sk;
+    const int far = kWin && kj >= p.sinks ? kj + p.window : 0x7fffffff;      // the first query that no longer sees this key
     bool ok = true;
     auto wait_all = [&](uint64_t* bar, uint32_t parity) { return mbar_wait_warp(bar, parity, abort_flag); };
-    int i = 0;
+    int i = istart;
     for (int it = 0; it < n_it; ++it) {
       const uint32_t par = (uint32_t)(it & 1);
       const int st = it & 1, q0 = (i0 + i) * BQ;
       const float4* nlse4 = reinterpret_cast<const float4*>(s_lse + st * 128 + wg * 64);
       const float4* ndlt4 = reinterpret_cast<const float4*>(s_dlt + st * 128 + wg * 64);
-      // only then can a query be older than a key of this block, or a key be past the end
-      const bool masked = (p.causal && q0 < k0 + BK) || block_off;
+      // only then can a query be older than a key of this block, a key be past the end or in front of a window
+      const bool masked = (p.causal && q0 < k0 + BK) || block_off || (kWin && q0 + BQ - k0 > p.window);
       if (!wait_all(&ld_full[st], (uint32_t)((it >> 1) & 1)) || !wait_all(s_full, par)) { ok = false; break; }
       tc_fence_after();
       float pf[64];
@@ -377,8 +445,8 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
               float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
               if constexpr (decltype(mask)::value) {
                 const int qi = q0 + wg * 64 + cc;
-                if (key_off || (p.causal && qi < kj)) p0 = 0.f;
-                if (key_off || (p.causal && qi + 1 < kj)) p1 = 0.f;
+                if (key_off || (p.causal && qi < kj) || (kWin && qi >= far)) p0 = 0.f;
+                if (key_off || (p.causal && qi + 1 < kj) || (kWin && qi + 1 >= far)) p1 = 0.f;
               }
               pf[cc] = p0;
               pf[cc + 1] = p1;
@@ -450,7 +518,14 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
 #pragma unroll
             for (int e = 0; e < 32; ++e) raw[e] = 0u;
           }
-          if (row_ok) {
+          if (kWin && partial) {
+            float* dst = p.sink_ws + ((((int64_t)bh * p.sink_blocks + kb) * p.sink_chunks + chunk) * 2 + which) * (BK * BD) + r * BD + wg * 64 + c * 32;
+            if (n_it > 0) {
+#pragma unroll
+              for (int g4 = 0; g4 < 8; ++g4)
+                *reinterpret_cast<uint4*>(dst + g4 * 4) = make_uint4(raw[g4 * 4], raw[g4 * 4 + 1], raw[g4 * 4 + 2], raw[g4 * 4 + 3]);
+            }
+          } else if (row_ok) {
             T* dst = (which ? dk_row : dv_row) + c * 32;
 #pragma unroll
             for (int g8 = 0; g8 < 4; ++g8) {
@@ -460,6 +535,18 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
               st16(dst + g8 * 8, v);
             }
           }
+        }
+      }
+    }
+    if constexpr (kWin) {
+      if (p.cu_q && b == p.B - 1 && chunk == 0) {       // packed rows past the last sequence: the CTAs of a head share them
+        Vec16<T> zero;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) zero.v[e] = ToF<T>::from(0.f);
+        for (int x = kb * 16 + (threadIdx.x >> 4); x < p.total_k - (koff + Sk); x += p.kv_blocks * 16) {
+          const int64_t row = koff + Sk + x;
+          st16(dk + (int64_t)hk * p.dk_sh + row * p.dk_ss + (threadIdx.x & 15) * 8, zero);
+          st16(dv + (int64_t)hk * p.dv_sh + row * p.dv_ss + (threadIdx.x & 15) * 8, zero);
         }
       }
     }
@@ -538,6 +625,48 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(const T* __restrict__ o
   }
 }
 
+// dV and dK of the blocks with sinks: the chunks' sums, added in order (the same for every run) and rounded once.  A thread owns
+// eight dimensions of a row.
+template <typename T>
+__global__ void __launch_bounds__(256) attn_sink_sum_kernel(T* __restrict__ dk, T* __restrict__ dv, const BwdParams p) {
+  const int which = blockIdx.y, r = (int)(blockIdx.x % 8) * 16 + (threadIdx.x >> 4), c = (threadIdx.x & 15) * 8;
+  const int unit = (int)(blockIdx.x / 8), kb = unit % p.sink_blocks, bh = unit / p.sink_blocks;
+  const int b = bh / p.Hkv, hk = bh - b * p.Hkv, kj = kb * BK + r;
+  int Sq = p.Sq, Sk = p.Sk, koff = 0, bt = b, q_blocks = p.q_blocks;
+  if (p.cu_q) {
+    Sq = p.cu_q[b + 1] - p.cu_q[b];
+    koff = p.cu_k[b];
+    Sk = p.cu_k[b + 1] - koff;
+    bt = 0;
+    q_blocks = (Sq + BQ - 1) / BQ;
+  }
+  if (kj >= Sk) return;
+  int first, end;
+  window_queries(p, kb, Sq, Sk, q_blocks, first, end);
+  const int n_it = (end - first) * (p.H / p.Hkv), per = (n_it + p.sink_chunks - 1) / p.sink_chunks;
+  float s[8] = {};
+  const float* src = p.sink_ws + (((int64_t)unit * p.sink_chunks) * 2 + which) * (BK * BD) + r * BD + c;
+  for (int ch = 0; ch * per < n_it; ++ch, src += 2 * BK * BD) {
+    const float4 x = *reinterpret_cast<const float4*>(src), y = *reinterpret_cast<const float4*>(src + 4);
+    s[0] += x.x; s[1] += x.y; s[2] += x.z; s[3] += x.w;
+    s[4] += y.x; s[5] += y.y; s[6] += y.z; s[7] += y.w;
+  }
+  Vec16<T> o;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) o.v[e] = ToF<T>::from(s[e]);
+  if (which) st16(dk + (int64_t)bt * p.dk_sb + (int64_t)hk * p.dk_sh + (int64_t)(koff + kj) * p.dk_ss + c, o);
+  else st16(dv + (int64_t)bt * p.dv_sb + (int64_t)hk * p.dv_sh + (int64_t)(koff + kj) * p.dv_ss + c, o);
+}
+
+// How many CTAs share the query blocks of a key block with sinks: as many as make their ranges about as long as the others'.
+int sink_chunks(const b200_attn_t* a) {
+  if (a->window <= 0 || a->sinks <= 0) return 1;
+  const int q_blocks = (a->Sq + BQ - 1) / BQ;
+  const int others = std::min<long long>(q_blocks, (a->window + BK - 2ll) / BQ + 1);
+  return std::max(1, std::min(64, (q_blocks + others - 1) / std::max(1, others)));
+}
+int sink_blocks(const b200_attn_t* a) { return a->window > 0 ? (std::min(a->sinks, a->Sk) + BK - 1) / BK : 0; }
+
 template <typename K>
 int bwd_setup(K kern) {
   cudaFuncAttributes at;
@@ -551,6 +680,11 @@ int bwd_setup(K kern) {
 }  // namespace b200k
 
 using namespace b200k;
+
+extern "C" int64_t b200_flash_attn_bwd_workspace(const b200_attn_t* a) {
+  const int chunks = sink_chunks(a);
+  return chunks > 1 ? (int64_t)a->B * a->Hkv * sink_blocks(a) * chunks * 2 * BK * BD : 0;
+}
 
 extern "C" int b200_flash_attn_bwd(const b200_attn_t* a, float* dq_accum, void* dk, void* dv, float* delta, const void* q,
                                    const void* k, const void* v, const void* o, const void* d_o, const float* lse,
@@ -608,24 +742,35 @@ extern "C" int b200_flash_attn_bwd(const b200_attn_t* a, float* dq_accum, void* 
   p.cu_q = a->cu_seqlens_q;
   p.cu_k = a->cu_seqlens_k;
   p.total_q = a->total_q;
-  const long long grid = (long long)a->B * a->Hkv * p.kv_blocks;
+  p.window = a->window;
+  p.sinks = a->sinks;
+  p.total_k = a->total_k;
+  p.sink_blocks = sink_blocks(a);
+  p.sink_chunks = sink_chunks(a);
+  p.sink_ws = a->workspace;
+  if (a->window > 0 && (!a->causal || a->window > (1 << 30) || a->sinks < 0 || (p.sink_chunks > 1 && !p.sink_ws)))
+    return (int)cudaErrorNotSupported;
+  const long long grid = (long long)a->B * a->Hkv * (p.kv_blocks + p.sink_blocks * (p.sink_chunks - 1));
   if (grid > 2147483647ll || rows / 8 + 1 > 2147483647ll) return (int)cudaErrorNotSupported;
   const int row_blocks = (dS + kDeltaRows - 1) / kDeltaRows;
   const unsigned delta_grid = (unsigned)((long long)dB * a->H * row_blocks);
-  if (bf16) {
-    static OncePerDevice once;
-    if (int e = once([] { return bwd_setup(attn_bwd_kernel<__nv_bfloat16>); })) return e;
-    attn_delta_kernel<__nv_bfloat16><<<delta_grid, 256, 0, stream>>>((const __nv_bfloat16*)o, (const __nv_bfloat16*)d_o, delta, dq_accum,
-                                                                     a->H, dS, row_blocks, a->o_sb, a->o_sh, a->o_ss, x[0], x[1], x[2]);
-    attn_bwd_kernel<__nv_bfloat16><<<(unsigned)grid, kBwdThreads, kBwdSmem, stream>>>(mq, mk, mv, mdo, mdq, (__nv_bfloat16*)dk,
-                                                                                     (__nv_bfloat16*)dv, p);
-  } else {
-    static OncePerDevice once;
-    if (int e = once([] { return bwd_setup(attn_bwd_kernel<__half>); })) return e;
-    attn_delta_kernel<__half><<<delta_grid, 256, 0, stream>>>((const __half*)o, (const __half*)d_o, delta, dq_accum, a->H, dS, row_blocks,
-                                                              a->o_sb, a->o_sh, a->o_ss, x[0], x[1], x[2]);
-    attn_bwd_kernel<__half><<<(unsigned)grid, kBwdThreads, kBwdSmem, stream>>>(mq, mk, mv, mdo, mdq, (__half*)dk, (__half*)dv, p);
-  }
-  note_launch(2);
-  return (int)cudaGetLastError();
+  auto launch = [&](auto kern, OncePerDevice& once, auto* gk, auto* gv) -> int {
+    using T = std::remove_pointer_t<decltype(gk)>;
+    if (int e = once([&] { return bwd_setup(kern); })) return e;
+    attn_delta_kernel<T><<<delta_grid, 256, 0, stream>>>((const T*)o, (const T*)d_o, delta, dq_accum, a->H, dS, row_blocks, a->o_sb, a->o_sh,
+                                                         a->o_ss, x[0], x[1], x[2]);
+    kern<<<(unsigned)grid, kBwdThreads, kBwdSmem, stream>>>(mq, mk, mv, mdo, mdq, gk, gv, p);
+    note_launch(2);
+    if (p.sink_blocks > 0 && p.sink_chunks > 1) {
+      attn_sink_sum_kernel<T><<<dim3((unsigned)(a->B * a->Hkv * p.sink_blocks * 8), 2), 256, 0, stream>>>(gk, gv, p);
+      note_launch();
+    }
+    return (int)cudaGetLastError();
+  };
+  static OncePerDevice once[4];
+  if (a->window > 0)
+    return bf16 ? launch(attn_bwd_kernel<__nv_bfloat16, true>, once[2], (__nv_bfloat16*)dk, (__nv_bfloat16*)dv)
+                : launch(attn_bwd_kernel<__half, true>, once[3], (__half*)dk, (__half*)dv);
+  return bf16 ? launch(attn_bwd_kernel<__nv_bfloat16, false>, once[0], (__nv_bfloat16*)dk, (__nv_bfloat16*)dv)
+              : launch(attn_bwd_kernel<__half, false>, once[1], (__half*)dk, (__half*)dv);
 }

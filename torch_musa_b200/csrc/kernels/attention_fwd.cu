@@ -1,5 +1,5 @@
-// Flash-attention forward on the 5th-generation tensor cores (head_dim 128, bf16 / fp16, optional causal mask,
-// grouped-query heads): two query tiles per CTA in ping-pong, scores and the output accumulators in TMEM, K / V through
+// Flash-attention forward on the 5th-generation tensor cores (head_dim 128, bf16 / fp16, optional causal mask or sliding
+// window with sinks, grouped-query heads): two query tiles per CTA in ping-pong, scores and the output accumulators in TMEM, K / V through
 // a TMA ring, every mbarrier wait bounded (status word as for the GEMMs).  The kernel comment below has the pipeline.
 //
 // Parity: the reference calls a closed vendor flash kernel (reference torch_musa/csrc/aten/ops/attention/mudnn/SDP.cpp:470-673).
@@ -37,6 +37,7 @@ struct AttnParams {
   const int* cu_k;
   int total_q;
   int* status;
+  int window, sinks;          // kWin: key j is visible when j <= i and (i - j < window or j < sinks)
 };
 
 // One CTA owns two adjacent 128-row query tiles of one (batch, head).  Per block of 128 keys and per tile t:
@@ -60,7 +61,13 @@ struct AttnParams {
 // after the first blocks, so O normally never leaves TMEM until the epilogue.
 // The MMA warp alternates between the tiles (P V and next S of tile 0, then of tile 1), so one tile's softmax runs while
 // the tensor core works for the other; K and V tiles stream through a five-slot TMA ring.
-template <typename T>
+//
+// kWin (sliding window of W keys and s sinks): the blocks without a visible key are left out.  The list of blocks that the two
+// tiles share is, in this order: the blocks that only tile 0's window reaches (one, or none), the blocks of the sinks, the
+// rest of tile 1's window.  So tile 0 takes a prefix of the list and tile 1 a suffix, and every block is loaded once.  Packed
+// rows of the next sequence, or of nobody, are set to zero in the last block of V: their probability is zero, but zero times
+// what lies there need not be.
+template <typename T, bool kWin>
 __global__ void __launch_bounds__(kAttnThreads, 1)
 attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
                 const __grid_constant__ CUtensorMap tmap_v, T* __restrict__ out, const AttnParams p) {
@@ -102,6 +109,27 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
     if (p.causal) k_end = min(Sk, q0 + AQ);
     nb[t] = q0 < Sq ? (k_end + AK - 1) / AK : 0;
   }
+  // kWin: the shared list of blocks is [lo0, lo0 + n_pre), then the sinks' [0, n_sink), then [lo1, ...); tile t takes its
+  // items [first_of(t), nb[t])
+  int second_first = 0, lo0 = 0, lo1 = 0, n_pre = 0, n_sink = 0;
+  if constexpr (kWin) {
+    const int sb = (min(p.sinks, Sk) + AK - 1) / AK, q0 = 2 * qp * AQ;
+    const bool second = q0 + AQ < Sq;
+    lo0 = max(max(0, q0 - p.window + 1) / AK, sb);
+    lo1 = second ? max(max(0, q0 + AQ - p.window + 1) / AK, sb) : lo0;
+    const int end0 = nb[0], end1 = nb[1];
+    n_pre = max(0, min(lo1, end0) - lo0);
+    n_sink = min(sb, max(end0, end1));
+    nb[0] = n_pre + min(sb, end0) + max(0, end0 - lo1);
+    nb[1] = second ? n_pre + n_sink + max(0, end1 - lo1) : 0;
+    if (nb[1] == n_pre) nb[1] = 0;      // no key at all
+    second_first = nb[1] > 0 ? n_pre : 0;
+  }
+  auto first_of = [&](int t) { return kWin && t == 1 ? second_first : 0; };
+  auto block_of = [&](int j) {
+    if constexpr (!kWin) return j;
+    else return j < n_pre ? lo0 + j : (j - n_pre < n_sink ? j - n_pre : lo1 + (j - n_pre - n_sink));
+  };
   const int nbmax = max(nb[0], nb[1]);
 
   if (threadIdx.x == 0) {
@@ -146,7 +174,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
           const int st = n % kRing;
           if (!mbar_wait(&r_empty[st], (uint32_t)(((n / kRing) & 1) ^ 1), abort_flag)) break;
           mbar_expect_tx(&r_full[st], kTile);
-          const int k0 = (n >> 1) * AK;
+          const int k0 = block_of(n >> 1) * AK;
           const CUtensorMap* map = (n & 1) ? &tmap_v : &tmap_k;   // V is read as an MN-major B operand: same boxes
           tma_load_4d(sR + st * kTile, map, &r_full[st], 0, koff + k0, hk, bt);
           tma_load_4d(sR + st * kTile + kTile / 2, map, &r_full[st], 64, koff + k0, hk, bt);
@@ -190,7 +218,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
         tc_fence_after();
         if (leader) {
           for (int t = 0; t < 2; ++t)
-            if (nb[t] > 0) {
+            if (nb[t] > 0 && first_of(t) == 0) {
               issue_s(t, 0);
               umma_commit(&mma_done[t]);
             }
@@ -201,16 +229,38 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
         const int nv = 2 * j + 1, nk = 2 * j + 2;
         if (!ring_wait(nv)) { ok = false; break; }
         if (j + 1 < nbmax && !ring_wait(nk)) { ok = false; break; }
+        if constexpr (kWin) {
+          const int rows = Sk - block_of(j) * AK;      // of this block that are the sequence's own
+          if (p.cu_q && rows < AK) {
+            uint8_t* tile = sR + (nv % kRing) * kTile;
+            for (int x = rows * 8 + lane; x < AK * 8; x += 32) {
+              *reinterpret_cast<uint4*>(tile + x * 16) = make_uint4(0, 0, 0, 0);
+              *reinterpret_cast<uint4*>(tile + kTile / 2 + x * 16) = make_uint4(0, 0, 0, 0);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+          }
+        }
         for (int t = 0; t < 2; ++t) {
+          const int j0 = first_of(t);
+          const bool next = j + 1 < nb[t] && j + 1 >= j0;
           if (j >= nb[t]) continue;
-          if (!wait(&p_ready[2 * t], (uint32_t)(j & 1))) { ok = false; break; }
+          if (j < j0) {
+            if (next && leader) {
+              issue_s(t, nk);
+              umma_commit(&mma_done[t]);
+            }
+            continue;
+          }
+          const uint32_t par = (uint32_t)((j - j0) & 1);
+          if (!wait(&p_ready[2 * t], par)) { ok = false; break; }
           tc_fence_after();
-          if (leader) issue_pv(t, nv, j == 0, 0, kFirstPart / 16);
-          if (!wait(&p_ready[2 * t + 1], (uint32_t)(j & 1))) { ok = false; break; }
+          if (leader) issue_pv(t, nv, j == j0, 0, kFirstPart / 16);
+          if (!wait(&p_ready[2 * t + 1], par)) { ok = false; break; }
           tc_fence_after();
           if (leader) {
             issue_pv(t, nv, false, kFirstPart / 16, AK / 16);
-            if (j + 1 < nb[t]) issue_s(t, nk);     // over P of block j: the tensor core works in issue order
+            if (next) issue_s(t, nk);              // over P of block j: the tensor core works in issue order
             umma_commit(&mma_done[t]);
           }
         }
@@ -235,7 +285,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
     float m_ref = -INFINITY;                 // maximum the exponents refer to (raised lazily)
     float l_run = 0.f;
     bool ok = true;
-    const int n_blocks = nb[t];
+    const int n_blocks = nb[t] - first_of(t);
     // warp-uniform wait: the warp-collective TMEM accesses and votes below need all 32 lanes to take the same path
     auto wait_all = [&](uint64_t* bar, uint32_t parity) {
       const bool w = mbar_wait(bar, parity, abort_flag);
@@ -244,12 +294,14 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
     for (int j = 0; j < n_blocks; ++j) {
       if (!wait_all(&mma_done[t], (uint32_t)(j & 1))) { ok = false; break; }
       tc_fence_after();
-      const int k0 = j * AK;
-      // the row's visible keys: [0, lim)
+      const int k0 = block_of(j + first_of(t)) * AK;
+      // the row's visible keys: [0, lim), without [hide0, hide1) in front of the window
       int lim = Sk - k0;
       if (p.causal) lim = min(lim, qi - k0 + 1);
       lim = max(0, min(lim, AK));
-      const bool full = __all_sync(0xffffffffu, lim == AK);
+      const int hide0 = kWin ? max(0, p.sinks - k0) : 0, hide1 = kWin ? qi - p.window + 1 - k0 : 0;
+      const bool full = __all_sync(0xffffffffu, lim == AK && hide0 >= hide1);
+      auto hidden = [&](int e) { return e >= lim || (kWin && e >= hide0 && e < hide1); };
       // the whole row of scores in registers
       uint32_t raw[4][32];
 #pragma unroll
@@ -267,8 +319,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
           fma2(x0, x1, __uint_as_float(raw[c][e]), __uint_as_float(raw[c][e + 1]), p.scale_log2, neg_m);
           float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
           if constexpr (decltype(masked)::value) {
-            if (c * 32 + e >= lim) p0 = 0.f;
-            if (c * 32 + e + 1 >= lim) p1 = 0.f;
+            if (hidden(c * 32 + e)) p0 = 0.f;
+            if (hidden(c * 32 + e + 1)) p1 = 0.f;
           }
           add2(l0, l1, p0, p1);
           pk[c][e >> 1] = pack2<T>(p0, p1);
@@ -289,8 +341,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
           for (int e = 0; e < 32; e += 2) {
             float a = __uint_as_float(raw[c][e]), b2 = __uint_as_float(raw[c][e + 1]);
             if constexpr (decltype(masked)::value) {
-              if (c * 32 + e >= lim) a = -INFINITY;
-              if (c * 32 + e + 1 >= lim) b2 = -INFINITY;
+              if (hidden(c * 32 + e)) a = -INFINITY;
+              if (hidden(c * 32 + e + 1)) b2 = -INFINITY;
             }
             mx[(e >> 1) & 3] = max3(mx[(e >> 1) & 3], a, b2);
           }
@@ -363,6 +415,21 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
       if (qi < Sq && p.lse)
         p.lse[p.cu_q ? (int64_t)h * p.total_q + qoff + qi : ((int64_t)b * p.H + h) * p.Sq + qi] = l_run > 0.f ? (m_ref + log2f(l_run)) * 0.6931471805599453f : -INFINITY;
     }
+    if constexpr (kWin) {
+      Vec16<T> zero;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) zero.v[e] = ToF<T>::from(0.f);
+      if (n_blocks == 0 && qi < Sq) {                  // a query that sees no key
+        T* orow = out + (int64_t)bt * p.o_sb + (int64_t)h * p.o_sh + (int64_t)(qoff + qi) * p.o_ss;
+        for (int c = 0; c < AD; c += 8) st16(orow + c, zero);
+        if (p.lse) p.lse[p.cu_q ? (int64_t)h * p.total_q + qoff + qi : ((int64_t)b * p.H + h) * p.Sq + qi] = -INFINITY;
+      }
+      if (p.cu_q && b == p.B - 1)                      // packed rows past the last sequence: the CTAs of a head share them
+        for (int x = qp * 16 + (threadIdx.x >> 4); x < p.total_q - (qoff + Sq); x += p.q_pairs * 16) {
+          st16(out + (int64_t)h * p.o_sh + (int64_t)(qoff + Sq + x) * p.o_ss + (threadIdx.x & 15) * 8, zero);
+          if (p.lse && (threadIdx.x & 15) == 0) p.lse[(int64_t)h * p.total_q + qoff + Sq + x] = -INFINITY;
+        }
+    }
   }
 
   tc_fence_before();
@@ -432,14 +499,19 @@ extern "C" int b200_flash_attn_fwd(const b200_attn_t* a, void* out, float* lse, 
   p.status = gemm_status_word_device();
   const long long grid = (long long)a->B * a->H * p.q_pairs;
   if (grid > 2147483647ll) return (int)cudaErrorNotSupported;
-  if (bf16) {
-    static OncePerDevice once;
-    if (int e = once([] { return fwd_setup(attn_fwd_kernel<__nv_bfloat16>); })) return e;
-    attn_fwd_kernel<__nv_bfloat16><<<(unsigned)grid, kAttnThreads, kAttnSmem, stream>>>(mq, mk, mv, (__nv_bfloat16*)out, p);
-  } else {
-    static OncePerDevice once;
-    if (int e = once([] { return fwd_setup(attn_fwd_kernel<__half>); })) return e;
-    attn_fwd_kernel<__half><<<(unsigned)grid, kAttnThreads, kAttnSmem, stream>>>(mq, mk, mv, (__half*)out, p);
+  p.window = a->window;
+  p.sinks = a->sinks;
+  auto launch = [&](auto kern, OncePerDevice& once, auto* o) -> int {
+    if (int e = once([&] { return fwd_setup(kern); })) return e;
+    kern<<<(unsigned)grid, kAttnThreads, kAttnSmem, stream>>>(mq, mk, mv, o, p);
+    B200K_LAUNCH_RET();
+  };
+  static OncePerDevice once[4];
+  if (a->window > 0) {
+    if (!a->causal || a->window > (1 << 30) || a->sinks < 0) return (int)cudaErrorNotSupported;
+    return bf16 ? launch(attn_fwd_kernel<__nv_bfloat16, true>, once[2], (__nv_bfloat16*)out)
+                : launch(attn_fwd_kernel<__half, true>, once[3], (__half*)out);
   }
-  B200K_LAUNCH_RET();
+  return bf16 ? launch(attn_fwd_kernel<__nv_bfloat16, false>, once[0], (__nv_bfloat16*)out)
+              : launch(attn_fwd_kernel<__half, false>, once[1], (__half*)out);
 }

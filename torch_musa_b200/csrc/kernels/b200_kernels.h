@@ -556,7 +556,13 @@ typedef struct {
   const int* cu_seqlens_q;
   const int* cu_seqlens_k;
   int total_q, total_k;
+  /* window > 0 (with causal): key j is visible to query i when j <= i and (i - j < window or j < sinks), positions inside the
+   * sequence.  0: no window. */
+  int window, sinks;
+  /* backward with a window: b200_flash_attn_bwd_workspace(desc) floats of scratch (may be NULL when that is 0) */
+  float* workspace;
 } b200_attn_t;
+B200_API int64_t b200_flash_attn_bwd_workspace(const b200_attn_t* desc);
 B200_API int b200_flash_attn_fwd(const b200_attn_t* desc, void* out, float* lse, const void* q, const void* k,
                                  const void* v, cudaStream_t stream);
 /* Backward of the same attention.  dq_accum [B, H, Sq, 128] fp32 (the call zeroes it; the caller converts it),
@@ -579,6 +585,43 @@ B200_API int b200_decode_attention(int dtype, void* out, const void* q, const vo
 B200_API int b200_decode_rope_cache(int dtype, void* q_out, const void* q, const void* k, const void* v, const int64_t* strides,
                                     const float* cosv, const float* sinv, const long long* pos, void* k_cache, void* v_cache,
                                     int B, int H, int Hkv, int max_len, int head_dim, int table_len, cudaStream_t stream);
+
+/* Attention of the n newest tokens of each sequence over a paged cache.  q [B, n, H, D] (strides q_*), out contiguous; pools
+ * k_pages / v_pages [num_pages, Hkv, page_size, D] with element strides for page, head and row (multiples of 8, rows contiguous
+ * and 16-byte aligned); block_table int32 [B, table_width], seq_lens int32 [B]: tokens of a sequence in the cache, the newest
+ * included.  Token i stands at position len - n + i and sees key j when j <= its position and, with window > 0, its position
+ * minus j < window or j < sinks.  Keys on a page number outside the pool are hidden and noted in *status (may be NULL); a
+ * token that sees no key gets zeros.  D is 64 or 128, page_size a multiple of 16. */
+typedef struct {
+  int dtype, head_dim;
+  int B, n, H, Hkv;
+  int num_pages, page_size, table_width;
+  int window, sinks;
+  float scale;
+  int64_t q_sb, q_sn, q_sh, k_sp, k_sh, k_sr, v_sp, v_sh, v_sr, table_sb;
+} b200_paged_attn_t;
+B200_API int b200_paged_attention(const b200_paged_attn_t* desc, void* out, const void* q, const void* k_pages, const void* v_pages,
+                                  const int* block_table, const int* seq_lens, int* status, cudaStream_t stream);
+
+/* Rotary embedding of T new tokens and their cache update in one launch: q_out [T, H, D] = rope(q); rope(k) and v go to the rows of
+ * the cache that the tokens' positions name (as above).  Tokens are packed sequence after sequence: T / B each, or
+ * cu_seqlens (int32 [B + 1]) when it is not NULL.  Tokens past the last sequence or before position 0 are padding: q_out is zero
+ * there and nothing is written.  cos / sin float [table_len, D / 2], rotate-half layout. */
+typedef struct {
+  int dtype, head_dim;
+  int T, B, H, Hkv;
+  int num_pages, page_size, table_width, table_len;
+  int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh, kp_sp, kp_sh, kp_sr, vp_sp, vp_sh, vp_sr, table_sb;
+} b200_paged_write_t;
+B200_API int b200_paged_rope_cache(const b200_paged_write_t* desc, void* q_out, const void* q, const void* k, const void* v,
+                                   const float* cosv, const float* sinv, void* k_pages, void* v_pages, const int* block_table,
+                                   const int* seq_lens, const int* cu_seqlens, int* status, cudaStream_t stream);
+
+/* Verification of n drafted tokens per sequence against target probabilities [B, n + 1, V] with given random numbers [B, n + 1]:
+ * taken [B], out [B, n + 1] (taken drafts, one sampled token, then -1).  draft [B, n, V] may be NULL (certain drafts).  strides:
+ * target sequence and position, draft sequence and position, tokens sequence, random numbers sequence (elements). */
+B200_API int b200_verify_drafts(int dtype, int64_t* taken, int64_t* out, const void* target, const void* draft, const int64_t* tokens,
+                                const float* uniforms, int B, int n, int V, const int64_t* strides, cudaStream_t stream);
 
 /* ---------------------------------------------------------------- expert-parallel MoE token exchange (bf16 rows)
  * E experts, E / world per rank in rank order; idx / slot / pos are int32 [T*K]; receive buffers hold cap_rows

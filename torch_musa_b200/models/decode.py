@@ -58,6 +58,8 @@ class LlamaDecoder:
     def __init__(self, model: Llama, batch: int, max_len: int, device=None, dtype: Optional[torch.dtype] = None,
                  tp_group=None):
         cfg = model.cfg
+        if cfg.window is not None:
+            raise ValueError("LlamaDecoder attends to its whole cache: a model with a window decodes with PagedLlamaDecoder")
         self.model, self.cfg, self.B, self.max_len = model, cfg, batch, max_len
         self.device = torch.device(device) if device is not None else next(model.parameters()).device
         dt = dtype or next(model.parameters()).dtype

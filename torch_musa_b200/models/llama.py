@@ -31,6 +31,8 @@ class LlamaConfig:
     fused_gate_up: bool = True     # one [2*ffn, dim] GEMM + packed SwiGLU kernel
     fused_qkv: bool = True         # one [(h + 2*kv) * hd, dim] GEMM
     fused_loss: bool = True        # fused cross entropy (no probability tensor)
+    window: Optional[int] = None   # sliding-window attention: a token sees this many keys, itself included ...
+    attention_sinks: int = 0       # ... and this many first ones
 
     @property
     def head_dim(self) -> int:
@@ -49,6 +51,17 @@ def llama_tiny_config(**kw) -> LlamaConfig:
     base = dict(vocab_size=512, dim=256, n_layers=2, n_heads=4, ffn_dim=512, max_seq_len=128)
     base.update(kw)
     return LlamaConfig(**base)
+
+
+def causal_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cfg: LlamaConfig) -> torch.Tensor:
+    """The decoder's attention of q [B, S, H, D] over k / v [B, S, Hkv, D], under the configuration's window if it has one;
+    returns [B, S, H * D]."""
+    B, S = q.shape[:2]
+    if cfg.window is not None:
+        return BF.window_attention(q, k, v, cfg.window, cfg.attention_sinks).reshape(B, S, -1)
+    o = F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), is_causal=True,
+                                       enable_gqa=(k.shape[2] != q.shape[2]))
+    return o.transpose(1, 2).reshape(B, S, -1)
 
 
 class RopeTables:
@@ -90,9 +103,7 @@ class Attention(nn.Module):
             v = self.wv(x).view(B, S, -1, hd)
         q = BF.rope(q, cos, sin, positions)
         k = BF.rope(k, cos, sin, positions)
-        o = F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), is_causal=True,
-                                           enable_gqa=(kv != h))
-        return self.wo(o.transpose(1, 2).reshape(B, S, -1))
+        return self.wo(causal_attention(q, k, v, cfg))
 
 
 class FeedForward(nn.Module):
@@ -189,8 +200,12 @@ class Llama(nn.Module):
         return sum(p.numel() for p in self.parameters())
 
     def flops_per_token(self, seq_len: int) -> float:
-        """Training FLOPs per token (fwd + bwd = 3x fwd), attention counted causally."""
+        """Training FLOPs per token (fwd + bwd = 3x fwd), attention counted causally, the keys outside a window left out."""
         c = self.cfg
         n = self.num_params() - c.vocab_size * c.dim  # embedding lookup is not a matmul
-        attn = 2 * 2 * c.n_layers * c.dim * seq_len / 2  # QK^T and PV, causal half
+        keys = seq_len / 2                               # the causal half
+        if c.window is not None and c.window < seq_len:
+            reach = c.window + min(c.attention_sinks, seq_len - c.window)      # keys of a late token (its sinks come on top)
+            keys = (c.window * c.window / 2 + (seq_len - c.window) * reach) / seq_len
+        attn = 2 * 2 * c.n_layers * c.dim * keys         # QK^T and PV
         return 3.0 * (2 * n + attn)

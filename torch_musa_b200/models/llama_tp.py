@@ -8,13 +8,12 @@ from typing import Optional
 
 import torch
 import torch.distributed as dist
-import torch.nn.functional as F
 from torch import nn
 
 from ..ops import functional as BF
 from ..parallel import tensor_parallel as TP
 from ..parallel.loss import parallel_fused_cross_entropy
-from .llama import LlamaConfig
+from .llama import LlamaConfig, causal_attention
 
 
 class TPAttention(nn.Module):
@@ -33,9 +32,7 @@ class TPAttention(nn.Module):
         qkv = self.wqkv(x_shard).view(B, S, self.h_l + 2 * self.kv_l, hd)
         q, k, v = qkv.split([self.h_l, self.kv_l, self.kv_l], dim=2)
         q, k = BF.rope(q, cos, sin), BF.rope(k, cos, sin)
-        o = F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), is_causal=True,
-                                           enable_gqa=(self.kv_l != self.h_l))
-        return self.wo(o.transpose(1, 2).reshape(B * S, self.h_l * hd))
+        return self.wo(causal_attention(q, k, v, self.cfg).view(B * S, self.h_l * hd))
 
 
 class TPFeedForward(nn.Module):

@@ -34,6 +34,8 @@ class MoEConfig:
     rope_theta: float = 10000.0
     max_seq_len: int = 4096
     capacity_factor: float = 2.0
+    window: Optional[int] = None   # sliding-window attention, as in LlamaConfig
+    attention_sinks: int = 0
     # benchmark mode: router logits are drawn N(0,1) per token instead of computed, so that expert loads are
     # balanced in expectation whatever the weights are (the router projection stays in the graph with zero weight)
     synthetic_router_logits: bool = False
@@ -41,7 +43,8 @@ class MoEConfig:
     def attention_config(self) -> LlamaConfig:
         return LlamaConfig(vocab_size=self.vocab_size, dim=self.dim, n_layers=self.n_layers, n_heads=self.n_heads,
                            n_kv_heads=self.n_kv_heads, ffn_dim=self.ffn_dim, norm_eps=self.norm_eps,
-                           rope_theta=self.rope_theta, max_seq_len=self.max_seq_len)
+                           rope_theta=self.rope_theta, max_seq_len=self.max_seq_len, window=self.window,
+                           attention_sinks=self.attention_sinks)
 
 
 def moe_tiny_config(**kw) -> MoEConfig:

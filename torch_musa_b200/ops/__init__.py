@@ -21,6 +21,10 @@ from .functional import (  # noqa: F401
     multi_tensor_l2norm,
     scaled_dot_product_attention,
     flash_attn_varlen_func,
+    window_attention,
+    paged_rope_cache,
+    paged_attention,
+    verify_drafts,
 )
 from .modules import RMSNorm, RoPE, SwishGLU, FusedCrossEntropyLoss, BatchNormAct2d  # noqa: F401
 from . import fake  # noqa: F401  (FakeTensor / meta rules for torch.compile)

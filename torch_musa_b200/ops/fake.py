@@ -131,12 +131,13 @@ def _(a, b, counts, mode, out):
 
 
 @_reg("varlen_attention")
-def _(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, causal=False, scale=None):
+def _(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, causal=False, scale=None, window=None, sinks=0):
     return torch.empty_like(q, memory_format=torch.contiguous_format), q.new_empty((q.shape[1], q.shape[0]), dtype=torch.float32)
 
 
 @_reg("varlen_attention_backward")
-def _(grad_out, q, k, v, out, lse, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, causal=False, scale=None):
+def _(grad_out, q, k, v, out, lse, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, causal=False, scale=None,
+      window=None, sinks=0):
     return (torch.empty_like(q, memory_format=torch.contiguous_format), torch.empty_like(k, memory_format=torch.contiguous_format),
             torch.empty_like(v, memory_format=torch.contiguous_format))
 
@@ -154,3 +155,28 @@ def _(dy, x, row_counts):
 @_reg("decode_rope_cache")
 def _(q, k, v, cos, sin, pos, k_cache, v_cache):
     return q.new_empty((q.shape[0], q.shape[-2], q.shape[-1]))
+
+
+@_reg("window_attention")
+def _(q, k, v, window, sinks=0, scale=None):
+    return q.new_empty(q.shape), q.new_empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32)
+
+
+@_reg("window_attention_backward")
+def _(grad_out, q, k, v, out, lse, window, sinks=0, scale=None):
+    return q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+
+
+@_reg("paged_attention")
+def _(q, k_pages, v_pages, block_table, seq_lens, window=None, sinks=0, scale=None):
+    return q.new_empty(q.shape)
+
+
+@_reg("paged_rope_cache")
+def _(q, k, v, cos, sin, k_pages, v_pages, block_table, seq_lens, cu_seqlens=None):
+    return q.new_empty(q.shape)
+
+
+@_reg("verify_drafts")
+def _(target_probs, draft_tokens, uniforms, draft_probs=None):
+    return draft_tokens.new_empty((target_probs.shape[0],)), draft_tokens.new_empty(target_probs.shape[:2])

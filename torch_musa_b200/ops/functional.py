@@ -353,35 +353,97 @@ def scaled_dot_product_attention(q, k, v, attn_mask=None, dropout_p: float = 0.0
                                           scale=scale, enable_gqa=enable_gqa)
 
 
-# ------------------------------------------------------------------------- packed variable-length attention
+# ------------------------------------------------------------------------- windowed and packed variable-length attention
+def _check_window(causal: bool, window: Optional[int], sinks: int) -> None:
+    if sinks < 0:
+        raise ValueError(f"sinks must not be negative, got {sinks}")
+    if window is not None:
+        if window <= 0:
+            raise ValueError(f"window must be positive, got {window}")
+        if not causal:
+            raise ValueError("a window needs causal=True")
+
+
+def _window_mask(sq: int, sk: int, window: Optional[int], sinks: int, device) -> torch.Tensor:
+    """[sq, sk], true where query i sees key j: ``j <= i and (i - j < window or j < sinks)``."""
+    i, j = torch.arange(sq, device=device)[:, None], torch.arange(sk, device=device)[None, :]
+    seen = j <= i
+    return seen if window is None else seen & ((i - j < window) | (j < sinks))
+
+
+def _native_attention(q, k, v) -> bool:
+    return (_on_device(q) and q.shape[-1] == 128 and q.dtype in (torch.bfloat16, torch.float16)
+            and k.dtype == q.dtype and v.dtype == q.dtype)
+
+
+class _WindowAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, window, sinks, scale):
+        out, lse = torch.ops.blackwell.window_attention(q, k, v, window, sinks, scale)
+        ctx.save_for_backward(q, k, v, out, lse)
+        ctx.args = (window, sinks, scale)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_out):
+        dq, dk, dv = torch.ops.blackwell.window_attention_backward(d_out, *ctx.saved_tensors, *ctx.args)
+        return dq, dk, dv, None, None, None
+
+
+def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int, sinks: int = 0,
+                     softmax_scale: Optional[float] = None) -> torch.Tensor:
+    """Causal attention with a sliding window and a few first tokens that stay visible: query i sees key j when
+    ``j <= i and (i - j < window or j < sinks)``.  ``q`` [B, Sq, H, D], ``k`` / ``v`` [B, Sk, Hkv, D] (Hkv divides H);
+    returns [B, Sq, H, D], zeros for a query that sees no key.  On the blackwell device with D = 128 and bf16 / fp16 the
+    tensor-core kernels skip the blocks of keys outside the mask, in both directions (gradients of dq are summed in
+    fp32 in the order in which blocks arrive); otherwise it is ``scaled_dot_product_attention`` with the mask."""
+    _check_window(True, window, sinks)
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3] or k.shape[2] == 0 or q.shape[2] % k.shape[2]:
+        raise ValueError(f"window_attention: q [B, Sq, H, D] and k, v [B, Sk, Hkv, D] with Hkv a divisor of H expected, got "
+                         f"{tuple(q.shape)}, {tuple(k.shape)} and {tuple(v.shape)}")
+    if _native_attention(q, k, v):
+        if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+            return _WindowAttention.apply(q, k, v, int(window), int(sinks), softmax_scale)
+        return torch.ops.blackwell.window_attention(q, k, v, int(window), int(sinks), softmax_scale)[0]
+    rep = q.shape[2] // k.shape[2]
+    kt, vt = k.transpose(1, 2), v.transpose(1, 2)
+    if rep > 1:
+        kt, vt = kt.repeat_interleave(rep, 1), vt.repeat_interleave(rep, 1)
+    mask = _window_mask(q.shape[1], k.shape[1], window, sinks, q.device)
+    return F.scaled_dot_product_attention(q.transpose(1, 2), kt, vt, attn_mask=mask, scale=softmax_scale).transpose(1, 2)
+
+
 class _VarlenAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, cu_q, cu_k, max_q, max_k, causal, scale):
-        out, lse = torch.ops.blackwell.varlen_attention(q, k, v, cu_q, cu_k, max_q, max_k, causal, scale)
+    def forward(ctx, q, k, v, cu_q, cu_k, max_q, max_k, causal, scale, window, sinks):
+        out, lse = torch.ops.blackwell.varlen_attention(q, k, v, cu_q, cu_k, max_q, max_k, causal, scale, window, sinks)
         ctx.save_for_backward(q, k, v, out, lse, cu_q, cu_k)
-        ctx.args = (max_q, max_k, causal, scale)
+        ctx.args = (max_q, max_k, causal, scale, window, sinks)
         return out
 
     @staticmethod
     def backward(ctx, d_out):
         q, k, v, out, lse, cu_q, cu_k = ctx.saved_tensors
         dq, dk, dv = torch.ops.blackwell.varlen_attention_backward(d_out, q, k, v, out, lse, cu_q, cu_k, *ctx.args)
-        return dq, dk, dv, None, None, None, None, None, None
+        return dq, dk, dv, None, None, None, None, None, None, None, None
 
 
 def flash_attn_varlen_func(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens_q: torch.Tensor,
                            cu_seqlens_k: torch.Tensor, max_seqlen_q: int, max_seqlen_k: int,
-                           softmax_scale: Optional[float] = None, causal: bool = False) -> torch.Tensor:
+                           softmax_scale: Optional[float] = None, causal: bool = False,
+                           window: Optional[int] = None, sinks: int = 0) -> torch.Tensor:
     """Attention over sequences of different lengths packed without padding: ``q`` [total_q, H, D], ``k`` / ``v``
     [total_k, Hkv, D]; sequence i owns rows ``cu_seqlens[i]:cu_seqlens[i + 1]`` (int32 prefix sums, on the device of
     the tensors).  Returns [total_q, H, D].  On the blackwell device with D = 128 and bf16 / fp16 the whole batch is
     one launch of the tensor-core forward (one more for the backward) and the lengths are never read on the host;
     otherwise the sequences are processed one by one with ``scaled_dot_product_attention``.  A causal mask compares
-    positions inside a sequence (key index <= query index)."""
-    if (_on_device(q) and q.shape[-1] == 128 and q.dtype in (torch.bfloat16, torch.float16)
-            and k.dtype == q.dtype and v.dtype == q.dtype):
+    positions inside a sequence (key index <= query index); ``window`` and ``sinks`` narrow it as in
+    ``window_attention``, and rows past the last sequence then get zeros, in the gradients too."""
+    _check_window(causal, window, sinks)
+    if _native_attention(q, k, v):
         return _VarlenAttention.apply(q, k, v, cu_seqlens_q.to(torch.int32), cu_seqlens_k.to(torch.int32),
-                                      int(max_seqlen_q), int(max_seqlen_k), bool(causal), softmax_scale)
+                                      int(max_seqlen_q), int(max_seqlen_k), bool(causal), softmax_scale, window, int(sinks))
     cq, ck = cu_seqlens_q.tolist(), cu_seqlens_k.tolist()
     rep = q.shape[1] // k.shape[1]
     outs = []
@@ -391,10 +453,159 @@ def flash_attn_varlen_func(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu
         vi = v[ck[i]:ck[i + 1]].transpose(0, 1).unsqueeze(0)
         if rep > 1:
             ki, vi = ki.repeat_interleave(rep, 1), vi.repeat_interleave(rep, 1)
-        mask = None
-        if causal:
-            sq, sk = qi.shape[2], ki.shape[2]
-            mask = torch.ones(sq, sk, dtype=torch.bool, device=q.device).tril()
+        mask = _window_mask(qi.shape[2], ki.shape[2], window, sinks, q.device) if causal else None
         o = F.scaled_dot_product_attention(qi, ki, vi, attn_mask=mask, scale=softmax_scale)
         outs.append(o.squeeze(0).transpose(0, 1))
+    if window is not None and cq[-1] < q.shape[0]:
+        outs.append(q.new_zeros((q.shape[0] - cq[-1],) + tuple(q.shape[1:])))
     return torch.cat(outs, 0)
+
+
+# ------------------------------------------------------------------------- paged key-value cache
+def _no_grad_inputs(op: str, *tensors) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{op} has no gradient: call it under torch.no_grad()")
+
+
+def _paged_native(q: torch.Tensor) -> bool:
+    return _on_device(q) and q.dtype in (torch.bfloat16, torch.float16) and q.shape[-1] in (64, 128)
+
+
+def paged_rope_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+                     k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                     cu_seqlens: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Rotary embedding (rotate-half layout) of new tokens and their paged cache update, one launch on the device.
+
+    ``q`` [T, H, D], ``k`` / ``v`` [T, Hkv, D] hold the new tokens sequence after sequence: the same number for each, or
+    ``cu_seqlens`` (int32 [B + 1]).  ``k_pages`` / ``v_pages`` [pages, Hkv, page size, D] are written in place;
+    ``block_table`` (int32 [B, W]) names each sequence's pages in order; ``seq_lens`` (int32 [B]) counts the tokens in the
+    cache, the new ones included: token i of n stands at position ``len - n + i``.  ``cos`` / ``sin`` are float32
+    [positions, D / 2].  Returns the rotated queries.  Tokens past the last sequence or before position 0 are padding:
+    zeros come back for them and nothing is written.  A page number outside the pool or a position outside the tables is
+    reported by the next ``synchronize()`` (the row is not written; the last angle is used).  Sequences do not
+    share the pages that they write."""
+    _no_grad_inputs("paged_rope_cache", q, k, v)
+    if _paged_native(q):
+        return torch.ops.blackwell.paged_rope_cache(q, k, v, cos, sin, k_pages, v_pages, block_table, seq_lens, cu_seqlens)
+    T, B, page = q.shape[0], seq_lens.shape[0], k_pages.shape[2]
+    t = torch.arange(T, device=q.device)
+    if cu_seqlens is None:
+        n = T // max(B, 1)
+        if n * B != T:
+            raise RuntimeError(f"paged_rope_cache: {T} tokens do not divide over {B} sequences")
+        cu = torch.arange(B + 1, device=q.device) * n
+    else:
+        cu = cu_seqlens.long()
+    seq = (torch.searchsorted(cu, t, right=True) - 1).clamp(0, max(B - 1, 0))
+    if B == 0:
+        return torch.zeros_like(q)
+    from_end = cu[seq + 1] - t
+    pos = seq_lens.long()[seq] - from_end
+    real = (from_end > 0) & (t >= cu[seq]) & (pos >= 0)
+    index = torch.div(pos.clamp_min(0), page, rounding_mode="floor")
+    inside = index < block_table.shape[1]
+    number = torch.full_like(index, -1) if block_table.shape[1] == 0 else torch.where(
+        inside, block_table.long()[seq, index.clamp_max(block_table.shape[1] - 1)], -1)
+    bad = real & ((number < 0) | (number >= k_pages.shape[0]))
+    late = real & (pos >= cos.shape[0])
+    if not _on_device(q) and bool((bad | late).any()):
+        raise IndexError("paged_rope_cache: a token's page or position does not exist")
+    angle = pos.clamp(0, cos.shape[0] - 1)
+    c, s, half = cos[angle][:, None], sin[angle][:, None], q.shape[-1] // 2
+
+    def rotate(x):
+        a, b = x[..., :half].float(), x[..., half:].float()
+        return torch.cat((a * c - b * s, b * c + a * s), -1).to(x.dtype)
+
+    keep = real & ~bad
+    rows = (number[keep], slice(None), (pos % page)[keep])
+    k_pages[rows] = rotate(k)[keep]
+    v_pages[rows] = v[keep]
+    return rotate(q).masked_fill(~real[:, None, None], 0)
+
+
+def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
+                    seq_lens: torch.Tensor, window: Optional[int] = None, sinks: int = 0,
+                    softmax_scale: Optional[float] = None) -> torch.Tensor:
+    """Attention of the n newest tokens of each sequence (``q`` [B, n, H, D]; n = 1 when decoding, more when drafted tokens
+    are checked) over a paged cache as ``paged_rope_cache`` writes it.  Token i sees the keys up to its own position
+    ``len - n + i``; ``window`` / ``sinks`` narrow that as in ``window_attention``.  Only pages with a visible key are
+    read: others may already belong to someone else, and their table entries may be anything.  A token that sees no key
+    (an empty sequence) gets zeros.  The keys of a page number outside the pool are hidden, which the next ``synchronize()``
+    reports."""
+    _check_window(True, window, sinks)
+    _no_grad_inputs("paged_attention", q, k_pages, v_pages)
+    if _paged_native(q):
+        return torch.ops.blackwell.paged_attention(q, k_pages, v_pages, block_table, seq_lens, window, int(sinks), softmax_scale)
+    B, n, H, D = q.shape
+    pages, Hkv, page, _ = k_pages.shape
+    L = block_table.shape[1] * page
+    if L == 0 or q.numel() == 0:
+        return torch.zeros_like(q)
+    table = block_table.long()
+    j = torch.arange(L, device=q.device)
+    pos = (seq_lens.long().clamp(0, L)[:, None] - n + torch.arange(n, device=q.device))[:, :, None]
+    seen = j <= pos
+    if window is not None:
+        seen = seen & ((pos - j < window) | (j < sinks))
+    there = ((table >= 0) & (table < pages)).repeat_interleave(page, 1)[:, None]
+    if not _on_device(q) and bool((seen & ~there).any()):
+        raise IndexError("paged_attention: a visible key's page does not exist")
+    seen = (seen & there)[:, None, None]                                                        # [B, 1, 1, n, L]
+    some = seen.any(3, keepdim=True).squeeze(3)[..., None]                                      # keys that any token sees
+    index = table.clamp(0, max(pages - 1, 0))
+
+    def rows(pool):
+        x = pool[index] if pages else pool.new_zeros((B, table.shape[1], Hkv, page, D))
+        return x.transpose(1, 2).reshape(B, Hkv, 1, L, D).float().masked_fill(~some, 0)
+
+    scale = softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(D)
+    x = (q.float().view(B, n, Hkv, H // Hkv, D).permute(0, 2, 3, 1, 4) @ rows(k_pages).transpose(-1, -2)) * scale
+    x = x.masked_fill(~seen, float("-inf"))
+    top = x.amax(-1, keepdim=True)
+    x = torch.exp(x - top.masked_fill(top == float("-inf"), 0))
+    out = (x @ rows(v_pages)) / x.sum(-1, keepdim=True).clamp_min(torch.finfo(torch.float32).tiny)
+    return out.permute(0, 3, 1, 2, 4).reshape(B, n, H, D).to(q.dtype)
+
+
+def verify_drafts(target_probs: torch.Tensor, draft_tokens: torch.Tensor, uniforms: torch.Tensor,
+                  draft_probs: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Checks drafted tokens against the target model's probabilities with given random numbers, so that what comes out is
+    distributed as if it were sampled from the target alone.
+
+    ``target_probs`` [B, n + 1, V] (the rows for the n drafted tokens and the one after them), ``draft_tokens`` int64 [B, n],
+    ``uniforms`` float32 [B, n + 1] in [0, 1), ``draft_probs`` [B, n, V] or None for drafts that were certain (a greedy
+    draft).  Draft i is taken while ``uniforms[i] * draft_probs[i, x_i] < target_probs[i, x_i]``; at the first refusal r one
+    token is drawn from ``max(target_probs[r] - draft_probs[r], 0)``, after n taken drafts from ``target_probs[n]``: the first
+    token at which the running sum exceeds ``uniforms[n]`` times the whole.  A draft outside the vocabulary (-1, say) ends a
+    sequence's draft early: the token there is drawn from the target's row.  Sums are held in 64 bits.
+
+    Returns ``(taken [B], tokens [B, n + 1])``, both int64: the taken drafts, the drawn token, then -1.  Where a row has no
+    weight at all (zeros or NaN) the drawn token is -1."""
+    _no_grad_inputs("verify_drafts", target_probs, draft_probs)
+    if _on_device(target_probs) and target_probs.dtype in (torch.float32, torch.bfloat16, torch.float16):
+        return torch.ops.blackwell.verify_drafts(target_probs, draft_tokens, uniforms, draft_probs)
+    B, n1, V = target_probs.shape
+    n, x, u = n1 - 1, draft_tokens, uniforms.double()
+    if tuple(x.shape) != (B, n) or tuple(u.shape) != (B, n1) or (draft_probs is not None and tuple(draft_probs.shape) != (B, n, V)):
+        raise RuntimeError("verify_drafts: draft_tokens [B, n], uniforms [B, n + 1] and draft_probs [B, n, V] expected")
+    known = (x >= 0) & (x < V)
+    at = x.clamp(0, V - 1)[..., None]
+    p = target_probs[:, :n].gather(2, at).squeeze(2).double()
+    q = draft_probs.gather(2, at).squeeze(2).double() if draft_probs is not None else torch.ones_like(p)
+    taken = (known & (u[:, :n] * q < p)).long().cumprod(1).sum(1)
+    row = torch.arange(B, device=x.device)
+    w = target_probs[row, taken].double()
+    if n > 0:
+        stop = taken.clamp_max(n - 1)
+        less = w - draft_probs[row, stop].double() if draft_probs is not None else w.scatter(1, at[row, stop], 0.0)
+        less = torch.where(less > 0, less, 0.0)
+        refused = (taken < n) & known[row, stop] & (less.sum(1) > 0)
+        w = torch.where(refused[:, None], less, w)
+    w = torch.where(w > 0, w, 0.0)
+    total = w.cumsum(1)
+    token = (total > u[:, n:] * total[:, -1:]).long().argmax(1)
+    token = torch.where(total[:, -1] > 0, token, -1)
+    i = torch.arange(n1, device=x.device)
+    drafts = torch.cat((x, x.new_full((B, 1), -1)), 1)
+    return taken, torch.where(i < taken[:, None], drafts, torch.where(i == taken[:, None], token[:, None], -1))
