@@ -8,7 +8,14 @@
 // torch_musa/csrc/aten/ops/attention/mudnn/SDP.cpp).
 #include "common.cuh"
 
+#include <cooperative_groups.h>
+
+#include <algorithm>
+#include <cstdlib>
 #include <initializer_list>
+#include <type_traits>
+
+namespace cg = cooperative_groups;
 
 namespace b200k {
 namespace {
@@ -16,7 +23,9 @@ namespace {
 struct PagedParams {
   int B, n, H, Hkv;
   int num_pages, page_size, table_width;
+  int page_shift;             // log2(page_size), or -1
   int window, sinks;          // window <= 0: every earlier key is visible
+  int row_groups, split;      // CTAs of one (sequence, key head): row groups x shares of the keys
   float scale_log2;
   int64_t q_sb, q_sn, q_sh;                    // element strides; rows of D contiguous elements
   int64_t k_sp, k_sh, k_sr, v_sp, v_sh, v_sr;  // page, head, row in the page
@@ -26,64 +35,403 @@ struct PagedParams {
   int* status;
 };
 
-// The number of the page that holds key j of a sequence, or -1 (and a note for the host) when the table has none.
-__device__ __forceinline__ int page_of(const PagedParams& p, const int* row, int index) {
-  int page = -1;
-  if (index < p.table_width) page = __ldg(row + index);
-  if (page < 0 || page >= p.num_pages) {
-    if (p.status) atomicExch(p.status, 1);
-    page = -1;
-  }
-  return page;
+constexpr int kPagedWarps = 4;
+constexpr int kStepKeys = 16;          // keys of one step of a warp: they lie in one page
+constexpr int kWarpRing = 16 * 1024;   // bytes of keys and values that a warp has in flight or in hand
+constexpr int kMaxSplit = 16;          // CTAs of a cluster
+
+template <int D> constexpr int ring_stages() { return kWarpRing / (kStepKeys * D * 2 * 2); }
+
+__device__ __forceinline__ uint32_t shared_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+// 16 bytes from global to shared memory without a register; zeros when `bytes` is 0
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+// four 8 x 8 matrices of 16-bit values, one row address per lane; _t: transposed
+__device__ __forceinline__ uint4 ldmatrix(uint32_t a) {
+  uint4 r;
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a) : "memory");
+  return r;
+}
+__device__ __forceinline__ uint4 ldmatrix_t(uint32_t a) {
+  uint4 r;
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a) : "memory");
+  return r;
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// (a, b) as 16-bit values, and what that rounding left of them
+template <typename T>
+__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+  T h[2] = {ToF<T>::from(a), ToF<T>::from(b)}, l[2] = {ToF<T>::from(a - ToF<T>::to(h[0])), ToF<T>::from(b - ToF<T>::to(h[1]))};
+  hi = *reinterpret_cast<const uint32_t*>(h);
+  lo = *reinterpret_cast<const uint32_t*>(l);
+}
+// whether one of the two 16-bit values is infinite or NaN: its exponent bits are all set
+template <typename T>
+__device__ __forceinline__ bool not_finite(uint32_t w) {
+  constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+  return (w & e) == e || (w & (e << 16)) == (e << 16);
 }
 
-// One warp per (sequence, new token, query head); its lanes split the D dimensions.  Online softmax in the log2 domain:
-// m' = max(m, s), l' = l 2^(m - m') + 2^(s - m'), o' = o 2^(m - m') + 2^(s - m') v.
-template <typename T, int D>
-__global__ void __launch_bounds__(128) paged_attn_kernel(T* __restrict__ out, const T* __restrict__ q, const T* __restrict__ kp,
-                                                         const T* __restrict__ vp, const PagedParams p) {
-  constexpr int E = D / 32;
-  const long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (w >= (long long)p.B * p.n * p.H) return;
-  const int lane = threadIdx.x & 31;
-  const int h = (int)(w % p.H), i = (int)(w / p.H % p.n), b = (int)(w / p.H / p.n);
-  const int hk = h / (p.H / p.Hkv);
-  const long long cap = (long long)p.table_width * p.page_size;
-  const int len = (int)min((long long)max(p.lens[b], 0), cap);
-  const int pos = len - p.n + i;
-  const int* row = p.table + b * p.table_sb;
-  float qv[E], o[E], m = -INFINITY, l = 0.f;
+// One CTA: one row group (up to 16 * MT rows = new tokens x query heads of a key head) of one (sequence, key head), one of C
+// contiguous shares of the visible keys.  A share is cut into steps of 16 keys that the four warps take in turn; each warp runs its
+// own online softmax, the warps join through shared memory and the C CTAs of a cluster through distributed shared memory.
+//
+// A warp copies the 16 rows of keys and of values of a step into a stage of its own ring (cp.async, whole rows at a time, 16-byte
+// pieces swapped by row so that the eight rows of a matrix lie in different banks) and reads them as operands of mma m16n8k16:
+//   S = Q K^T  (16 rows x 16 keys) with ldmatrix, O += P V (16 rows x D dimensions, 16 keys deep) with ldmatrix.trans.
+// P is S's accumulator layout, and goes in as a 16-bit value plus the 16-bit remainder of its rounding (2^-16 or better).
+template <typename T, int D, int MT>
+__global__ void __launch_bounds__(kPagedWarps * 32, MT == 1 ? 3 : 2) paged_attn_kernel(T* __restrict__ out, const T* __restrict__ q, const T* __restrict__ kp,
+                                                                         const T* __restrict__ vp, const PagedParams p) {
+  constexpr int kRows = 16 * MT, kStages = ring_stages<D>(), kStage = kStepKeys * D * 4;
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ float s_m[kPagedWarps][kRows], s_l[kPagedWarps][kRows];
+  __shared__ float s_top[kRows], s_sum[kRows];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int G = p.H / p.Hkv, rows_all = p.n * G;
+  const int rank = (int)(blockIdx.x % p.split);
+  int unit = (int)(blockIdx.x / p.split);
+  const int group = unit % p.row_groups;
+  unit /= p.row_groups;
+  const int hk = unit % p.Hkv, b = unit / p.Hkv;
+  const int r0 = group * kRows, rows = min(kRows, rows_all - r0);
+  const int len = (int)min((long long)max(__ldg(p.lens + b), 0), (long long)p.table_width * p.page_size);
+  // positions of the oldest and the newest token of the group; the steps of 16 keys that one of them sees
+  const int pos0 = len - p.n + r0 / G, pos1 = len - p.n + (r0 + rows - 1) / G;
+  const int wlo = p.window > 0 ? max(0, pos0 - p.window + 1) : 0;
+  const int end = pos1 >= 0 ? pos1 / kStepKeys + 1 : 0;
+  const int sink_steps = min(end, (p.sinks + kStepKeys - 1) / kStepKeys), first = max(wlo / kStepKeys, sink_steps);
+  const int steps = sink_steps + max(0, end - first);
+  const int s0 = (int)((long long)steps * rank / p.split), s1 = (int)((long long)steps * (rank + 1) / p.split);
+  auto key_of = [&](int s) { return (s < sink_steps ? s : s - sink_steps + first) * kStepKeys; };
+
+  // Q as operands: rows g and g + 8 of each 16, dimensions 16 ks + 2 t and 8 further
+  uint4 qf[D / 16];
+  uint4* sq = reinterpret_cast<uint4*>(smem + kPagedWarps * kWarpRing) + lane;      // MT == 2: [m][ks][lane], they would not fit
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    qv[e] = ToF<T>::to(q[b * p.q_sb + i * p.q_sn + h * p.q_sh + lane * E + e]) * p.scale_log2;
-    o[e] = 0.f;
-  }
-  const int lo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
-  int page = -1, at = -1;
-  for (int j = (p.window > 0 && p.sinks > 0) ? 0 : lo; j <= pos; ++j) {
-    if (j >= p.sinks && j < lo) j = lo;
-    if (j / p.page_size != at) {
-      at = j / p.page_size;
-      page = page_of(p, row, at);
+  for (int m = 0; m < MT; ++m) {
+    if (MT > 1 && warp != m) continue;
+    const T* row[2];
+    bool real[2];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int r = m * 16 + half * 8 + g;
+      real[half] = r < rows;
+      row[half] = q + b * p.q_sb + (r0 + r) / G * p.q_sn + (hk * G + (r0 + r) % G) * p.q_sh + 2 * t;
     }
-    if (page < 0) continue;
-    const int64_t r = j % p.page_size;
-    const T* kr = kp + page * p.k_sp + hk * p.k_sh + r * p.k_sr + lane * E;
-    const T* vr = vp + page * p.v_sp + hk * p.v_sh + r * p.v_sr + lane * E;
-    float s = 0.f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) s = fmaf(qv[e], ToF<T>::to(kr[e]), s);
-    s = warp_sum(s);
-    const float m_new = fmaxf(m, s);
-    const float a = m == -INFINITY ? 0.f : exp2f(m - m_new), x = s == -INFINITY ? 0.f : exp2f(s - m_new);   // a NaN score stays one
-    l = l * a + x;
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = fmaf(x, ToF<T>::to(vr[e]), o[e] * a);
-    m = m_new;
+    for (int ks = 0; ks < D / 16; ++ks) {
+      auto word = [&](int half, int d) { return real[half] ? __ldg(reinterpret_cast<const uint32_t*>(row[half] + d)) : 0u; };
+      const uint4 x = make_uint4(word(0, ks * 16), word(1, ks * 16), word(0, ks * 16 + 8), word(1, ks * 16 + 8));
+      if constexpr (MT == 1) qf[ks] = x;
+      else sq[(m * (D / 16) + ks) * 32] = x;
+    }
   }
-  T* dst = out + w * D + lane * E;
+
+  const uint32_t ring = shared_u32(smem) + warp * kWarpRing;
+  const int* table = p.table + b * p.table_sb;
+  constexpr int kPieces = D / 8, kPerCopy = 32 / kPieces;      // 16-byte pieces of a row, rows that one instruction copies
+  const int crow = lane / kPieces, cpiece = lane % kPieces;
+  const T* kbase = kp + hk * p.k_sh + crow * p.k_sr + cpiece * 8;
+  const T* vbase = vp + hk * p.v_sh + crow * p.v_sr + cpiece * 8;
+  const int mi = lane >> 3, mr = lane & 7;
+  // a lane's row address in a stage for ldmatrix; the piece 2 x of a row is at ((2 x) ^ swap) * 16, for x < 4
+  const uint32_t krow = (uint32_t)(((mi >> 1) * 8 + mr) * D * 2), kswap = (uint32_t)(((mi & 1) ^ mr) * 16);
+  const uint32_t vrow = (uint32_t)(kStepKeys * D * 2 + ((mi & 1) * 8 + mr) * D * 2), vswap = (uint32_t)(((mi >> 1) ^ mr) * 16);
+  auto entry = [&](int s) {          // the page number of a step, read one step before it is needed
+    if (s >= s1) return -1;
+    const int k0 = key_of(s);
+    return __ldg(table + (p.page_shift >= 0 ? k0 >> p.page_shift : k0 / p.page_size));
+  };
+  uint32_t found = 0;                // one bit a stage: whether the page of its step is in the pool
+  auto issue = [&](int s, int number, int stage) {
+    if (s < s1) {
+      const int k0 = key_of(s);
+      const bool there = number >= 0 && number < p.num_pages;
+      if (!there && lane == 0 && p.status) atomicExch(p.status, 1);
+      found = (found & ~(1u << stage)) | ((uint32_t)there << stage);
+      const int64_t row = p.page_shift >= 0 ? k0 & (p.page_size - 1) : k0 % p.page_size, page = there ? number : 0;
+      const T* ks = kbase + page * p.k_sp + row * p.k_sr;
+      const T* vs = vbase + page * p.v_sp + row * p.v_sr;
+      const uint32_t dst = ring + stage * kStage + (uint32_t)(crow * D * 2);
+      // keys that no row sees are not read: zeros instead (with a probability of zero nothing else would be safe)
+      auto copy = [&](auto whole) {
 #pragma unroll
-  for (int e = 0; e < E; ++e) dst[e] = ToF<T>::from(l == 0.f ? 0.f : o[e] / l);
+        for (int i = 0; i < kStepKeys / kPerCopy; ++i) {
+          const int r = i * kPerCopy + crow, j = k0 + r;
+          const int n16 = decltype(whole)::value || (there && j <= pos1 && (j >= wlo || j < p.sinks)) ? 16 : 0;
+          const uint32_t d = dst + (uint32_t)(i * kPerCopy * D * 2) + (uint32_t)((cpiece ^ (r & 7)) * 16);
+          copy16(d, ks + i * kPerCopy * p.k_sr, n16);
+          copy16(d + kStepKeys * D * 2, vs + i * kPerCopy * p.v_sr, n16);
+        }
+      };
+      if (there && k0 + kStepKeys - 1 <= pos1 && (k0 >= wlo || k0 + kStepKeys <= p.sinks)) copy(std::true_type{});
+      else copy(std::false_type{});
+    }
+    copy_commit();
+  };
+
+  float o[MT][D / 8][4], m_run[MT][2], l_run[MT][2];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+#pragma unroll
+    for (int x = 0; x < D / 8; ++x)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[m][x][e] = 0.f;
+    m_run[m][0] = m_run[m][1] = -INFINITY;
+    l_run[m][0] = l_run[m][1] = 0.f;
+  }
+
+  if constexpr (MT > 1) __syncthreads();
+  int s = s0 + warp, fetch = s;
+  int number = entry(fetch);
+#pragma unroll
+  for (int st = 0; st < kStages; ++st) {
+    const int now = number;
+    number = entry(fetch + kPagedWarps);
+    issue(fetch, now, st);
+    fetch += kPagedWarps;
+  }
+  int stage = 0;
+  for (; s < s1; s += kPagedWarps) {
+    copy_wait<kStages - 1>();
+    __syncwarp();
+    const int k0 = key_of(s);
+    const uint32_t src = ring + stage * kStage;
+    float sc[MT][2][4];
+    {
+      float part[MT][2][4];          // odd products: four chains of half the length instead of two
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[m][nt][e] = part[m][nt][e] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
+        const uint4 kf = ldmatrix(src + krow + (((uint32_t)(ks & 3) * 32) ^ kswap) + (uint32_t)(ks >> 2) * 128);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          const uint4 x = MT == 1 ? qf[ks] : sq[(m * (D / 16) + ks) * 32];
+          const uint32_t a[4] = {x.x, x.y, x.z, x.w};
+          mma16816<T>(ks & 1 ? part[m][0] : sc[m][0], a, kf.x, kf.y);
+          mma16816<T>(ks & 1 ? part[m][1] : sc[m][1], a, kf.z, kf.w);
+        }
+      }
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[m][nt][e] += part[m][nt][e];
+    }
+    auto values = [&](int j) {         // the operands of dimensions [8 j, 8 j + 16), j even
+      return ldmatrix_t(src + vrow + (((uint32_t)(j & 7) * 16) ^ vswap) + (uint32_t)(j >> 3) * 128);
+    };
+    const bool there = (found >> stage) & 1u;
+    const bool all = there && k0 + kStepKeys - 1 <= pos0 && (p.window <= 0 || k0 > pos1 - p.window || k0 + kStepKeys <= p.sinks);
+    const bool mixed = !all && pos0 != pos1;
+    auto sees = [&](int pos, int j) { return there && j <= pos && (p.window <= 0 || j > pos - p.window || j < p.sinks); };
+
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      float mx[2];
+      if (!all) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int pos = len - p.n + (r0 + m * 16 + half * 8 + g) / G;
+#pragma unroll
+          for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              if (!sees(pos, k0 + nt * 8 + 2 * t + e)) sc[m][nt][half * 2 + e] = -INFINITY;
+        }
+      }
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        float x = fmaxf(fmaxf(sc[m][0][half * 2], sc[m][0][half * 2 + 1]), fmaxf(sc[m][1][half * 2], sc[m][1][half * 2 + 1]));
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+        mx[half] = x * p.scale_log2;
+      }
+      if (__any_sync(0xffffffffu, mx[0] > m_run[m][0] || mx[1] > m_run[m][1])) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const float m_new = fmaxf(m_run[m][half], mx[half]);
+          const float alpha = m_new == -INFINITY ? 1.f : exp2_fast(m_run[m][half] - m_new);
+          m_run[m][half] = m_new;
+          l_run[m][half] *= alpha;
+#pragma unroll
+          for (int x = 0; x < D / 8; ++x) {
+            o[m][x][half * 2] *= alpha;
+            o[m][x][half * 2 + 1] *= alpha;
+          }
+        }
+      }
+      uint32_t hi[4], lo[4];      // rows g and g + 8 of keys 2t.., then of keys 2t + 8..
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const float ref = m_run[m][half] == -INFINITY ? 0.f : m_run[m][half];
+          const float p0 = exp2_fast(fmaf(sc[m][nt][half * 2], p.scale_log2, -ref)), p1 = exp2_fast(fmaf(sc[m][nt][half * 2 + 1], p.scale_log2, -ref));
+          l_run[m][half] += p0 + p1;
+          split2<T>(p0, p1, hi[nt * 2 + half], lo[nt * 2 + half]);
+        }
+      bool careful = false;
+      if (mixed) {
+        bool odd = false;
+#pragma unroll 1
+        for (int j = 0; j < D / 8; j += 2) {
+          const uint4 v = values(j);
+          odd = odd || not_finite<T>(v.x) || not_finite<T>(v.y) || not_finite<T>(v.z) || not_finite<T>(v.w);
+        }
+        careful = __any_sync(0xffffffffu, odd);
+      }
+      if (!careful) {
+#pragma unroll
+        for (int j = 0; j < D / 8; j += 2) {
+          const uint4 v = values(j);
+          mma16816<T>(o[m][j], hi, v.x, v.y);
+          mma16816<T>(o[m][j + 1], hi, v.z, v.w);
+          mma16816<T>(o[m][j], lo, v.x, v.y);
+          mma16816<T>(o[m][j + 1], lo, v.z, v.w);
+        }
+      } else {
+        // An infinity or a NaN among values that some rows see and others do not: token by token, with the values that the token
+        // does not see as zeros, and only its own rows kept.
+        for (int pos = pos0; pos <= pos1; ++pos) {
+          const uint32_t see0 = (sees(pos, k0 + 2 * t) ? 0xffffu : 0u) | (sees(pos, k0 + 2 * t + 1) ? 0xffff0000u : 0u);
+          const uint32_t see1 = (sees(pos, k0 + 2 * t + 8) ? 0xffffu : 0u) | (sees(pos, k0 + 2 * t + 9) ? 0xffff0000u : 0u);
+          const bool mine = len - p.n + (r0 + m * 16 + g) / G == pos, mine8 = len - p.n + (r0 + m * 16 + 8 + g) / G == pos;
+#pragma unroll
+          for (int j = 0; j < D / 8; j += 2) {
+            const uint4 v = values(j);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              float acc[4] = {0.f, 0.f, 0.f, 0.f};
+              mma16816<T>(acc, hi, (x ? v.z : v.x) & see0, (x ? v.w : v.y) & see1);
+              mma16816<T>(acc, lo, (x ? v.z : v.x) & see0, (x ? v.w : v.y) & see1);
+              if (mine) { o[m][j + x][0] += acc[0]; o[m][j + x][1] += acc[1]; }
+              if (mine8) { o[m][j + x][2] += acc[2]; o[m][j + x][3] += acc[3]; }
+            }
+          }
+        }
+      }
+    }
+    __syncwarp();
+    const int now = number;
+    number = entry(fetch + kPagedWarps);
+    issue(fetch, now, stage);
+    fetch += kPagedWarps;
+    if (++stage == kStages) stage = 0;
+  }
+
+  // ---- the warps' parts: maxima and sums first, then the outputs relative to the common maximum
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      float l = l_run[m][half];
+      l += __shfl_xor_sync(0xffffffffu, l, 1);
+      l += __shfl_xor_sync(0xffffffffu, l, 2);
+      if (t == 0) {
+        s_m[warp][m * 16 + half * 8 + g] = m_run[m][half];
+        s_l[warp][m * 16 + half * 8 + g] = l;
+      }
+    }
+  copy_wait<0>();
+  __syncthreads();
+  float* part = reinterpret_cast<float*>(smem);            // [warps][kRows][D]
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int r = m * 16 + half * 8 + g;
+      float top = s_m[0][r];
+#pragma unroll
+      for (int w = 1; w < kPagedWarps; ++w) top = fmaxf(top, s_m[w][r]);
+      const float f = m_run[m][half] == -INFINITY ? 1.f : exp2_fast(m_run[m][half] - top);   // no key: zeros, or NaN
+      if (warp == 0 && t == 0) {
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < kPagedWarps; ++w) {
+          const float lw = s_l[w][r];
+          sum += s_m[w][r] == -INFINITY ? lw : lw * exp2_fast(s_m[w][r] - top);
+        }
+        s_top[r] = top;
+        s_sum[r] = sum;
+      }
+      float* dst = part + ((size_t)warp * kRows + r) * D + 2 * t;
+#pragma unroll
+      for (int j = 0; j < D / 8; ++j)
+        *reinterpret_cast<float2*>(dst + j * 8) = make_float2(o[m][j][half * 2] * f, o[m][j][half * 2 + 1] * f);
+    }
+  __syncthreads();
+  auto store = [&](int r, int d, const float (&v)[4], float sum) {
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;       // no key: zeros
+    T o4[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o4[e] = ToF<T>::from(sum == 0.f ? 0.f : v[e] * inv);
+    const int i = (r0 + r) / G, h = hk * G + (r0 + r) % G;
+    *reinterpret_cast<uint2*>(out + (((int64_t)b * p.n + i) * p.H + h) * D + d) = *reinterpret_cast<const uint2*>(o4);
+  };
+  if (p.split == 1) {
+    for (int x = threadIdx.x * 4; x < rows * D; x += kPagedWarps * 32 * 4) {
+      float v[4] = {};
+#pragma unroll
+      for (int w = 0; w < kPagedWarps; ++w) {
+        const float4 y = *reinterpret_cast<const float4*>(part + w * kRows * D + x);
+        v[0] += y.x; v[1] += y.y; v[2] += y.z; v[3] += y.w;
+      }
+      store(x / D, x % D, v, s_sum[x / D]);
+    }
+    return;
+  }
+  for (int x = threadIdx.x * 4; x < rows * D; x += kPagedWarps * 32 * 4) {       // the CTA's sum, over warp 0's part
+    float4 v = *reinterpret_cast<const float4*>(part + x);
+#pragma unroll
+    for (int w = 1; w < kPagedWarps; ++w) {
+      const float4 y = *reinterpret_cast<const float4*>(part + w * kRows * D + x);
+      v.x += y.x; v.y += y.y; v.z += y.z; v.w += y.w;
+    }
+    *reinterpret_cast<float4*>(part + x) = v;
+  }
+  // ---- the cluster's parts: every CTA finishes its share of the elements
+  cg::cluster_group cluster = cg::this_cluster();
+  cluster.sync();
+  const int quads = rows * D / 4, share = (quads + p.split - 1) / p.split;
+  for (int x = rank * share + threadIdx.x; x < min(quads, (rank + 1) * share); x += kPagedWarps * 32) {
+    const int r = x * 4 / D;
+    float top = -INFINITY, sum = 0.f, v[4] = {};
+    for (int c = 0; c < p.split; ++c) top = fmaxf(top, *cluster.map_shared_rank(&s_top[r], c));
+    for (int c = 0; c < p.split; ++c) {
+      const float mc = *cluster.map_shared_rank(&s_top[r], c), lc = *cluster.map_shared_rank(&s_sum[r], c);
+      const float4 y = *cluster.map_shared_rank(reinterpret_cast<const float4*>(part) + x, c);
+      const float f = mc == -INFINITY ? 1.f : exp2_fast(mc - top);      // a CTA without a key has zeros
+      sum += lc * f;
+      v[0] += y.x * f; v[1] += y.y * f; v[2] += y.z * f; v[3] += y.w * f;
+    }
+    store(r, x * 4 % D, v, sum);
+  }
+  cluster.sync();
 }
 
 struct PagedWriteParams {
@@ -190,13 +538,51 @@ bool rows_of_16_bytes(const void* ptr, std::initializer_list<int64_t> strides) {
   return true;
 }
 
-template <typename T, int D>
-int launch_paged(const b200_paged_attn_t* a, void* out, const void* q, const void* kp, const void* vp, const PagedParams& p,
-                 cudaStream_t stream) {
-  const long long warps = (long long)p.B * p.n * p.H, grid = (warps + 3) / 4;
+template <typename T, int D, int MT>
+int launch_paged(void* out, const void* q, const void* kp, const void* vp, PagedParams p, cudaStream_t stream) {
+  const int rows = p.n * (p.H / p.Hkv);
+  p.row_groups = (rows + 16 * MT - 1) / (16 * MT);
+  const long long units = (long long)p.B * p.Hkv * p.row_groups;
+  const long long cap = (long long)p.table_width * p.page_size;
+  const long long keys = p.window > 0 ? std::min(cap, (long long)p.window + p.sinks + p.n) : cap;
+  p.split = 1;
+  static const int target = std::getenv("B200_PAGED_TARGET") ? std::atoi(std::getenv("B200_PAGED_TARGET")) : 2 * kSMs;
+  while (p.split < kMaxSplit && units * p.split < target && keys > (long long)p.split * kPagedWarps * kStepKeys) p.split *= 2;
+  const long long grid = units * p.split;
   if (grid > 2147483647ll) return (int)cudaErrorNotSupported;
-  paged_attn_kernel<T, D><<<(unsigned)grid, 128, 0, stream>>>((T*)out, (const T*)q, (const T*)kp, (const T*)vp, p);
-  B200K_LAUNCH_RET();
+  constexpr int smem = kPagedWarps * kWarpRing + (MT > 1 ? MT * (D / 16) * 512 : 0);
+  auto kern = paged_attn_kernel<T, D, MT>;
+  static OncePerDevice once;
+  if (int e = once([&] {
+        if (int r = opt_in_smem(kern, smem)) return r;
+        return (int)cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+      }))
+    return e;
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = (unsigned)p.split;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(kPagedWarps * 32);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = p.split > 1 ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, (T*)out, (const T*)q, (const T*)kp, (const T*)vp, p);
+  if (e != cudaSuccess) {
+    (void)cudaGetLastError();
+    return (int)e;
+  }
+  note_launch();
+  return 0;
+}
+
+template <typename T>
+int launch_paged(int head_dim, void* out, const void* q, const void* kp, const void* vp, const PagedParams& p, cudaStream_t stream) {
+  const bool few = p.n * (p.H / p.Hkv) <= 16;
+  if (head_dim == 128) return few ? launch_paged<T, 128, 1>(out, q, kp, vp, p, stream) : launch_paged<T, 128, 2>(out, q, kp, vp, p, stream);
+  return few ? launch_paged<T, 64, 1>(out, q, kp, vp, p, stream) : launch_paged<T, 64, 2>(out, q, kp, vp, p, stream);
 }
 
 }  // namespace
@@ -225,11 +611,11 @@ extern "C" int b200_paged_attention(const b200_paged_attn_t* a, void* out, const
   p.table = block_table;
   p.lens = seq_lens;
   p.status = status;
-  const bool bf16 = a->dtype == B200_BF16, wide = a->head_dim == 128;
-  if (bf16) return wide ? launch_paged<__nv_bfloat16, 128>(a, out, q, k_pages, v_pages, p, stream)
-                        : launch_paged<__nv_bfloat16, 64>(a, out, q, k_pages, v_pages, p, stream);
-  return wide ? launch_paged<__half, 128>(a, out, q, k_pages, v_pages, p, stream)
-              : launch_paged<__half, 64>(a, out, q, k_pages, v_pages, p, stream);
+  p.page_shift = -1;
+  for (int x = 4; x < 31; ++x)
+    if (p.page_size == 1 << x) p.page_shift = x;
+  return a->dtype == B200_BF16 ? launch_paged<__nv_bfloat16>(a->head_dim, out, q, k_pages, v_pages, p, stream)
+                               : launch_paged<__half>(a->head_dim, out, q, k_pages, v_pages, p, stream);
 }
 
 extern "C" int b200_paged_rope_cache(const b200_paged_write_t* a, void* q_out, const void* q, const void* k, const void* v,
