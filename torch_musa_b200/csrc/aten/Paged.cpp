@@ -85,10 +85,12 @@ at::Tensor paged_attention(const at::Tensor& q_, const at::Tensor& k_pages, cons
   a.k_sp = stride_of(k_pages, 0); a.k_sh = stride_of(k_pages, 1); a.k_sr = k_pages.stride(2);
   a.v_sp = stride_of(v_pages, 0); a.v_sh = stride_of(v_pages, 1); a.v_sr = v_pages.stride(2);
   a.table_sb = block_table.stride(0);
+  at::Tensor ws;
+  if (const int64_t n = b200_paged_attention_workspace(&a)) ws = at::empty({n}, q.options().dtype(at::kFloat));
   DeviceSwitch sw(q.device().index());
   const int e = b200_paged_attention(&a, out.mutable_data_ptr(), q.const_data_ptr(), k_pages.const_data_ptr(), v_pages.const_data_ptr(),
                                      block_table.const_data_ptr<int>(), seq_lens.const_data_ptr<int>(),
-                                     device_assert_word(q.device().index()), current_raw_stream(q));
+                                     ws.defined() ? ws.mutable_data_ptr<float>() : nullptr, device_assert_word(q.device().index()), current_raw_stream(q));
   TORCH_CHECK(e != (int)cudaErrorNotSupported, op, ": unsupported sizes or strides");
   B200_KERNEL_CALL(e);
   return out;

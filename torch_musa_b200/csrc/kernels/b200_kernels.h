@@ -591,7 +591,8 @@ B200_API int b200_decode_rope_cache(int dtype, void* q_out, const void* q, const
  * and 16-byte aligned); block_table int32 [B, table_width], seq_lens int32 [B]: tokens of a sequence in the cache, the newest
  * included.  Token i stands at position len - n + i and sees key j when j <= its position and, with window > 0, its position
  * minus j < window or j < sinks.  Keys on a page number outside the pool are hidden and noted in *status (may be NULL); a
- * token that sees no key gets zeros.  D is 64 or 128, page_size a multiple of 16. */
+ * token that sees no key gets zeros.  D is 64 or 128, page_size a multiple of 16.  workspace: as many floats as
+ * b200_paged_attention_workspace says for the same description (NULL when that is 0). */
 typedef struct {
   int dtype, head_dim;
   int B, n, H, Hkv;
@@ -601,7 +602,8 @@ typedef struct {
   int64_t q_sb, q_sn, q_sh, k_sp, k_sh, k_sr, v_sp, v_sh, v_sr, table_sb;
 } b200_paged_attn_t;
 B200_API int b200_paged_attention(const b200_paged_attn_t* desc, void* out, const void* q, const void* k_pages, const void* v_pages,
-                                  const int* block_table, const int* seq_lens, int* status, cudaStream_t stream);
+                                  const int* block_table, const int* seq_lens, float* workspace, int* status, cudaStream_t stream);
+B200_API int64_t b200_paged_attention_workspace(const b200_paged_attn_t* desc);
 
 /* Rotary embedding of T new tokens and their cache update in one launch: q_out [T, H, D] = rope(q); rope(k) and v go to the rows of
  * the cache that the tokens' positions name (as above).  Tokens are packed sequence after sequence: T / B each, or

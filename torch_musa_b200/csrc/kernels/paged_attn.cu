@@ -8,24 +8,35 @@
 // torch_musa/csrc/aten/ops/attention/mudnn/SDP.cpp).
 #include "common.cuh"
 
-#include <cooperative_groups.h>
-
 #include <algorithm>
-#include <cstdlib>
 #include <initializer_list>
 #include <type_traits>
-
-namespace cg = cooperative_groups;
 
 namespace b200k {
 namespace {
 
+// x / d for 0 <= x < 2^31 with one multiplication: m = ceil(2^(32 + s) / d) - 2^32 for s = ceil(log2 d)
+struct FastDiv {
+  uint32_t mul, shift;
+  __device__ __forceinline__ int operator()(int x) const {
+    const uint32_t h = __umulhi((uint32_t)x, mul);
+    return (int)((h + (((uint32_t)x - h) >> (shift ? 1 : 0))) >> (shift ? shift - 1 : 0));
+  }
+};
+inline FastDiv fast_div(uint32_t d) {
+  uint32_t s = 0;
+  while ((1ull << s) < d) ++s;
+  return FastDiv{(uint32_t)((((1ull << s) - d) << 32) / d + 1), s};
+}
+
 struct PagedParams {
   int B, n, H, Hkv;
   int num_pages, page_size, table_width;
-  int page_shift;             // log2(page_size), or -1
+  FastDiv by_page, by_heads;  // page_size; query heads of a key head
   int window, sinks;          // window <= 0: every earlier key is visible
-  int row_groups, split;      // CTAs of one (sequence, key head): row groups x shares of the keys
+  int split, outer;           // CTAs of a cluster and clusters that share the keys of a row group
+  FastDiv by_split, by_outer;
+  float* parts;               // outer > 1: [B, Hkv, rows, outer][D + 4]: a cluster's output, sum and maximum
   float scale_log2;
   int64_t q_sb, q_sn, q_sh;                    // element strides; rows of D contiguous elements
   int64_t k_sp, k_sh, k_sr, v_sp, v_sh, v_sr;  // page, head, row in the page
@@ -36,11 +47,11 @@ struct PagedParams {
 };
 
 constexpr int kPagedWarps = 4;
-constexpr int kStepKeys = 16;          // keys of one step of a warp: they lie in one page
-constexpr int kWarpRing = 16 * 1024;   // bytes of keys and values that a warp has in flight or in hand
-constexpr int kMaxSplit = 16;          // CTAs of a cluster
-
-template <int D> constexpr int ring_stages() { return kWarpRing / (kStepKeys * D * 2 * 2); }
+constexpr int kPageRows = 16;          // rows of a page come in multiples of this
+constexpr int kStageBytes = 8192;      // keys and values of one step of a warp: 16 keys of 128 dimensions, 32 of 64
+constexpr int kStages = 2;
+constexpr int kWarpRing = kStages * kStageBytes;
+constexpr float kRaise = 8.f;          // log2: how far a score may exceed the reference maximum
 
 __device__ __forceinline__ uint32_t shared_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 // 16 bytes from global to shared memory without a register; zeros when `bytes` is 0
@@ -61,19 +72,44 @@ __device__ __forceinline__ uint4 ldmatrix_t(uint32_t a) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a) : "memory");
   return r;
 }
+// from the shared memory of another CTA of the cluster
+__device__ __forceinline__ uint32_t remote(uint32_t a, int rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float remote1(uint32_t a, int rank) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote(a, rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 remote4(uint32_t a, int rank) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(remote(a, rank)) : "memory");
+  return v;
+}
+// transposes an 8 x 8 matrix of 16-bit values that lies over the warp's registers
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// d = a b + c
 template <typename T>
-__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]) {
   if constexpr (std::is_same<T, __half>::value)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
   else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
 // (a, b) as 16-bit values, and what that rounding left of them
 template <typename T>
@@ -89,61 +125,49 @@ __device__ __forceinline__ bool not_finite(uint32_t w) {
   return (w & e) == e || (w & (e << 16)) == (e << 16);
 }
 
-// One CTA: one row group (up to 16 * MT rows = new tokens x query heads of a key head) of one (sequence, key head), one of C
-// contiguous shares of the visible keys.  A share is cut into steps of 16 keys that the four warps take in turn; each warp runs its
-// own online softmax, the warps join through shared memory and the C CTAs of a cluster through distributed shared memory.
-//
-// A warp copies the 16 rows of keys and of values of a step into a stage of its own ring (cp.async, whole rows at a time, 16-byte
-// pieces swapped by row so that the eight rows of a matrix lie in different banks) and reads them as operands of mma m16n8k16:
-//   S = Q K^T  (16 rows x 16 keys) with ldmatrix, O += P V (16 rows x D dimensions, 16 keys deep) with ldmatrix.trans.
-// P is S's accumulator layout, and goes in as a 16-bit value plus the 16-bit remainder of its rounding (2^-16 or better).
-template <typename T, int D, int MT>
-__global__ void __launch_bounds__(kPagedWarps * 32, MT == 1 ? 3 : 2) paged_attn_kernel(T* __restrict__ out, const T* __restrict__ q, const T* __restrict__ kp,
+// One CTA: one row group (up to 8 * NT rows = new tokens x query heads of a key head) of one (sequence, key head), one of several
+// contiguous shares of the visible keys.  A share is cut into steps of 16 keys (32 when D is 64) that the four warps take in turn;
+// each warp runs its own online softmax, the warps join through shared memory and the CTAs of a cluster through distributed shared
+// memory.  A warp copies the rows of keys and of values of a step into a stage of its own ring (cp.async, whole rows at a time,
+// 16-byte pieces swapped by row so that the eight rows of a matrix lie in different banks).  The products are mma m16n8k16 with the
+// long side first, because a key head seldom has more than eight rows:
+//   S^T = K Q^T    16 keys x 8 rows; K by ldmatrix, Q in registers;
+//   O^T += V^T P^T  16 dimensions x 8 rows, 16 keys deep; V^T by ldmatrix.trans, P^T from S^T by movmatrix.
+// A lane's columns are rows 2 t and 2 t + 1 in both, so a row's maximum and sum stay with the lanes that hold its outputs.  P goes in as
+// a 16-bit value plus the 16-bit remainder of its rounding (2^-16 or better).  The maximum that exponents refer to is raised only
+// when a score exceeds it by 2^8: then eight lanes have to be asked, which most steps leave out.
+// kDense: the rows of a page follow one another (the layout of the pools as they are made), so that a copy's address is a constant
+// away from the page's.
+template <typename T, int D, int NT, bool kDense>
+__global__ void __launch_bounds__(kPagedWarps * 32, NT <= 2 ? 3 : 2) paged_attn_kernel(T* __restrict__ out, const T* __restrict__ q, const T* __restrict__ kp,
                                                                          const T* __restrict__ vp, const PagedParams p) {
-  constexpr int kRows = 16 * MT, kStages = ring_stages<D>(), kStage = kStepKeys * D * 4;
+  constexpr int kRows = 8 * NT, kHalves = kStageBytes / (kPageRows * D * 4), kKeys = kHalves * kPageRows, kHalf = kPageRows * D * 2;
+  constexpr int kPad = D + 4;            // floats of a row of a part: the four lanes' rows then lie in different banks
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ float s_m[kPagedWarps][kRows], s_l[kPagedWarps][kRows];
   __shared__ float s_top[kRows], s_sum[kRows];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int G = p.H / p.Hkv, rows_all = p.n * G;
-  const int rank = (int)(blockIdx.x % p.split);
-  int unit = (int)(blockIdx.x / p.split);
-  const int group = unit % p.row_groups;
-  unit /= p.row_groups;
-  const int hk = unit % p.Hkv, b = unit / p.Hkv;
-  const int r0 = group * kRows, rows = min(kRows, rows_all - r0);
-  const int len = (int)min((long long)max(__ldg(p.lens + b), 0), (long long)p.table_width * p.page_size);
-  // positions of the oldest and the newest token of the group; the steps of 16 keys that one of them sees
-  const int pos0 = len - p.n + r0 / G, pos1 = len - p.n + (r0 + rows - 1) / G;
+  const int G = p.H / p.Hkv, rows_all = p.n * G, split = p.split;
+  const int cluster = p.by_split((int)blockIdx.x), rank = (int)blockIdx.x - cluster * split;      // clusters lie along x
+  const int group = p.by_outer(cluster), outer = cluster - group * p.outer;
+  const int r0 = group * kRows;
+  const int hk = blockIdx.y, b = blockIdx.z;
+  const int rows = min(kRows, rows_all - r0);
+  const int len = min(max(__ldg(p.lens + b), 0), p.table_width * p.page_size);
+  // positions of the oldest and the newest token of the group; the steps that one of them sees
+  const int pos0 = len - p.n + p.by_heads(r0), pos1 = len - p.n + p.by_heads(r0 + rows - 1);
+  // positions of this lane's rows: 2 t and 2 t + 1 of each eight
+  int pos[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) pos[nt][e] = len - p.n + p.by_heads(r0 + nt * 8 + 2 * t + e);
   const int wlo = p.window > 0 ? max(0, pos0 - p.window + 1) : 0;
-  const int end = pos1 >= 0 ? pos1 / kStepKeys + 1 : 0;
-  const int sink_steps = min(end, (p.sinks + kStepKeys - 1) / kStepKeys), first = max(wlo / kStepKeys, sink_steps);
-  const int steps = sink_steps + max(0, end - first);
-  const int s0 = (int)((long long)steps * rank / p.split), s1 = (int)((long long)steps * (rank + 1) / p.split);
-  auto key_of = [&](int s) { return (s < sink_steps ? s : s - sink_steps + first) * kStepKeys; };
-
-  // Q as operands: rows g and g + 8 of each 16, dimensions 16 ks + 2 t and 8 further
-  uint4 qf[D / 16];
-  uint4* sq = reinterpret_cast<uint4*>(smem + kPagedWarps * kWarpRing) + lane;      // MT == 2: [m][ks][lane], they would not fit
-#pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    if (MT > 1 && warp != m) continue;
-    const T* row[2];
-    bool real[2];
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const int r = m * 16 + half * 8 + g;
-      real[half] = r < rows;
-      row[half] = q + b * p.q_sb + (r0 + r) / G * p.q_sn + (hk * G + (r0 + r) % G) * p.q_sh + 2 * t;
-    }
-#pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks) {
-      auto word = [&](int half, int d) { return real[half] ? __ldg(reinterpret_cast<const uint32_t*>(row[half] + d)) : 0u; };
-      const uint4 x = make_uint4(word(0, ks * 16), word(1, ks * 16), word(0, ks * 16 + 8), word(1, ks * 16 + 8));
-      if constexpr (MT == 1) qf[ks] = x;
-      else sq[(m * (D / 16) + ks) * 32] = x;
-    }
-  }
+  const int end = pos1 >= 0 ? pos1 / kKeys + 1 : 0;
+  const int sink_steps = min(end, (p.sinks + kKeys - 1) / kKeys), first = max(wlo / kKeys, sink_steps);
+  const int steps = sink_steps + max(0, end - first), shares = split * p.outer, mine = outer * split + rank;
+  const int s0 = (int)((long long)steps * mine / shares), s1 = (int)((long long)steps * (mine + 1) / shares);
+  auto key_of = [&](int s) { return (s < sink_steps ? s : s - sink_steps + first) * kKeys; };
 
   const uint32_t ring = shared_u32(smem) + warp * kWarpRing;
   const int* table = p.table + b * p.table_sb;
@@ -151,193 +175,254 @@ __global__ void __launch_bounds__(kPagedWarps * 32, MT == 1 ? 3 : 2) paged_attn_
   const int crow = lane / kPieces, cpiece = lane % kPieces;
   const T* kbase = kp + hk * p.k_sh + crow * p.k_sr + cpiece * 8;
   const T* vbase = vp + hk * p.v_sh + crow * p.v_sr + cpiece * 8;
+  constexpr int kSwaps = 8 / kPerCopy;   // rows r of copy i: their swap depends on i modulo this
+  uint32_t cdst[kSwaps];
+#pragma unroll
+  for (int i = 0; i < kSwaps; ++i) cdst[i] = (uint32_t)(crow * D * 2 + ((cpiece ^ ((i * kPerCopy + crow) & 7)) * 16));
   const int mi = lane >> 3, mr = lane & 7;
   // a lane's row address in a stage for ldmatrix; the piece 2 x of a row is at ((2 x) ^ swap) * 16, for x < 4
-  const uint32_t krow = (uint32_t)(((mi >> 1) * 8 + mr) * D * 2), kswap = (uint32_t)(((mi & 1) ^ mr) * 16);
-  const uint32_t vrow = (uint32_t)(kStepKeys * D * 2 + ((mi & 1) * 8 + mr) * D * 2), vswap = (uint32_t)(((mi >> 1) ^ mr) * 16);
-  auto entry = [&](int s) {          // the page number of a step, read one step before it is needed
-    if (s >= s1) return -1;
-    const int k0 = key_of(s);
-    return __ldg(table + (p.page_shift >= 0 ? k0 >> p.page_shift : k0 / p.page_size));
-  };
-  uint32_t found = 0;                // one bit a stage: whether the page of its step is in the pool
-  auto issue = [&](int s, int number, int stage) {
-    if (s < s1) {
-      const int k0 = key_of(s);
-      const bool there = number >= 0 && number < p.num_pages;
-      if (!there && lane == 0 && p.status) atomicExch(p.status, 1);
-      found = (found & ~(1u << stage)) | ((uint32_t)there << stage);
-      const int64_t row = p.page_shift >= 0 ? k0 & (p.page_size - 1) : k0 % p.page_size, page = there ? number : 0;
-      const T* ks = kbase + page * p.k_sp + row * p.k_sr;
-      const T* vs = vbase + page * p.v_sp + row * p.v_sr;
-      const uint32_t dst = ring + stage * kStage + (uint32_t)(crow * D * 2);
-      // keys that no row sees are not read: zeros instead (with a probability of zero nothing else would be safe)
-      auto copy = [&](auto whole) {
+  uint32_t kaddr[4], vaddr[4];
 #pragma unroll
-        for (int i = 0; i < kStepKeys / kPerCopy; ++i) {
-          const int r = i * kPerCopy + crow, j = k0 + r;
-          const int n16 = decltype(whole)::value || (there && j <= pos1 && (j >= wlo || j < p.sinks)) ? 16 : 0;
-          const uint32_t d = dst + (uint32_t)(i * kPerCopy * D * 2) + (uint32_t)((cpiece ^ (r & 7)) * 16);
-          copy16(d, ks + i * kPerCopy * p.k_sr, n16);
-          copy16(d + kStepKeys * D * 2, vs + i * kPerCopy * p.v_sr, n16);
-        }
-      };
-      if (there && k0 + kStepKeys - 1 <= pos1 && (k0 >= wlo || k0 + kStepKeys <= p.sinks)) copy(std::true_type{});
-      else copy(std::false_type{});
+  for (int x = 0; x < 4; ++x) {
+    kaddr[x] = ring + (uint32_t)(((mi & 1) * 8 + mr) * D * 2) + (((uint32_t)x * 32) ^ (uint32_t)(((mi >> 1) ^ mr) * 16));
+    vaddr[x] = ring + (uint32_t)(kHalves * kHalf + ((mi >> 1) * 8 + mr) * D * 2) + (((uint32_t)x * 32) ^ (uint32_t)(((mi & 1) ^ mr) * 16));
+  }
+
+  struct Pages { int n[kHalves]; };
+  auto entry = [&](int s) {          // the page numbers of a step, read one step before they are needed
+    Pages e;
+    const int k0 = key_of(s);
+#pragma unroll
+    for (int x = 0; x < kHalves; ++x) e.n[x] = s < s1 && k0 + x * kPageRows <= pos1 ? __ldg(table + p.by_page(k0 + x * kPageRows)) : -1;
+    return e;
+  };
+  uint32_t found = 0;                // one bit a stage and half: whether its page is in the pool
+  auto issue = [&](int s, const Pages& e, int stage) {
+    if (s < s1) {
+#pragma unroll
+      for (int x = 0; x < kHalves; ++x) {
+        const int k0 = key_of(s) + x * kPageRows, number = e.n[x];
+        const bool there = (unsigned)number < (unsigned)p.num_pages;
+        if (!there && k0 <= pos1 && lane == 0 && p.status) atomicExch(p.status, 1);
+        const uint32_t bit = 1u << (stage * kHalves + x);
+        found = there ? found | bit : found & ~bit;
+        const uint32_t page = there ? (uint32_t)number : 0u, row = (uint32_t)(k0 - p.by_page(k0) * p.page_size);
+        const T* ks = kbase + (uint64_t)page * (uint64_t)p.k_sp + (kDense ? row * D : (uint64_t)row * (uint64_t)p.k_sr);
+        const T* vs = vbase + (uint64_t)page * (uint64_t)p.v_sp + (kDense ? row * D : (uint64_t)row * (uint64_t)p.v_sr);
+        const uint32_t dst = ring + stage * kStageBytes + x * kHalf;
+        // keys that no row sees are not read: zeros instead (with a probability of zero nothing else would be safe)
+        auto copy = [&](auto whole) {
+#pragma unroll
+          for (int i = 0; i < kPageRows / kPerCopy; ++i) {
+            const int j = k0 + i * kPerCopy + crow;
+            const int n16 = decltype(whole)::value || (there && j <= pos1 && (j >= wlo || j < p.sinks)) ? 16 : 0;
+            const uint32_t d = dst + cdst[i % kSwaps] + (uint32_t)(i * kPerCopy * D * 2);
+            copy16(d, ks + (kDense ? i * kPerCopy * D : i * kPerCopy * p.k_sr), n16);
+            copy16(d + kHalves * kHalf, vs + (kDense ? i * kPerCopy * D : i * kPerCopy * p.v_sr), n16);
+          }
+        };
+        if (there && k0 + kPageRows - 1 <= pos1 && (k0 >= wlo || k0 + kPageRows <= p.sinks)) copy(std::true_type{});
+        else copy(std::false_type{});
+      }
     }
     copy_commit();
   };
-
-  float o[MT][D / 8][4], m_run[MT][2], l_run[MT][2];
-#pragma unroll
-  for (int m = 0; m < MT; ++m) {
-#pragma unroll
-    for (int x = 0; x < D / 8; ++x)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[m][x][e] = 0.f;
-    m_run[m][0] = m_run[m][1] = -INFINITY;
-    l_run[m][0] = l_run[m][1] = 0.f;
-  }
-
-  if constexpr (MT > 1) __syncthreads();
   int s = s0 + warp, fetch = s;
-  int number = entry(fetch);
+  Pages number = entry(fetch);
 #pragma unroll
   for (int st = 0; st < kStages; ++st) {
-    const int now = number;
+    const Pages now = number;
     number = entry(fetch + kPagedWarps);
     issue(fetch, now, st);
     fetch += kPagedWarps;
   }
+
+  // Q as operands: row g of each eight, dimensions 16 ks + 2 t and 8 further
+  uint32_t qf[NT][D / 16][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int r = nt * 8 + g, i = p.by_heads(r0 + r);
+    const T* row = q + b * p.q_sb + i * p.q_sn + (hk * G + r0 + r - i * G) * p.q_sh + 2 * t;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) qf[nt][ks][e] = r < rows ? __ldg(reinterpret_cast<const uint32_t*>(row + ks * 16 + e * 8)) : 0u;
+  }
+
+  float o[NT][D / 16][4], m_run[NT][2], l_run[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+    for (int x = 0; x < D / 16; ++x)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[nt][x][e] = 0.f;
+    m_run[nt][0] = m_run[nt][1] = -INFINITY;
+    l_run[nt][0] = l_run[nt][1] = 0.f;
+  }
+
   int stage = 0;
   for (; s < s1; s += kPagedWarps) {
     copy_wait<kStages - 1>();
     __syncwarp();
     const int k0 = key_of(s);
-    const uint32_t src = ring + stage * kStage;
-    float sc[MT][2][4];
+    const uint32_t at = stage * kStageBytes;
+    const uint32_t ka[4] = {kaddr[0] + at, kaddr[1] + at, kaddr[2] + at, kaddr[3] + at};
+    const uint32_t va[4] = {vaddr[0] + at, vaddr[1] + at, vaddr[2] + at, vaddr[3] + at};
+    float sc[kHalves][NT][4];            // key g (and g + 8) of a half, rows 2 t and 2 t + 1
     {
-      float part[MT][2][4];          // odd products: four chains of half the length instead of two
+      constexpr int kChains = kHalves * NT >= 4 ? 1 : 4 / (kHalves * NT);      // independent sums in flight: four at least
+      float part[kChains][kHalves][NT][4];
+      const float zero[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
+      for (int ks = 0; ks < D / 16; ++ks)
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt)
+        for (int x = 0; x < kHalves; ++x) {
+          const uint4 kf = ldmatrix(ka[ks & 3] + (ks >> 2) * 128 + x * kHalf);
+          const uint32_t a[4] = {kf.x, kf.y, kf.z, kf.w};
 #pragma unroll
-          for (int e = 0; e < 4; ++e) sc[m][nt][e] = part[m][nt][e] = 0.f;
-#pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) {
-        const uint4 kf = ldmatrix(src + krow + (((uint32_t)(ks & 3) * 32) ^ kswap) + (uint32_t)(ks >> 2) * 128);
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          const uint4 x = MT == 1 ? qf[ks] : sq[(m * (D / 16) + ks) * 32];
-          const uint32_t a[4] = {x.x, x.y, x.z, x.w};
-          mma16816<T>(ks & 1 ? part[m][0] : sc[m][0], a, kf.x, kf.y);
-          mma16816<T>(ks & 1 ? part[m][1] : sc[m][1], a, kf.z, kf.w);
-        }
-      }
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) sc[m][nt][e] += part[m][nt][e];
-    }
-    auto values = [&](int j) {         // the operands of dimensions [8 j, 8 j + 16), j even
-      return ldmatrix_t(src + vrow + (((uint32_t)(j & 7) * 16) ^ vswap) + (uint32_t)(j >> 3) * 128);
-    };
-    const bool there = (found >> stage) & 1u;
-    const bool all = there && k0 + kStepKeys - 1 <= pos0 && (p.window <= 0 || k0 > pos1 - p.window || k0 + kStepKeys <= p.sinks);
-    const bool mixed = !all && pos0 != pos1;
-    auto sees = [&](int pos, int j) { return there && j <= pos && (p.window <= 0 || j > pos - p.window || j < p.sinks); };
-
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      float mx[2];
-      if (!all) {
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int pos = len - p.n + (r0 + m * 16 + half * 8 + g) / G;
-#pragma unroll
-          for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-              if (!sees(pos, k0 + nt * 8 + 2 * t + e)) sc[m][nt][half * 2 + e] = -INFINITY;
-        }
-      }
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        float x = fmaxf(fmaxf(sc[m][0][half * 2], sc[m][0][half * 2 + 1]), fmaxf(sc[m][1][half * 2], sc[m][1][half * 2 + 1]));
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-        mx[half] = x * p.scale_log2;
-      }
-      if (__any_sync(0xffffffffu, mx[0] > m_run[m][0] || mx[1] > m_run[m][1])) {
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const float m_new = fmaxf(m_run[m][half], mx[half]);
-          const float alpha = m_new == -INFINITY ? 1.f : exp2_fast(m_run[m][half] - m_new);
-          m_run[m][half] = m_new;
-          l_run[m][half] *= alpha;
-#pragma unroll
-          for (int x = 0; x < D / 8; ++x) {
-            o[m][x][half * 2] *= alpha;
-            o[m][x][half * 2 + 1] *= alpha;
+          for (int nt = 0; nt < NT; ++nt) {
+            float(&d)[4] = part[ks % kChains][x][nt];
+            if (ks < kChains) mma16816<T>(d, a, qf[nt][ks][0], qf[nt][ks][1], zero);
+            else mma16816<T>(d, a, qf[nt][ks][0], qf[nt][ks][1], d);
           }
         }
-      }
-      uint32_t hi[4], lo[4];      // rows g and g + 8 of keys 2t.., then of keys 2t + 8..
 #pragma unroll
-      for (int nt = 0; nt < 2; ++nt)
+      for (int x = 0; x < kHalves; ++x)
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const float ref = m_run[m][half] == -INFINITY ? 0.f : m_run[m][half];
-          const float p0 = exp2_fast(fmaf(sc[m][nt][half * 2], p.scale_log2, -ref)), p1 = exp2_fast(fmaf(sc[m][nt][half * 2 + 1], p.scale_log2, -ref));
-          l_run[m][half] += p0 + p1;
-          split2<T>(p0, p1, hi[nt * 2 + half], lo[nt * 2 + half]);
-        }
-      bool careful = false;
-      if (mixed) {
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            sc[x][nt][e] = part[0][x][nt][e];
+#pragma unroll
+            for (int c = 1; c < kChains; ++c) sc[x][nt][e] += part[c][x][nt][e];
+          }
+    }
+    // V^T of dimensions [16 j, 16 j + 16) and the keys of half x
+    auto values = [&](int j, int x) { return ldmatrix_t(va[j & 3] + (j >> 2) * 128 + x * kHalf); };
+    const uint32_t pages = (found >> (stage * kHalves)) & ((1u << kHalves) - 1u);
+    const bool all = pages == (1u << kHalves) - 1u && k0 + kKeys - 1 <= pos0 && (p.window <= 0 || k0 > pos1 - p.window || k0 + kKeys <= p.sinks);
+    auto sees = [&](int ps, int j) {
+      return ((pages >> ((j - k0) / kPageRows)) & 1u) && j <= ps && (p.window <= 0 || j > ps - p.window || j < p.sinks);
+    };
+    bool careful = false;
+    if (!all) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int x = 0; x < kHalves; ++x)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (!sees(pos[nt][e & 1], k0 + x * kPageRows + (e >> 1) * 8 + g)) sc[x][nt][e] = -INFINITY;
+      if (pos0 != pos1) {            // rows differ in what they see
         bool odd = false;
 #pragma unroll 1
-        for (int j = 0; j < D / 8; j += 2) {
-          const uint4 v = values(j);
-          odd = odd || not_finite<T>(v.x) || not_finite<T>(v.y) || not_finite<T>(v.z) || not_finite<T>(v.w);
-        }
+        for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+          for (int x = 0; x < kHalves; ++x) {
+            const uint4 v = ldmatrix_t((j & 2 ? (j & 1 ? va[3] : va[2]) : (j & 1 ? va[1] : va[0])) + (j >> 2) * 128 + x * kHalf);
+            odd = odd || not_finite<T>(v.x) || not_finite<T>(v.y) || not_finite<T>(v.z) || not_finite<T>(v.w);
+          }
         careful = __any_sync(0xffffffffu, odd);
       }
-      if (!careful) {
+    }
+    // a score that exceeds the reference by 2^8: every row's maximum is found and becomes the reference
+    bool above = false;
 #pragma unroll
-        for (int j = 0; j < D / 8; j += 2) {
-          const uint4 v = values(j);
-          mma16816<T>(o[m][j], hi, v.x, v.y);
-          mma16816<T>(o[m][j + 1], hi, v.z, v.w);
-          mma16816<T>(o[m][j], lo, v.x, v.y);
-          mma16816<T>(o[m][j + 1], lo, v.z, v.w);
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float x = fmaxf(sc[0][nt][e], sc[0][nt][e + 2]);
+        if constexpr (kHalves == 2) x = fmaxf(x, fmaxf(sc[1][nt][e], sc[1][nt][e + 2]));
+        above = above || x * p.scale_log2 > m_run[nt][e] + kRaise;
+      }
+    if (__any_sync(0xffffffffu, above)) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float x = fmaxf(sc[0][nt][e], sc[0][nt][e + 2]);
+          if constexpr (kHalves == 2) x = fmaxf(x, fmaxf(sc[1][nt][e], sc[1][nt][e + 2]));
+#pragma unroll
+          for (int w = 4; w < 32; w <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, w));
+          const float m_new = fmaxf(m_run[nt][e], x * p.scale_log2);
+          const float alpha = m_new == -INFINITY ? 1.f : exp2_fast(m_run[nt][e] - m_new);
+          m_run[nt][e] = m_new;
+          l_run[nt][e] *= alpha;
+#pragma unroll
+          for (int j = 0; j < D / 16; ++j) {
+            o[nt][j][e] *= alpha;
+            o[nt][j][e + 2] *= alpha;
+          }
         }
-      } else {
-        // An infinity or a NaN among values that some rows see and others do not: token by token, with the values that the token
-        // does not see as zeros, and only its own rows kept.
-        for (int pos = pos0; pos <= pos1; ++pos) {
-          const uint32_t see0 = (sees(pos, k0 + 2 * t) ? 0xffffu : 0u) | (sees(pos, k0 + 2 * t + 1) ? 0xffff0000u : 0u);
-          const uint32_t see1 = (sees(pos, k0 + 2 * t + 8) ? 0xffffu : 0u) | (sees(pos, k0 + 2 * t + 9) ? 0xffff0000u : 0u);
-          const bool mine = len - p.n + (r0 + m * 16 + g) / G == pos, mine8 = len - p.n + (r0 + m * 16 + 8 + g) / G == pos;
+    }
+    uint32_t hi[kHalves][NT][2], lo[kHalves][NT][2];      // P^T: keys 2 t.. and 2 t + 8.. of row g
 #pragma unroll
-          for (int j = 0; j < D / 8; j += 2) {
-            const uint4 v = values(j);
+    for (int nt = 0; nt < NT; ++nt) {
+      const float ref0 = m_run[nt][0] == -INFINITY ? 0.f : m_run[nt][0], ref1 = m_run[nt][1] == -INFINITY ? 0.f : m_run[nt][1];
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              float acc[4] = {0.f, 0.f, 0.f, 0.f};
-              mma16816<T>(acc, hi, (x ? v.z : v.x) & see0, (x ? v.w : v.y) & see1);
-              mma16816<T>(acc, lo, (x ? v.z : v.x) & see0, (x ? v.w : v.y) & see1);
-              if (mine) { o[m][j + x][0] += acc[0]; o[m][j + x][1] += acc[1]; }
-              if (mine8) { o[m][j + x][2] += acc[2]; o[m][j + x][3] += acc[3]; }
+      for (int x = 0; x < kHalves; ++x)
+#pragma unroll
+        for (int k8 = 0; k8 < 2; ++k8) {
+          const float p0 = exp2_fast(fmaf(sc[x][nt][k8 * 2], p.scale_log2, -ref0)), p1 = exp2_fast(fmaf(sc[x][nt][k8 * 2 + 1], p.scale_log2, -ref1));
+          l_run[nt][0] += p0;
+          l_run[nt][1] += p1;
+          uint32_t h, l;
+          split2<T>(p0, p1, h, l);
+          hi[x][nt][k8] = transpose8(h);
+          lo[x][nt][k8] = transpose8(l);
+        }
+    }
+    if (!careful) {
+      constexpr int kBatch = 4;            // operands in hand: the two products of an output are four or more apart
+#pragma unroll
+      for (int j0 = 0; j0 < D / 16; j0 += kBatch)
+#pragma unroll
+        for (int x = 0; x < kHalves; ++x) {
+          uint4 v[kBatch];
+#pragma unroll
+          for (int j = 0; j < kBatch; ++j) v[j] = values(j0 + j, x);
+#pragma unroll
+          for (int part = 0; part < 2; ++part)
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j) {
+              const uint32_t a[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                const uint32_t(&w)[2] = part ? lo[x][nt] : hi[x][nt];
+                mma16816<T>(o[nt][j0 + j], a, w[0], w[1], o[nt][j0 + j]);
+              }
+            }
+        }
+    } else {
+      // An infinity or a NaN among values that some rows see and others do not: token by token, with the values that the token
+      // does not see as zeros, and only its own rows kept.
+#pragma unroll 1
+      for (int ps = pos0; ps <= pos1; ++ps) {
+#pragma unroll
+        for (int x = 0; x < kHalves; ++x) {
+          const int kx = k0 + x * kPageRows + 2 * t;
+          const uint32_t see0 = (sees(ps, kx) ? 0xffffu : 0u) | (sees(ps, kx + 1) ? 0xffff0000u : 0u);
+          const uint32_t see1 = (sees(ps, kx + 8) ? 0xffffu : 0u) | (sees(ps, kx + 9) ? 0xffff0000u : 0u);
+#pragma unroll
+          for (int j = 0; j < D / 16; ++j) {
+            const uint4 v = values(j, x);
+            const uint32_t a[4] = {v.x & see0, v.y & see0, v.z & see1, v.w & see1};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+              float acc[4];
+              mma16816<T>(acc, a, hi[x][nt][0], hi[x][nt][1], zero);
+              mma16816<T>(acc, a, lo[x][nt][0], lo[x][nt][1], acc);
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (pos[nt][e & 1] == ps) o[nt][j][e] += acc[e];
             }
           }
         }
       }
     }
     __syncwarp();
-    const int now = number;
+    const Pages now = number;
     number = entry(fetch + kPagedWarps);
     issue(fetch, now, stage);
     fetch += kPagedWarps;
@@ -346,92 +431,139 @@ __global__ void __launch_bounds__(kPagedWarps * 32, MT == 1 ? 3 : 2) paged_attn_
 
   // ---- the warps' parts: maxima and sums first, then the outputs relative to the common maximum
 #pragma unroll
-  for (int m = 0; m < MT; ++m)
+  for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      float l = l_run[m][half];
-      l += __shfl_xor_sync(0xffffffffu, l, 1);
-      l += __shfl_xor_sync(0xffffffffu, l, 2);
-      if (t == 0) {
-        s_m[warp][m * 16 + half * 8 + g] = m_run[m][half];
-        s_l[warp][m * 16 + half * 8 + g] = l;
+    for (int e = 0; e < 2; ++e) {
+      float l = l_run[nt][e];
+#pragma unroll
+      for (int w = 4; w < 32; w <<= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
+      if (g == 0) {
+        s_m[warp][nt * 8 + 2 * t + e] = m_run[nt][e];
+        s_l[warp][nt * 8 + 2 * t + e] = l;
       }
     }
   copy_wait<0>();
   __syncthreads();
-  float* part = reinterpret_cast<float*>(smem);            // [warps][kRows][D]
+  float* part = reinterpret_cast<float*>(smem);            // [warps][kRows][kPad]
 #pragma unroll
-  for (int m = 0; m < MT; ++m)
+  for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const int r = m * 16 + half * 8 + g;
+    for (int e = 0; e < 2; ++e) {
+      const int r = nt * 8 + 2 * t + e;
+      if (r >= rows) continue;
       float top = s_m[0][r];
 #pragma unroll
       for (int w = 1; w < kPagedWarps; ++w) top = fmaxf(top, s_m[w][r]);
-      const float f = m_run[m][half] == -INFINITY ? 1.f : exp2_fast(m_run[m][half] - top);   // no key: zeros, or NaN
-      if (warp == 0 && t == 0) {
+      const float f = m_run[nt][e] == -INFINITY ? 1.f : exp2_fast(m_run[nt][e] - top);   // no key: zeros, or NaN
+      if (warp == 0 && g == 0) {
         float sum = 0.f;
 #pragma unroll
-        for (int w = 0; w < kPagedWarps; ++w) {
-          const float lw = s_l[w][r];
-          sum += s_m[w][r] == -INFINITY ? lw : lw * exp2_fast(s_m[w][r] - top);
-        }
+        for (int w = 0; w < kPagedWarps; ++w) sum += s_m[w][r] == -INFINITY ? s_l[w][r] : s_l[w][r] * exp2_fast(s_m[w][r] - top);
         s_top[r] = top;
         s_sum[r] = sum;
       }
-      float* dst = part + ((size_t)warp * kRows + r) * D + 2 * t;
+      float* dst = part + ((size_t)warp * kRows + r) * kPad + g;
 #pragma unroll
-      for (int j = 0; j < D / 8; ++j)
-        *reinterpret_cast<float2*>(dst + j * 8) = make_float2(o[m][j][half * 2] * f, o[m][j][half * 2 + 1] * f);
+      for (int j = 0; j < D / 16; ++j) {
+        dst[j * 16] = o[nt][j][e] * f;
+        dst[j * 16 + 8] = o[nt][j][e + 2] * f;
+      }
     }
   __syncthreads();
-  auto store = [&](int r, int d, const float (&v)[4], float sum) {
+  auto store = [&](int r, int d, const float (&v)[4], float sum, float top) {
+    if (p.outer > 1) {
+      float* dst = p.parts + ((((int64_t)b * p.Hkv + hk) * rows_all + r0 + r) * p.outer + outer) * (D + 4);
+      *reinterpret_cast<float4*>(dst + d) = make_float4(v[0], v[1], v[2], v[3]);
+      if (d == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(sum, top);
+      return;
+    }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;       // no key: zeros
     T o4[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) o4[e] = ToF<T>::from(sum == 0.f ? 0.f : v[e] * inv);
-    const int i = (r0 + r) / G, h = hk * G + (r0 + r) % G;
+    const int i = p.by_heads(r0 + r), h = hk * G + r0 + r - i * G;
     *reinterpret_cast<uint2*>(out + (((int64_t)b * p.n + i) * p.H + h) * D + d) = *reinterpret_cast<const uint2*>(o4);
   };
-  if (p.split == 1) {
-    for (int x = threadIdx.x * 4; x < rows * D; x += kPagedWarps * 32 * 4) {
-      float v[4] = {};
-#pragma unroll
-      for (int w = 0; w < kPagedWarps; ++w) {
-        const float4 y = *reinterpret_cast<const float4*>(part + w * kRows * D + x);
-        v[0] += y.x; v[1] += y.y; v[2] += y.z; v[3] += y.w;
-      }
-      store(x / D, x % D, v, s_sum[x / D]);
-    }
-    return;
-  }
-  for (int x = threadIdx.x * 4; x < rows * D; x += kPagedWarps * 32 * 4) {       // the CTA's sum, over warp 0's part
-    float4 v = *reinterpret_cast<const float4*>(part + x);
+  for (int x = threadIdx.x; x < rows * (D / 4); x += kPagedWarps * 32) {       // the CTA's sum, over warp 0's part
+    const int r = x / (D / 4), d = x % (D / 4) * 4;
+    float4 v = *reinterpret_cast<const float4*>(part + r * kPad + d);
 #pragma unroll
     for (int w = 1; w < kPagedWarps; ++w) {
-      const float4 y = *reinterpret_cast<const float4*>(part + w * kRows * D + x);
+      const float4 y = *reinterpret_cast<const float4*>(part + (w * kRows + r) * kPad + d);
       v.x += y.x; v.y += y.y; v.z += y.z; v.w += y.w;
     }
-    *reinterpret_cast<float4*>(part + x) = v;
-  }
-  // ---- the cluster's parts: every CTA finishes its share of the elements
-  cg::cluster_group cluster = cg::this_cluster();
-  cluster.sync();
-  const int quads = rows * D / 4, share = (quads + p.split - 1) / p.split;
-  for (int x = rank * share + threadIdx.x; x < min(quads, (rank + 1) * share); x += kPagedWarps * 32) {
-    const int r = x * 4 / D;
-    float top = -INFINITY, sum = 0.f, v[4] = {};
-    for (int c = 0; c < p.split; ++c) top = fmaxf(top, *cluster.map_shared_rank(&s_top[r], c));
-    for (int c = 0; c < p.split; ++c) {
-      const float mc = *cluster.map_shared_rank(&s_top[r], c), lc = *cluster.map_shared_rank(&s_sum[r], c);
-      const float4 y = *cluster.map_shared_rank(reinterpret_cast<const float4*>(part) + x, c);
-      const float f = mc == -INFINITY ? 1.f : exp2_fast(mc - top);      // a CTA without a key has zeros
-      sum += lc * f;
-      v[0] += y.x * f; v[1] += y.y * f; v[2] += y.z * f; v[3] += y.w * f;
+    if (split == 1) {
+      const float v4[4] = {v.x, v.y, v.z, v.w};
+      store(r, d, v4, s_sum[r], s_top[r]);
+    } else {
+      *reinterpret_cast<float4*>(part + r * kPad + d) = v;
     }
-    store(r, x * 4 % D, v, sum);
   }
-  cluster.sync();
+  if (split == 1) return;
+  // ---- the cluster's parts: every CTA finishes its share of the elements
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  const uint32_t a_top = shared_u32(s_top), a_sum = shared_u32(s_sum), a_part = shared_u32(part);
+  const int quads = rows * D / 4, share = (quads + split - 1) / split;
+  for (int x = rank * share + threadIdx.x; x < min(quads, (rank + 1) * share); x += kPagedWarps * 32) {
+    const int r = x / (D / 4), d = x % (D / 4) * 4;
+    float top = -INFINITY, sum = 0.f, v[4] = {};
+    // four CTAs at a time, all their loads in flight; relative to the maximum so far, as always
+    for (int c0 = 0; c0 < split; c0 += 4) {
+      float mc[4], lc[4];
+      float4 y[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        mc[c] = -INFINITY;
+        lc[c] = 0.f;
+        y[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (c0 + c < split) {
+          mc[c] = remote1(a_top + r * 4, c0 + c);
+          lc[c] = remote1(a_sum + r * 4, c0 + c);
+          y[c] = remote4(a_part + (r * kPad + d) * 4, c0 + c);
+        }
+      }
+      const float up = fmaxf(fmaxf(fmaxf(mc[0], mc[1]), fmaxf(mc[2], mc[3])), top);
+      const float old = top == -INFINITY ? 1.f : exp2_fast(top - up);
+      top = up;
+      sum *= old;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] *= old;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const float f = mc[c] == -INFINITY ? 1.f : exp2_fast(mc[c] - up);      // a CTA without a key has zeros
+        sum += lc[c] * f;
+        v[0] += y[c].x * f; v[1] += y[c].y * f; v[2] += y[c].z * f; v[3] += y[c].w * f;
+      }
+    }
+    store(r, d, v, sum, top);
+  }
+  // nobody leaves while its memory may still be read
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+
+// Joins the clusters' parts of a row: a thread owns four dimensions of one row.
+template <typename T, int D>
+__global__ void __launch_bounds__(128) paged_join_kernel(T* __restrict__ out, const PagedParams p) {
+  const int G = p.H / p.Hkv, rows_all = p.n * G;
+  const int64_t x = (int64_t)blockIdx.x * 128 + threadIdx.x, row = x / (D / 4);
+  if (row >= (int64_t)p.B * p.Hkv * rows_all) return;
+  const int d = (int)(x % (D / 4)) * 4;
+  const float* src = p.parts + row * p.outer * (D + 4);
+  float top = -INFINITY, sum = 0.f, v[4] = {};
+  for (int c = 0; c < p.outer; ++c) top = fmaxf(top, src[c * (D + 4) + D + 1]);
+  for (int c = 0; c < p.outer; ++c) {
+    const float4 y = *reinterpret_cast<const float4*>(src + c * (D + 4) + d);
+    const float2 st = *reinterpret_cast<const float2*>(src + c * (D + 4) + D);
+    const float f = st.y == -INFINITY ? 1.f : exp2_fast(st.y - top);
+    sum += st.x * f;
+    v[0] += y.x * f; v[1] += y.y * f; v[2] += y.z * f; v[3] += y.w * f;
+  }
+  const int64_t unit = row / rows_all;
+  const int r = (int)(row - unit * rows_all), i = p.by_heads(r), h = (int)(unit % p.Hkv) * G + r - i * G;
+  T o4[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o4[e] = ToF<T>::from(sum == 0.f ? 0.f : v[e] / sum);
+  *reinterpret_cast<uint2*>(out + ((unit / p.Hkv * p.n + i) * p.H + h) * D + d) = *reinterpret_cast<const uint2*>(o4);
 }
 
 struct PagedWriteParams {
@@ -538,20 +670,38 @@ bool rows_of_16_bytes(const void* ptr, std::initializer_list<int64_t> strides) {
   return true;
 }
 
-template <typename T, int D, int MT>
-int launch_paged(void* out, const void* q, const void* kp, const void* vp, PagedParams p, cudaStream_t stream) {
-  const int rows = p.n * (p.H / p.Hkv);
-  p.row_groups = (rows + 16 * MT - 1) / (16 * MT);
-  const long long units = (long long)p.B * p.Hkv * p.row_groups;
-  const long long cap = (long long)p.table_width * p.page_size;
-  const long long keys = p.window > 0 ? std::min(cap, (long long)p.window + p.sinks + p.n) : cap;
-  p.split = 1;
-  static const int target = std::getenv("B200_PAGED_TARGET") ? std::atoi(std::getenv("B200_PAGED_TARGET")) : 2 * kSMs;
-  while (p.split < kMaxSplit && units * p.split < target && keys > (long long)p.split * kPagedWarps * kStepKeys) p.split *= 2;
-  const long long grid = units * p.split;
-  if (grid > 2147483647ll) return (int)cudaErrorNotSupported;
-  constexpr int smem = kPagedWarps * kWarpRing + (MT > 1 ? MT * (D / 16) * 512 : 0);
-  auto kern = paged_attn_kernel<T, D, MT>;
+// How the keys of a row group are shared: CTAs of a cluster, and clusters whose parts a second kernel joins.
+struct PagedPlan {
+  int tiles;          // eights of rows of a CTA
+  long long groups;   // row groups of a (sequence, key head)
+  int split, outer;
+};
+PagedPlan paged_plan(const b200_paged_attn_t* a) {
+  PagedPlan p{};
+  const long long eights = ((long long)a->n * (a->H / a->Hkv) + 7) / 8;
+  p.groups = (eights + 3) / 4;
+  p.tiles = (int)((eights + p.groups - 1) / p.groups);
+  const long long units = (long long)a->B * a->Hkv * p.groups, cap = (long long)a->table_width * a->page_size;
+  const long long keys = a->window > 0 ? std::min(cap, (long long)a->window + a->sinks + a->n) : cap;
+  const long long slots = kSMs * (p.tiles <= 2 ? 3 : 2);      // CTAs that are resident at once
+  const long long most = std::max(1ll, keys / 64);            // a step for every warp of a share
+  p.outer = 1;
+  if (units * 16 < 2 * kSMs && keys > 16 * 1024) {
+    const long long shares = std::max(1ll, std::min(slots / units, keys / 256));
+    p.outer = (int)((shares + 7) / 8);
+    p.split = (int)(shares / p.outer);
+  } else {
+    // clusters of more than eight leave about a quarter of the places empty (a cluster lies within one group of SMs)
+    const long long one_wave = std::max(std::min(slots / units, 8ll), slots * 3 / 4 / units);
+    p.split = (int)std::min({std::max(one_wave, units < 2 * slots ? 2ll : 1ll), most, 16ll});
+  }
+  return p;
+}
+
+template <typename T, int D, int NT, bool kDense>
+int launch_paged(const PagedPlan& plan, void* out, const void* q, const void* kp, const void* vp, const PagedParams& p, cudaStream_t stream) {
+  constexpr int smem = kPagedWarps * std::max<int>(kWarpRing, 8 * NT * (D + 4) * 4);
+  auto kern = paged_attn_kernel<T, D, NT, kDense>;
   static OncePerDevice once;
   if (int e = once([&] {
         if (int r = opt_in_smem(kern, smem)) return r;
@@ -561,28 +711,45 @@ int launch_paged(void* out, const void* q, const void* kp, const void* vp, Paged
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = (unsigned)p.split;
+  attr.val.clusterDim.x = (unsigned)plan.split;
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cfg.gridDim = dim3((unsigned)grid);
+  cfg.gridDim = dim3((unsigned)(plan.groups * plan.split * plan.outer), (unsigned)p.Hkv, (unsigned)p.B);
   cfg.blockDim = dim3(kPagedWarps * 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cfg.attrs = &attr;
-  cfg.numAttrs = p.split > 1 ? 1 : 0;
+  cfg.numAttrs = plan.split > 1 ? 1 : 0;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, (T*)out, (const T*)q, (const T*)kp, (const T*)vp, p);
   if (e != cudaSuccess) {
     (void)cudaGetLastError();
     return (int)e;
   }
   note_launch();
-  return 0;
+  if (plan.outer == 1) return 0;
+  const long long threads = (long long)p.B * p.Hkv * p.n * (p.H / p.Hkv) * (D / 4);
+  paged_join_kernel<T, D><<<(unsigned)((threads + 127) / 128), 128, 0, stream>>>((T*)out, p);
+  B200K_LAUNCH_RET();
 }
 
-template <typename T>
-int launch_paged(int head_dim, void* out, const void* q, const void* kp, const void* vp, const PagedParams& p, cudaStream_t stream) {
-  const bool few = p.n * (p.H / p.Hkv) <= 16;
-  if (head_dim == 128) return few ? launch_paged<T, 128, 1>(out, q, kp, vp, p, stream) : launch_paged<T, 128, 2>(out, q, kp, vp, p, stream);
-  return few ? launch_paged<T, 64, 1>(out, q, kp, vp, p, stream) : launch_paged<T, 64, 2>(out, q, kp, vp, p, stream);
+template <typename T, int D>
+int launch_paged(const PagedPlan& plan, void* out, const void* q, const void* kp, const void* vp, const PagedParams& p, cudaStream_t stream) {
+  const bool dense = p.k_sr == D && p.v_sr == D;
+#define B200_PAGED_LAUNCH(NT) \
+  return dense ? launch_paged<T, D, NT, true>(plan, out, q, kp, vp, p, stream) : launch_paged<T, D, NT, false>(plan, out, q, kp, vp, p, stream)
+  switch (plan.tiles) {
+    case 1: B200_PAGED_LAUNCH(1);
+    case 2: B200_PAGED_LAUNCH(2);
+    case 3: B200_PAGED_LAUNCH(3);
+    default: B200_PAGED_LAUNCH(4);
+  }
+#undef B200_PAGED_LAUNCH
+}
+
+bool paged_sizes_ok(const b200_paged_attn_t* a) {
+  return (a->dtype == B200_BF16 || a->dtype == B200_F16) && (a->head_dim == 64 || a->head_dim == 128) && a->B > 0 && a->n > 0 && a->H > 0 &&
+         a->Hkv > 0 && a->H % a->Hkv == 0 && a->page_size > 0 && a->page_size % kPageRows == 0 && a->num_pages >= 0 && a->table_width > 0 &&
+         (long long)a->table_width * a->page_size <= 2147483647ll && a->sinks >= 0 && a->B <= 65535 && a->Hkv <= 65535 &&
+         (long long)a->n * (a->H / a->Hkv) <= (1 << 24);
 }
 
 }  // namespace
@@ -590,12 +757,15 @@ int launch_paged(int head_dim, void* out, const void* q, const void* kp, const v
 
 using namespace b200k;
 
+extern "C" int64_t b200_paged_attention_workspace(const b200_paged_attn_t* a) {
+  if (!paged_sizes_ok(a)) return 0;
+  const PagedPlan plan = paged_plan(a);
+  return plan.outer > 1 ? (int64_t)a->B * a->H * a->n * plan.outer * (a->head_dim + 4) : 0;
+}
+
 extern "C" int b200_paged_attention(const b200_paged_attn_t* a, void* out, const void* q, const void* k_pages, const void* v_pages,
-                                    const int* block_table, const int* seq_lens, int* status, cudaStream_t stream) {
-  if ((a->dtype != B200_BF16 && a->dtype != B200_F16) || (a->head_dim != 64 && a->head_dim != 128) || a->B <= 0 || a->n <= 0 ||
-      a->H <= 0 || a->Hkv <= 0 || a->H % a->Hkv != 0 || a->page_size <= 0 || a->page_size % 16 != 0 || a->num_pages < 0 ||
-      a->table_width <= 0 || (long long)a->table_width * a->page_size > 2147483647ll || a->sinks < 0)
-    return (int)cudaErrorNotSupported;
+                                    const int* block_table, const int* seq_lens, float* workspace, int* status, cudaStream_t stream) {
+  if (!paged_sizes_ok(a)) return (int)cudaErrorNotSupported;
   if (!rows_of_16_bytes(q, {a->q_sb, a->q_sn, a->q_sh}) || !rows_of_16_bytes(k_pages, {a->k_sp, a->k_sh, a->k_sr}) ||
       !rows_of_16_bytes(v_pages, {a->v_sp, a->v_sh, a->v_sr}) || !rows_of_16_bytes(out, {}))
     return (int)cudaErrorNotSupported;
@@ -611,11 +781,22 @@ extern "C" int b200_paged_attention(const b200_paged_attn_t* a, void* out, const
   p.table = block_table;
   p.lens = seq_lens;
   p.status = status;
-  p.page_shift = -1;
-  for (int x = 4; x < 31; ++x)
-    if (p.page_size == 1 << x) p.page_shift = x;
-  return a->dtype == B200_BF16 ? launch_paged<__nv_bfloat16>(a->head_dim, out, q, k_pages, v_pages, p, stream)
-                               : launch_paged<__half>(a->head_dim, out, q, k_pages, v_pages, p, stream);
+  const PagedPlan plan = paged_plan(a);
+  if (plan.outer > 1 && !workspace) return (int)cudaErrorInvalidValue;
+  if (plan.groups * plan.split * plan.outer > 2147483647ll) return (int)cudaErrorNotSupported;
+  p.by_page = fast_div((uint32_t)p.page_size);
+  p.by_heads = fast_div((uint32_t)(p.H / p.Hkv));
+  p.split = plan.split;
+  p.outer = plan.outer;
+  p.by_split = fast_div((uint32_t)plan.split);
+  p.by_outer = fast_div((uint32_t)plan.outer);
+  p.parts = workspace;
+  const bool wide = a->head_dim == 128;
+  if (a->dtype == B200_BF16)
+    return wide ? launch_paged<__nv_bfloat16, 128>(plan, out, q, k_pages, v_pages, p, stream)
+                : launch_paged<__nv_bfloat16, 64>(plan, out, q, k_pages, v_pages, p, stream);
+  return wide ? launch_paged<__half, 128>(plan, out, q, k_pages, v_pages, p, stream)
+              : launch_paged<__half, 64>(plan, out, q, k_pages, v_pages, p, stream);
 }
 
 extern "C" int b200_paged_rope_cache(const b200_paged_write_t* a, void* q_out, const void* q, const void* k, const void* v,
