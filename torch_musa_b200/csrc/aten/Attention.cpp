@@ -233,6 +233,12 @@ void window_desc(b200_attn_t& a, const char* op, bool causal, std::optional<int6
   a.window = (int)std::min<int64_t>(*window, 1 << 30);     // longer than any sequence
   a.sinks = (int)std::min<int64_t>(sinks, 1 << 30);
 }
+// Hidden scores are -inf before they are scaled, and maxima are taken there.
+double window_scale(const char* op, std::optional<double> scale) {
+  const double s = scale.value_or(1.0 / std::sqrt(128.0));
+  TORCH_CHECK(s > 0 && std::isfinite(s), op, ": the scale must be positive, got ", s);
+  return s;
+}
 
 void varlen_desc(b200_attn_t& a, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& cu_q,
                  const at::Tensor& cu_k, int64_t max_q, int64_t max_k, bool causal, std::optional<double> scale,
@@ -258,6 +264,7 @@ void varlen_desc(b200_attn_t& a, const at::Tensor& q, const at::Tensor& k, const
   a.total_q = (int)q.size(0);
   a.total_k = (int)k.size(0);
   window_desc(a, "varlen_attention", causal, window, sinks);
+  if (window.has_value()) window_scale("varlen_attention", scale);
 }
 
 // With a window there is an answer where nobody has a key or a query: zeros, and an lse of -inf.
@@ -345,7 +352,7 @@ void dense_window_desc(b200_attn_t& a, const char* op, const at::Tensor& q, cons
   a.Sq = (int)q.size(1); a.Sk = (int)k.size(1); a.head_dim = 128;
   a.dtype = kdtype(q.scalar_type());
   a.causal = 1;
-  a.scale = (float)scale.value_or(1.0 / std::sqrt(128.0));
+  a.scale = (float)window_scale(op, scale);
   a.q_sb = q.stride(0); a.q_sh = q.stride(2); a.q_ss = q.stride(1);
   a.k_sb = k.stride(0); a.k_sh = k.stride(2); a.k_ss = k.stride(1);
   a.v_sb = v.stride(0); a.v_sh = v.stride(2); a.v_ss = v.stride(1);

@@ -7,6 +7,7 @@
 #include "core/DeviceAssert.h"
 
 #include <ATen/Functions.h>
+#include <ATen/core/grad_mode.h>
 #include <torch/library.h>
 
 #include <algorithm>
@@ -17,6 +18,11 @@ namespace b200 {
 namespace ops {
 
 namespace {
+
+void check_no_grad(const char* op, std::initializer_list<const at::Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const at::Tensor* t : ts) TORCH_CHECK(!t->defined() || !t->requires_grad(), op, " has no gradient: call it under torch.no_grad()");
+}
 
 void check_int32(const char* op, const char* name, const at::Tensor& t, int64_t dim) {
   TORCH_CHECK(t.scalar_type() == at::kInt && t.dim() == dim && (t.numel() <= 1 || t.stride(-1) == 1), op, ": ", name, " must be int32 with ",
@@ -55,6 +61,7 @@ at::Tensor paged_attention(const at::Tensor& q_, const at::Tensor& k_pages, cons
   const char* op = "paged_attention";
   TORCH_CHECK(on_device(q_), op, ": expected a blackwell tensor, got ", q_.device());
   check_devices(op, q_, k_pages, v_pages, block_table, seq_lens);
+  check_no_grad(op, {&q_, &k_pages, &v_pages});
   TORCH_CHECK(q_.dim() == 4, op, ": q must be [sequences, new tokens, heads, head_dim], got ", q_.sizes());
   const int64_t B = q_.size(0), n = q_.size(1), H = q_.size(2), D = q_.size(3);
   TORCH_CHECK((q_.scalar_type() == at::kBFloat16 || q_.scalar_type() == at::kHalf) && (D == 64 || D == 128), op,
@@ -66,6 +73,7 @@ at::Tensor paged_attention(const at::Tensor& q_, const at::Tensor& k_pages, cons
   TORCH_CHECK(block_table.size(0) == B && seq_lens.size(0) == B, op, ": block_table and seq_lens must have a row per sequence");
   TORCH_CHECK(!window.has_value() || *window > 0, op, ": window must be positive");
   TORCH_CHECK(sinks >= 0, op, ": sinks must not be negative");
+  TORCH_CHECK(!scale.has_value() || (*scale > 0 && std::isfinite(*scale)), op, ": the scale must be positive, got ", scale.value_or(0.0));
   TORCH_CHECK(block_table.size(1) <= INT_MAX / k_pages.size(2), op, ": block_table covers more than 2^31 tokens");
   if (block_table.size(1) == 0) return at::zeros({B, n, H, D}, q_.options());
   at::Tensor out = at::empty({B, n, H, D}, q_.options());
@@ -102,6 +110,7 @@ at::Tensor paged_rope_cache(const at::Tensor& q_, const at::Tensor& k_, const at
   const char* op = "paged_rope_cache";
   TORCH_CHECK(on_device(q_), op, ": expected a blackwell tensor, got ", q_.device());
   check_devices(op, q_, k_, v_, cos, sin, k_pages, v_pages, block_table, seq_lens, cu_seqlens);
+  check_no_grad(op, {&q_, &k_, &v_, &k_pages, &v_pages});
   TORCH_CHECK(q_.dim() == 3 && k_.dim() == 3 && v_.sizes() == k_.sizes() && k_.size(0) == q_.size(0) && k_.size(2) == q_.size(2), op,
               ": q must be [tokens, heads, head_dim], k and v [tokens, kv heads, head_dim], got ", q_.sizes(), ", ", k_.sizes(), " and ",
               v_.sizes());
@@ -166,6 +175,8 @@ std::tuple<at::Tensor, at::Tensor> verify_drafts(const at::Tensor& target_, cons
               ": draft_tokens must be int64 [sequences, drafts]");
   TORCH_CHECK(uniforms_.scalar_type() == at::kFloat && uniforms_.dim() == 2 && uniforms_.size(0) == B && uniforms_.size(1) == n + 1, op,
               ": uniforms must be float32 [sequences, drafts + 1]");
+  check_no_grad(op, {&target_});
+  if (draft_.has_value()) check_no_grad(op, {&*draft_});
   auto rows = [](const at::Tensor& t) { return t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous(); };
   const at::Tensor target = rows(target_), tokens = rows(tokens_), uniforms = rows(uniforms_);
   at::Tensor draft;

@@ -433,6 +433,15 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
           uint32_t raw[32], pk[16];
           tmem_ld32(s_addr + (uint32_t)(c * 32), raw);
           tmem_ld_wait();
+          if constexpr (kWin) {      // as in the forward: what is not seen becomes -inf, and the block goes the common way
+            if (masked) {
+              const int q = q0 + wg * 64 + c * 32;
+              const uint32_t seen = key_off ? 0u : low_bits(far - q) & ~low_bits(kj - q);
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (!((seen >> e) & 1u)) raw[e] = 0xff800000u;
+            }
+          }
 #pragma unroll
           for (int e4 = 0; e4 < 8; ++e4) {
             const float4 nl = nlse4[c * 8 + e4];
@@ -445,8 +454,8 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
               float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
               if constexpr (decltype(mask)::value) {
                 const int qi = q0 + wg * 64 + cc;
-                if (key_off || (p.causal && qi < kj) || (kWin && qi >= far)) p0 = 0.f;
-                if (key_off || (p.causal && qi + 1 < kj) || (kWin && qi + 1 >= far)) p1 = 0.f;
+                if (key_off || (p.causal && qi < kj)) p0 = 0.f;
+                if (key_off || (p.causal && qi + 1 < kj)) p1 = 0.f;
               }
               pf[cc] = p0;
               pf[cc + 1] = p1;
@@ -456,8 +465,12 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
           tmem_st16(s_addr + (uint32_t)(c * 16), pk);   // over columns of S^T that this thread has read
         }
       };
-      if (masked) probs(std::true_type{});
-      else probs(std::false_type{});
+      if constexpr (kWin) {
+        probs(std::false_type{});
+      } else {
+        if (masked) probs(std::true_type{});
+        else probs(std::false_type{});
+      }
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();

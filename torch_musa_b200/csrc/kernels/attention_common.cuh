@@ -104,6 +104,8 @@ __device__ __forceinline__ void mul2(float& d0, float& d1, float x0, float x1, f
       : "=f"(d0), "=f"(d1)
       : "f"(x0), "f"(x1), "f"(y0), "f"(y1));
 }
+// the n lowest bits, for any n
+__device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u); }
 // two floats to one packed pair of 16-bit values (one conversion instruction)
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float a, float b);

@@ -301,12 +301,25 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
       lim = max(0, min(lim, AK));
       const int hide0 = kWin ? max(0, p.sinks - k0) : 0, hide1 = kWin ? qi - p.window + 1 - k0 : 0;
       const bool full = __all_sync(0xffffffffu, lim == AK && hide0 >= hide1);
-      auto hidden = [&](int e) { return e >= lim || (kWin && e >= hide0 && e < hide1); };
       // the whole row of scores in registers
       uint32_t raw[4][32];
 #pragma unroll
       for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + (uint32_t)(c * 32), raw[c]);
       tmem_ld_wait();
+      // kWin: what the row does not see becomes -inf here, two instructions an element, and the block goes the common way.  The tests
+      // inside the loops below, three times for each element, are four times the code, and a windowed CTA meets a masked block so
+      // often that it waits for instructions: 32 heads x 4096, window 64, 174 us with them.
+      if constexpr (kWin) {
+        if (!full) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const uint32_t seen = low_bits(lim - c * 32) & ~(low_bits(hide1 - c * 32) & ~low_bits(hide0 - c * 32));
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (!((seen >> e) & 1u)) raw[c][e] = 0xff800000u;
+          }
+        }
+      }
       // P = exp2(S * scale - m) as bf16 / fp16 pairs over the first 64 columns of S; packed fp32 arithmetic, one
       // special-function instruction per exponential, one conversion per pair.  Two instantiations: with the mask test
       // inside one, every element pays a compare and a select.
@@ -319,8 +332,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
           fma2(x0, x1, __uint_as_float(raw[c][e]), __uint_as_float(raw[c][e + 1]), p.scale_log2, neg_m);
           float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
           if constexpr (decltype(masked)::value) {
-            if (hidden(c * 32 + e)) p0 = 0.f;
-            if (hidden(c * 32 + e + 1)) p1 = 0.f;
+            if (c * 32 + e >= lim) p0 = 0.f;
+            if (c * 32 + e + 1 >= lim) p1 = 0.f;
           }
           add2(l0, l1, p0, p1);
           pk[c][e >> 1] = pack2<T>(p0, p1);
@@ -341,8 +354,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
           for (int e = 0; e < 32; e += 2) {
             float a = __uint_as_float(raw[c][e]), b2 = __uint_as_float(raw[c][e + 1]);
             if constexpr (decltype(masked)::value) {
-              if (hidden(c * 32 + e)) a = -INFINITY;
-              if (hidden(c * 32 + e + 1)) b2 = -INFINITY;
+              if (c * 32 + e >= lim) a = -INFINITY;
+              if (c * 32 + e + 1 >= lim) b2 = -INFINITY;
             }
             mx[(e >> 1) & 3] = max3(mx[(e >> 1) & 3], a, b2);
           }
@@ -384,8 +397,12 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
           tmem_st16(s_addr + (uint32_t)(c * 16), pk[c]);
         }
       };
-      if (full) block(std::false_type{});
-      else block(std::true_type{});
+      if constexpr (kWin) {
+        block(std::false_type{});
+      } else {
+        if (full) block(std::false_type{});
+        else block(std::true_type{});
+      }
       l_run += l0 + l1;
       tmem_st_wait();
       tc_fence_before();

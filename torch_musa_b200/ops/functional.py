@@ -354,7 +354,9 @@ def scaled_dot_product_attention(q, k, v, attn_mask=None, dropout_p: float = 0.0
 
 
 # ------------------------------------------------------------------------- windowed and packed variable-length attention
-def _check_window(causal: bool, window: Optional[int], sinks: int) -> None:
+def _check_window(causal: bool, window: Optional[int], sinks: int, scale: Optional[float]) -> None:
+    if scale is not None and window is not None and not 0 < scale < math.inf:
+        raise ValueError(f"the softmax scale must be positive, got {scale}")
     if sinks < 0:
         raise ValueError(f"sinks must not be negative, got {sinks}")
     if window is not None:
@@ -398,7 +400,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     returns [B, Sq, H, D], zeros for a query that sees no key.  On the blackwell device with D = 128 and bf16 / fp16 the
     tensor-core kernels skip the blocks of keys outside the mask, in both directions (gradients of dq are summed in
     fp32 in the order in which blocks arrive); otherwise it is ``scaled_dot_product_attention`` with the mask."""
-    _check_window(True, window, sinks)
+    _check_window(True, window, sinks, softmax_scale)
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3] or k.shape[2] == 0 or q.shape[2] % k.shape[2]:
         raise ValueError(f"window_attention: q [B, Sq, H, D] and k, v [B, Sk, Hkv, D] with Hkv a divisor of H expected, got "
                          f"{tuple(q.shape)}, {tuple(k.shape)} and {tuple(v.shape)}")
@@ -440,7 +442,7 @@ def flash_attn_varlen_func(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu
     otherwise the sequences are processed one by one with ``scaled_dot_product_attention``.  A causal mask compares
     positions inside a sequence (key index <= query index); ``window`` and ``sinks`` narrow it as in
     ``window_attention``, and rows past the last sequence then get zeros, in the gradients too."""
-    _check_window(causal, window, sinks)
+    _check_window(causal, window, sinks, softmax_scale)
     if _native_attention(q, k, v):
         return _VarlenAttention.apply(q, k, v, cu_seqlens_q.to(torch.int32), cu_seqlens_k.to(torch.int32),
                                       int(max_seqlen_q), int(max_seqlen_k), bool(causal), softmax_scale, window, int(sinks))
@@ -462,7 +464,7 @@ def flash_attn_varlen_func(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu
 
 
 # ------------------------------------------------------------------------- paged key-value cache
-def _no_grad_inputs(op: str, *tensors) -> None:
+def _no_grad_inputs(op: str, *tensors) -> None:      # on the device the operators say so themselves
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"{op} has no gradient: call it under torch.no_grad()")
 
@@ -484,9 +486,9 @@ def paged_rope_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: tor
     zeros come back for them and nothing is written.  A page number outside the pool or a position outside the tables is
     reported by the next ``synchronize()`` (the row is not written; the last angle is used).  Sequences do not
     share the pages that they write."""
-    _no_grad_inputs("paged_rope_cache", q, k, v)
     if _paged_native(q):
         return torch.ops.blackwell.paged_rope_cache(q, k, v, cos, sin, k_pages, v_pages, block_table, seq_lens, cu_seqlens)
+    _no_grad_inputs("paged_rope_cache", q, k, v)
     T, B, page = q.shape[0], seq_lens.shape[0], k_pages.shape[2]
     t = torch.arange(T, device=q.device)
     if cu_seqlens is None:
@@ -533,10 +535,12 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     read: others may already belong to someone else, and their table entries may be anything.  A token that sees no key
     (an empty sequence) gets zeros.  The keys of a page number outside the pool are hidden, which the next ``synchronize()``
     reports."""
-    _check_window(True, window, sinks)
-    _no_grad_inputs("paged_attention", q, k_pages, v_pages)
+    _check_window(True, window, sinks, softmax_scale)
+    if softmax_scale is not None and not 0 < softmax_scale < math.inf:
+        raise ValueError(f"the softmax scale must be positive, got {softmax_scale}")
     if _paged_native(q):
-        return torch.ops.blackwell.paged_attention(q, k_pages, v_pages, block_table, seq_lens, window, int(sinks), softmax_scale)
+        return torch.ops.blackwell.paged_attention(q, k_pages, v_pages, block_table, seq_lens, window, sinks, softmax_scale)
+    _no_grad_inputs("paged_attention", q, k_pages, v_pages)
     B, n, H, D = q.shape
     pages, Hkv, page, _ = k_pages.shape
     L = block_table.shape[1] * page
@@ -582,9 +586,9 @@ def verify_drafts(target_probs: torch.Tensor, draft_tokens: torch.Tensor, unifor
 
     Returns ``(taken [B], tokens [B, n + 1])``, both int64: the taken drafts, the drawn token, then -1.  Where a row has no
     weight at all (zeros or NaN) the drawn token is -1."""
-    _no_grad_inputs("verify_drafts", target_probs, draft_probs)
     if _on_device(target_probs) and target_probs.dtype in (torch.float32, torch.bfloat16, torch.float16):
         return torch.ops.blackwell.verify_drafts(target_probs, draft_tokens, uniforms, draft_probs)
+    _no_grad_inputs("verify_drafts", target_probs, draft_probs)
     B, n1, V = target_probs.shape
     n, x, u = n1 - 1, draft_tokens, uniforms.double()
     if tuple(x.shape) != (B, n) or tuple(u.shape) != (B, n1) or (draft_probs is not None and tuple(draft_probs.shape) != (B, n, V)):
