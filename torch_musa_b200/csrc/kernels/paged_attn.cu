@@ -48,9 +48,7 @@ struct PagedParams {
 
 constexpr int kPagedWarps = 4;
 constexpr int kPageRows = 16;          // rows of a page come in multiples of this
-constexpr int kStageBytes = 8192;      // keys and values of one step of a warp: 16 keys of 128 dimensions, 32 of 64
-constexpr int kStages = 2;
-constexpr int kWarpRing = kStages * kStageBytes;
+constexpr int kWarpRing = 16 * 1024;   // keys and values that a warp has in flight or in hand
 constexpr float kRaise = 8.f;          // log2: how far a score may exceed the reference maximum
 
 __device__ __forceinline__ uint32_t shared_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -94,6 +92,9 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
+__device__ __forceinline__ void zero16(uint32_t a) { asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(a), "r"(0) : "memory"); }
+// the n lowest bits, for any n
+__device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u); }
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -126,7 +127,7 @@ __device__ __forceinline__ bool not_finite(uint32_t w) {
 }
 
 // One CTA: one row group (up to 8 * NT rows = new tokens x query heads of a key head) of one (sequence, key head), one of several
-// contiguous shares of the visible keys.  A share is cut into steps of 16 keys (32 when D is 64) that the four warps take in turn;
+// contiguous shares of the visible keys.  A share is cut into steps of 16 keys (32 when D is 64 and the rows few) that the four warps take in turn;
 // each warp runs its own online softmax, the warps join through shared memory and the CTAs of a cluster through distributed shared
 // memory.  A warp copies the rows of keys and of values of a step into a stage of its own ring (cp.async, whole rows at a time,
 // 16-byte pieces swapped by row so that the eight rows of a matrix lie in different banks).  The products are mma m16n8k16 with the
@@ -139,9 +140,10 @@ __device__ __forceinline__ bool not_finite(uint32_t w) {
 // kDense: the rows of a page follow one another (the layout of the pools as they are made), so that a copy's address is a constant
 // away from the page's.
 template <typename T, int D, int NT, bool kDense>
-__global__ void __launch_bounds__(kPagedWarps * 32, NT <= 2 ? 3 : 2) paged_attn_kernel(T* __restrict__ out, const T* __restrict__ q, const T* __restrict__ kp,
+__global__ void __launch_bounds__(kPagedWarps * 32, NT * D <= 256 ? 3 : 2) paged_attn_kernel(T* __restrict__ out, const T* __restrict__ q, const T* __restrict__ kp,
                                                                          const T* __restrict__ vp, const PagedParams p) {
-  constexpr int kRows = 8 * NT, kHalves = kStageBytes / (kPageRows * D * 4), kKeys = kHalves * kPageRows, kHalf = kPageRows * D * 2;
+  constexpr int kRows = 8 * NT, kHalves = D == 64 && NT <= 2 ? 2 : 1, kKeys = kHalves * kPageRows, kHalf = kPageRows * D * 2;
+  constexpr int kStageBytes = 2 * kHalves * kHalf, kStages = kWarpRing / kStageBytes;
   constexpr int kPad = D + 4;            // floats of a row of a part: the four lanes' rows then lie in different banks
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ float s_m[kPagedWarps][kRows], s_l[kPagedWarps][kRows];
@@ -210,33 +212,17 @@ __global__ void __launch_bounds__(kPagedWarps * 32, NT <= 2 ? 3 : 2) paged_attn_
         const T* ks = kbase + (uint64_t)page * (uint64_t)p.k_sp + (kDense ? row * D : (uint64_t)row * (uint64_t)p.k_sr);
         const T* vs = vbase + (uint64_t)page * (uint64_t)p.v_sp + (kDense ? row * D : (uint64_t)row * (uint64_t)p.v_sr);
         const uint32_t dst = ring + stage * kStageBytes + x * kHalf;
-        // keys that no row sees are not read: zeros instead (with a probability of zero nothing else would be safe)
-        auto copy = [&](auto whole) {
+        const int n16 = there ? 16 : 0;        // a page that is not there: zeros
 #pragma unroll
-          for (int i = 0; i < kPageRows / kPerCopy; ++i) {
-            const int j = k0 + i * kPerCopy + crow;
-            const int n16 = decltype(whole)::value || (there && j <= pos1 && (j >= wlo || j < p.sinks)) ? 16 : 0;
-            const uint32_t d = dst + cdst[i % kSwaps] + (uint32_t)(i * kPerCopy * D * 2);
-            copy16(d, ks + (kDense ? i * kPerCopy * D : i * kPerCopy * p.k_sr), n16);
-            copy16(d + kHalves * kHalf, vs + (kDense ? i * kPerCopy * D : i * kPerCopy * p.v_sr), n16);
-          }
-        };
-        if (there && k0 + kPageRows - 1 <= pos1 && (k0 >= wlo || k0 + kPageRows <= p.sinks)) copy(std::true_type{});
-        else copy(std::false_type{});
+        for (int i = 0; i < kPageRows / kPerCopy; ++i) {
+          const uint32_t d = dst + cdst[i % kSwaps] + (uint32_t)(i * kPerCopy * D * 2);
+          copy16(d, ks + (kDense ? i * kPerCopy * D : i * kPerCopy * p.k_sr), n16);
+          copy16(d + kHalves * kHalf, vs + (kDense ? i * kPerCopy * D : i * kPerCopy * p.v_sr), n16);
+        }
       }
     }
     copy_commit();
   };
-  int s = s0 + warp, fetch = s;
-  Pages number = entry(fetch);
-#pragma unroll
-  for (int st = 0; st < kStages; ++st) {
-    const Pages now = number;
-    number = entry(fetch + kPagedWarps);
-    issue(fetch, now, st);
-    fetch += kPagedWarps;
-  }
-
   // Q as operands: row g of each eight, dimensions 16 ks + 2 t and 8 further
   uint32_t qf[NT][D / 16][2];
 #pragma unroll
@@ -260,8 +246,12 @@ __global__ void __launch_bounds__(kPagedWarps * 32, NT <= 2 ? 3 : 2) paged_attn_
     l_run[nt][0] = l_run[nt][1] = 0.f;
   }
 
+  // The first passes only fill the ring, so that the code of the copies is there once: a CTA has few steps, and code that it meets
+  // for the first time costs more than what it does.
+  Pages number = entry(s0 + warp);
   int stage = 0;
-  for (; s < s1; s += kPagedWarps) {
+  for (int s = s0 + warp - kStages * kPagedWarps; s < s1; s += kPagedWarps) {
+    if (s >= s0) {
     copy_wait<kStages - 1>();
     __syncwarp();
     const int k0 = key_of(s);
@@ -301,18 +291,33 @@ __global__ void __launch_bounds__(kPagedWarps * 32, NT <= 2 ? 3 : 2) paged_attn_
     auto values = [&](int j, int x) { return ldmatrix_t(va[j & 3] + (j >> 2) * 128 + x * kHalf); };
     const uint32_t pages = (found >> (stage * kHalves)) & ((1u << kHalves) - 1u);
     const bool all = pages == (1u << kHalves) - 1u && k0 + kKeys - 1 <= pos0 && (p.window <= 0 || k0 > pos1 - p.window || k0 + kKeys <= p.sinks);
-    auto sees = [&](int ps, int j) {
-      return ((pages >> ((j - k0) / kPageRows)) & 1u) && j <= ps && (p.window <= 0 || j > ps - p.window || j < p.sinks);
+    // bit j: a token at position ps sees key k0 + j
+    auto sees = [&](int ps) {
+      const uint32_t there = kHalves == 1 ? (pages ? 0xffffu : 0u) : (pages & 1u ? 0xffffu : 0u) | (pages & 2u ? 0xffff0000u : 0u);
+      return there & low_bits(ps + 1 - k0) & ~(p.window > 0 ? low_bits(ps - p.window + 1 - k0) & ~low_bits(p.sinks - k0) : 0u);
     };
     bool careful = false;
     if (!all) {
+      // Values that no row sees become zero: with a probability of zero nothing else would be safe.
+      // Some row sees a key when it is not past the newest token, and a sink or not in front of the oldest one's window.
+      const uint32_t unseen = ~(low_bits(pos1 + 1 - k0) & ~(low_bits(wlo - k0) & ~low_bits(p.sinks - k0))) & (kKeys == 32 ? ~0u : 0xffffu);
+      if (unseen) {
+#pragma unroll
+        for (int i = 0; i < kKeys / kPerCopy; ++i)
+          if ((unseen >> (i * kPerCopy + crow)) & 1u) zero16(ring + at + kHalves * kHalf + (uint32_t)(crow * D * 2 + cpiece * 16 + i * kPerCopy * D * 2));
+        __syncwarp();
+      }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int x = 0; x < kHalves; ++x)
+        for (int e = 0; e < 2; ++e) {
+          const uint32_t w = sees(pos[nt][e]) >> g;
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (!sees(pos[nt][e & 1], k0 + x * kPageRows + (e >> 1) * 8 + g)) sc[x][nt][e] = -INFINITY;
+          for (int x = 0; x < kHalves; ++x)
+#pragma unroll
+            for (int k8 = 0; k8 < 2; ++k8)
+              if (!((w >> (x * 16 + k8 * 8)) & 1u)) sc[x][nt][k8 * 2 + e] = -INFINITY;
+        }
       if (pos0 != pos1) {            // rows differ in what they see
         bool odd = false;
 #pragma unroll 1
@@ -400,9 +405,9 @@ __global__ void __launch_bounds__(kPagedWarps * 32, NT <= 2 ? 3 : 2) paged_attn_
       for (int ps = pos0; ps <= pos1; ++ps) {
 #pragma unroll
         for (int x = 0; x < kHalves; ++x) {
-          const int kx = k0 + x * kPageRows + 2 * t;
-          const uint32_t see0 = (sees(ps, kx) ? 0xffffu : 0u) | (sees(ps, kx + 1) ? 0xffff0000u : 0u);
-          const uint32_t see1 = (sees(ps, kx + 8) ? 0xffffu : 0u) | (sees(ps, kx + 9) ? 0xffff0000u : 0u);
+          const uint32_t w = sees(ps) >> (x * 16 + 2 * t);
+          const uint32_t see0 = (w & 1u ? 0xffffu : 0u) | (w & 2u ? 0xffff0000u : 0u);
+          const uint32_t see1 = (w & 0x100u ? 0xffffu : 0u) | (w & 0x200u ? 0xffff0000u : 0u);
 #pragma unroll
           for (int j = 0; j < D / 16; ++j) {
             const uint4 v = values(j, x);
@@ -422,10 +427,10 @@ __global__ void __launch_bounds__(kPagedWarps * 32, NT <= 2 ? 3 : 2) paged_attn_
       }
     }
     __syncwarp();
+    }
     const Pages now = number;
-    number = entry(fetch + kPagedWarps);
-    issue(fetch, now, stage);
-    fetch += kPagedWarps;
+    number = entry(s + (kStages + 1) * kPagedWarps);
+    issue(s + kStages * kPagedWarps, now, stage);
     if (++stage == kStages) stage = 0;
   }
 
@@ -683,7 +688,7 @@ PagedPlan paged_plan(const b200_paged_attn_t* a) {
   p.tiles = (int)((eights + p.groups - 1) / p.groups);
   const long long units = (long long)a->B * a->Hkv * p.groups, cap = (long long)a->table_width * a->page_size;
   const long long keys = a->window > 0 ? std::min(cap, (long long)a->window + a->sinks + a->n) : cap;
-  const long long slots = kSMs * (p.tiles <= 2 ? 3 : 2);      // CTAs that are resident at once
+  const long long slots = kSMs * (p.tiles * a->head_dim <= 256 ? 3 : 2);      // CTAs that are resident at once
   const long long most = std::max(1ll, keys / 64);            // a step for every warp of a share
   p.outer = 1;
   if (units * 16 < 2 * kSMs && keys > 16 * 1024) {
