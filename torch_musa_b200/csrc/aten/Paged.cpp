@@ -137,7 +137,7 @@ at::Tensor paged_rope_cache(const at::Tensor& q_, const at::Tensor& k_, const at
   if (B == 0) return at::zeros({T, H, D}, q_.options());
   at::Tensor out = at::empty({T, H, D}, q_.options());
   if (T == 0) return out;
-  const at::Tensor q = aligned_rows(q_), k = aligned_rows(k_), v = aligned_rows(v_);
+  const at::Tensor q = aligned_rows(q_), k = aligned_rows(k_), v = aligned_rows(v_), cosr = aligned_rows(cos), sinr = aligned_rows(sin);
   b200_paged_write_t a{};
   a.dtype = kdtype(q.scalar_type());
   a.head_dim = (int)D;
@@ -154,7 +154,7 @@ at::Tensor paged_rope_cache(const at::Tensor& q_, const at::Tensor& k_, const at
   a.table_sb = block_table.stride(0);
   DeviceSwitch sw(q.device().index());
   const int e = b200_paged_rope_cache(&a, out.mutable_data_ptr(), q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(),
-                                      cos.const_data_ptr<float>(), sin.const_data_ptr<float>(), k_pages.mutable_data_ptr(),
+                                      cosr.const_data_ptr<float>(), sinr.const_data_ptr<float>(), k_pages.mutable_data_ptr(),
                                       v_pages.mutable_data_ptr(), block_table.const_data_ptr<int>(), seq_lens.const_data_ptr<int>(),
                                       packed ? cu_seqlens->const_data_ptr<int>() : nullptr, device_assert_word(q.device().index()),
                                       current_raw_stream(q));
