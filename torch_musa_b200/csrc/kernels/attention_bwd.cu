@@ -68,6 +68,7 @@ struct BwdParams {
   int total_q;
   // kWin: key j is visible when j <= i and (i - j < window or j < sinks)
   int window, sinks, total_k;
+  int units;                      // units of work that the CTAs share
   int sink_blocks, sink_chunks;   // key blocks with sinks, CTAs that share the query blocks of one of them
   float* sink_ws;                 // sink_chunks > 1: fp32 [B * Hkv][sink_blocks][sink_chunks][dV, dK][128][128]
 };
@@ -136,56 +137,87 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
   uint64_t* all_done = bars + 13;            // tcgen05.commit: dV, dK complete
   uint64_t* ld_full = bars + 14;             // [2]  lse and delta of a query block are there
   uint64_t* ld_empty = bars + 16;            // [2]  8 warps
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 18);
+  uint64_t* acc_empty = bars + 18;           // 8 warps: dV and dK of the unit are in registers
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 19);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // all (batch, head) instances of the earliest key block first: under a causal mask it meets the most query blocks
-  const int n_bh = p.B * p.Hkv;
-  int kb = (int)(blockIdx.x / n_bh), chunk = 0;
-  if constexpr (kWin) {              // kb counts (block with sinks, chunk) pairs first
-    const int pairs = p.sink_blocks * p.sink_chunks;
-    if (kb < pairs) {
-      chunk = kb % p.sink_chunks;
-      kb /= p.sink_chunks;
-    } else {
-      kb -= pairs - p.sink_blocks;
-    }
-  }
-  const int bh = (int)(blockIdx.x % n_bh);
-  const int b = bh / p.Hkv, hk = bh - b * p.Hkv;
-  const int G = p.H / p.Hkv;
-  const int k0 = kb * BK;
-  // this instance's sequence (see the forward kernel): rows past a packed sequence's end are loaded, masked by index
-  // (their probabilities and score gradients are exact zeros) and never stored
-  int Sq = p.Sq, Sk = p.Sk, qoff = 0, koff = 0, bt = b, q_blocks = p.q_blocks;
-  if (p.cu_q) {
-    qoff = p.cu_q[b];
-    Sq = p.cu_q[b + 1] - qoff;
-    koff = p.cu_k[b];
-    Sk = p.cu_k[b + 1] - koff;
-    bt = 0;
-    q_blocks = (Sq + BQ - 1) / BQ;
-  }
-  int i0 = p.causal ? min(q_blocks, k0 / BQ) : 0;   // first query block that sees these keys
-  int n_i = k0 < Sk ? q_blocks - i0 : 0;            // a key block past the sequence's end has nothing to do
-  int n_it = n_i * G, h0 = hk * G, istart = 0;
+  // One unit of work: a key block of one (batch, kv head), or a chunk of one.  All (batch, head) instances of the earliest key block
+  // come first: under a causal mask it meets the most query blocks.
+  const int n_bh = p.B * p.Hkv, G = p.H / p.Hkv;
+  int kb = 0, chunk = 0, bh = 0, b = 0, hk = 0, k0 = 0;
+  int Sq = 0, Sk = 0, qoff = 0, koff = 0, bt = 0;
+  int i0 = 0, n_i = 0, n_it = 0, h0 = 0, istart = 0;      // first query block, query blocks, pairs, where the pairs start
   bool partial = false;
-  if constexpr (kWin) {
-    int end;
-    window_queries(p, kb, Sq, Sk, q_blocks, i0, end);
-    n_i = end - i0;
-    n_it = n_i * G;
-    if (kb < p.sink_blocks && p.sink_chunks > 1) {     // pairs [chunk * per, (chunk + 1) * per) of this block's
-      partial = true;
-      const int per = (n_it + p.sink_chunks - 1) / p.sink_chunks, from = min(n_it, chunk * per);
-      n_it = min(n_it, from + per) - from;
-      if (n_i > 0) {
-        h0 += from / n_i;
-        istart = from % n_i;
+  auto set_unit = [&](int unit) {
+    kb = unit / n_bh;
+    if constexpr (kWin) {            // kb counts (block with sinks, chunk) pairs first
+      const int pairs = p.sink_blocks * p.sink_chunks;
+      chunk = 0;
+      if (kb < pairs) {
+        chunk = kb % p.sink_chunks;
+        kb /= p.sink_chunks;
+      } else {
+        kb -= pairs - p.sink_blocks;
       }
     }
-  }
+    bh = unit % n_bh;
+    b = bh / p.Hkv;
+    hk = bh - b * p.Hkv;
+    k0 = kb * BK;
+    // this instance's sequence (see the forward kernel): rows past a packed sequence's end are loaded, masked by index
+    // (their probabilities and score gradients are exact zeros) and never stored
+    Sq = p.Sq;
+    Sk = p.Sk;
+    bt = b;
+    int q_blocks = p.q_blocks;
+    if (p.cu_q) {
+      qoff = p.cu_q[b];
+      Sq = p.cu_q[b + 1] - qoff;
+      koff = p.cu_k[b];
+      Sk = p.cu_k[b + 1] - koff;
+      bt = 0;
+      q_blocks = (Sq + BQ - 1) / BQ;
+    }
+    i0 = p.causal ? min(q_blocks, k0 / BQ) : 0;       // first query block that sees these keys
+    n_i = k0 < Sk ? q_blocks - i0 : 0;                // a key block past the sequence's end has nothing to do
+    n_it = n_i * G;
+    h0 = hk * G;
+    if constexpr (kWin) {
+      int end;
+      window_queries(p, kb, Sq, Sk, q_blocks, i0, end);
+      n_i = end - i0;
+      n_it = n_i * G;
+      istart = 0;
+      partial = kb < p.sink_blocks && p.sink_chunks > 1;
+      if (partial) {                                  // pairs [chunk * per, (chunk + 1) * per) of this block's
+        const int per = (n_it + p.sink_chunks - 1) / p.sink_chunks, from = min(n_it, chunk * per);
+        n_it = min(n_it, from + per) - from;
+        if (n_i > 0) {
+          h0 += from / n_i;
+          istart = from % n_i;
+        }
+      }
+    }
+  };
+  // Calls f() for every unit of this CTA until it returns false.  Without a window a CTA has one unit.  With one the units are short
+  // (nine pairs at a window of 1024), and starting and ending a CTA cost as much as three or four of them: then a CTA stays on its
+  // SM and takes every 148th unit, turning round at either end so that long and short ones even out, and the loads, the first
+  // products and the exponentials of a unit run while the one before it is stored.
+  auto each_unit = [&](auto f) {
+    if constexpr (!kWin) {
+      set_unit((int)blockIdx.x);
+      f();
+    } else {
+      for (int round = 0;; ++round) {
+        const int unit = round * (int)gridDim.x + (round & 1 ? (int)(gridDim.x - 1 - blockIdx.x) : (int)blockIdx.x);
+        if (round * (int)gridDim.x >= p.units) break;
+        if (unit >= p.units) continue;
+        set_unit(unit);
+        if (!f()) break;
+      }
+    }
+  };
 
   if (threadIdx.x == 0) {
     *abort_flag = 0;
@@ -205,6 +237,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
     mbar_init(dq_full, 1);
     mbar_init(dq_drained, 4);
     mbar_init(all_done, 1);
+    mbar_init(acc_empty, 8);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     prefetch_tmap(&tmap_q);
     prefetch_tmap(&tmap_k);
@@ -226,25 +259,38 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
     regs_dec<kOtherRegs>();
     if (warp == 12) {
       // ------------------------------------------------------------ TMA producer
-      if (lane == 0 && n_it > 0) {
-        mbar_expect_tx(kv_full, 2 * kTile);
-        tma_load_4d(sK, &tmap_k, kv_full, 0, koff + k0, hk, bt);
-        tma_load_4d(sK + kTile / 2, &tmap_k, kv_full, 64, koff + k0, hk, bt);
-        tma_load_4d(sV, &tmap_v, kv_full, 0, koff + k0, hk, bt);
-        tma_load_4d(sV + kTile / 2, &tmap_v, kv_full, 64, koff + k0, hk, bt);
-        int h = h0, i = istart;
-        for (int it = 0; it < n_it; ++it) {
-          const int q0 = (i0 + i) * BQ, st = it & 1;
-          if (!mbar_wait(&q_empty[st], (uint32_t)(((it >> 1) & 1) ^ 1), abort_flag)) break;
-          mbar_expect_tx(&q_full[st], kTile);
-          tma_load_4d(sQ + st * kTile, &tmap_q, &q_full[st], 0, qoff + q0, h, bt);
-          tma_load_4d(sQ + st * kTile + kTile / 2, &tmap_q, &q_full[st], 64, qoff + q0, h, bt);
-          if (!mbar_wait(do_empty, (uint32_t)((it & 1) ^ 1), abort_flag)) break;
-          mbar_expect_tx(do_full, kTile);
-          tma_load_4d(sdO, &tmap_do, do_full, 0, qoff + q0, h, bt);
-          tma_load_4d(sdO + kTile / 2, &tmap_do, do_full, 64, qoff + q0, h, bt);
-          if (++i == n_i) { i = 0; ++h; }
-        }
+      if (lane == 0) {
+        int gi = 0, live = 0;            // pairs and units with pairs so far: the phases of the barriers
+        auto load_kv = [&]() {
+          mbar_expect_tx(kv_full, 2 * kTile);
+          tma_load_4d(sK, &tmap_k, kv_full, 0, koff + k0, hk, bt);
+          tma_load_4d(sK + kTile / 2, &tmap_k, kv_full, 64, koff + k0, hk, bt);
+          tma_load_4d(sV, &tmap_v, kv_full, 0, koff + k0, hk, bt);
+          tma_load_4d(sV + kTile / 2, &tmap_v, kv_full, 64, koff + k0, hk, bt);
+        };
+        each_unit([&]() -> bool {
+          if (n_it == 0) return true;
+          if (!kWin || live == 0) load_kv();
+          int h = h0, i = istart;
+          for (int it = 0; it < n_it; ++it, ++gi) {
+            const int q0 = (i0 + i) * BQ, st = gi & 1;
+            if (!mbar_wait(&q_empty[st], (uint32_t)(((gi >> 1) & 1) ^ 1), abort_flag)) return false;
+            mbar_expect_tx(&q_full[st], kTile);
+            tma_load_4d(sQ + st * kTile, &tmap_q, &q_full[st], 0, qoff + q0, h, bt);
+            tma_load_4d(sQ + st * kTile + kTile / 2, &tmap_q, &q_full[st], 64, qoff + q0, h, bt);
+            if (!mbar_wait(do_empty, (uint32_t)((gi & 1) ^ 1), abort_flag)) return false;
+            mbar_expect_tx(do_full, kTile);
+            tma_load_4d(sdO, &tmap_do, do_full, 0, qoff + q0, h, bt);
+            tma_load_4d(sdO + kTile / 2, &tmap_do, do_full, 64, qoff + q0, h, bt);
+            if (kWin && it == 0 && live > 0) {       // K and V are free when every product of the unit before is done
+              if (!mbar_wait(all_done, (uint32_t)((live - 1) & 1), abort_flag)) return false;
+              load_kv();
+            }
+            if (++i == n_i) { i = 0; ++h; }
+          }
+          ++live;
+          return true;
+        });
       }
       __syncwarp();
     } else if (warp == 13) {
@@ -261,79 +307,89 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
       const uint64_t dK_mn = mndesc(sK), dO_mn = mndesc(sdO), dQ_mn = mndesc(sQ), dS_mn = mndesc(sS);
       auto koff16 = [](int kk) { return (uint32_t)(((kk >> 2) * (kTile / 2) + (kk & 3) * 32) >> 4); };   // K-major: two 64-column atoms
       auto mnoff16 = [](int kk) { return (uint32_t)((kk * 2048) >> 4); };                                // MN-major: 16 rows of 128 bytes
-      bool ok = n_it > 0 && wait(kv_full, 0) && wait(&q_full[0], 0);
-      // kWin: the rows of the current and the next query block that are the sequence's own (128 or more: all)
-      int mi = istart;
-      auto own_rows = [&]() { return Sq - (i0 + mi) * BQ; };
-      if (kWin && ok && p.cu_q) {
-        if (k0 + BK > Sk) {
-          zero_tail(sK, Sk - k0, lane);
-          zero_tail(sV, Sk - k0, lane);
-        }
-        if (own_rows() < BQ) zero_tail(sQ, own_rows(), lane);
-      }
-      if (ok) {
-        tc_fence_after();
-        if (issuer) {
-#pragma unroll
-          for (int kk = 0; kk < 8; ++kk) umma_f16(tmem_base + kColS, dK_k + koff16(kk), dQ_k + koff16(kk), idesc_kk, kk != 0 ? 1u : 0u);
-          umma_commit(s_full);
-        }
-      }
-      for (int it = 0; it < n_it && ok; ++it) {
-        const uint32_t tq = (uint32_t)((it & 1) * (kTile >> 4)), tq_next = (uint32_t)(((it + 1) & 1) * (kTile >> 4));
-        if (!wait(do_full, it)) { ok = false; break; }
-        if (kWin && p.cu_q && own_rows() < BQ) zero_tail(sdO, own_rows(), lane);
-        if (it > 0 && !wait(dq_drained, it - 1)) { ok = false; break; }
-        tc_fence_after();
-        if (issuer) {
-#pragma unroll
-          for (int kk = 0; kk < 8; ++kk) umma_f16(tmem_base + kColDP, dV_k + koff16(kk), dO_k + koff16(kk), idesc_kk, kk != 0 ? 1u : 0u);
-          umma_commit(dp_full);                        // dP^T = V dO^T
-        }
-        if (!wait(p_ready, it)) { ok = false; break; }
-        tc_fence_after();
-        if (issuer) {
-#pragma unroll
-          for (int kk = 0; kk < 8; ++kk)               // dV += P^T dO; P^T of 64 queries over the left of its half of S^T
-            umma_f16_ts(tmem_base + kColDV, tmem_base + kColS + (uint32_t)((kk >> 2) * 64 + (kk & 3) * 8), dO_mn + mnoff16(kk),
-                        idesc_kmn, (it == 0 && kk == 0) ? 0u : 1u);
-          umma_commit(do_empty);
-        }
-        if (it + 1 < n_it) {
-          if (!wait(&q_full[(it + 1) & 1], (it + 1) >> 1)) { ok = false; break; }
-          if constexpr (kWin) {
-            if (++mi == n_i) mi = 0;
-            if (p.cu_q && own_rows() < BQ) zero_tail(sQ + ((it + 1) & 1) * kTile, own_rows(), lane);
+      int base = 0, live = 0;              // pairs before this unit's, units with pairs so far
+      each_unit([&]() -> bool {
+        if (n_it == 0) return true;
+        bool ok = wait(kv_full, live) && wait(&q_full[base & 1], base >> 1);
+        // kWin: the rows of the current and the next query block that are the sequence's own (128 or more: all)
+        int mi = istart;
+        auto own_rows = [&]() { return Sq - (i0 + mi) * BQ; };
+        if (kWin && ok && p.cu_q) {
+          if (k0 + BK > Sk) {
+            zero_tail(sK, Sk - k0, lane);
+            zero_tail(sV, Sk - k0, lane);
           }
+          if (own_rows() < BQ) zero_tail(sQ + (base & 1) * kTile, own_rows(), lane);
+        }
+        if (ok) {
           tc_fence_after();
           if (issuer) {
+            const uint32_t tq = (uint32_t)((base & 1) * (kTile >> 4));
 #pragma unroll
-            for (int kk = 0; kk < 8; ++kk)             // S^T of the next pair, over P^T of this one
-              umma_f16(tmem_base + kColS, dK_k + koff16(kk), dQ_k + tq_next + koff16(kk), idesc_kk, kk != 0 ? 1u : 0u);
+            for (int kk = 0; kk < 8; ++kk) umma_f16(tmem_base + kColS, dK_k + koff16(kk), dQ_k + tq + koff16(kk), idesc_kk, kk != 0 ? 1u : 0u);
             umma_commit(s_full);
           }
         }
-        if (!wait(ds_ready, it)) { ok = false; break; }
-        tc_fence_after();
-        if (issuer) {
+        for (int it = 0; it < n_it && ok; ++it) {
+          const int gi = base + it;
+          const uint32_t tq = (uint32_t)((gi & 1) * (kTile >> 4)), tq_next = (uint32_t)(((gi + 1) & 1) * (kTile >> 4));
+          if (!wait(do_full, gi)) { ok = false; break; }
+          if (kWin && p.cu_q && own_rows() < BQ) zero_tail(sdO, own_rows(), lane);
+          if (gi > 0 && !wait(dq_drained, gi - 1)) { ok = false; break; }
+          tc_fence_after();
+          if (issuer) {
 #pragma unroll
-          for (int kk = 0; kk < 8; ++kk)               // dQ = dS K over the consumed dP^T
-            umma_f16(tmem_base + kColDP, dS_mn + mnoff16(kk), dK_mn + mnoff16(kk), idesc_mnmn, kk != 0 ? 1u : 0u);
-          umma_commit(dq_full);
+            for (int kk = 0; kk < 8; ++kk) umma_f16(tmem_base + kColDP, dV_k + koff16(kk), dO_k + koff16(kk), idesc_kk, kk != 0 ? 1u : 0u);
+            umma_commit(dp_full);                        // dP^T = V dO^T
+          }
+          if (!wait(p_ready, gi)) { ok = false; break; }
+          if (kWin && it == 0 && live > 0 && !wait(acc_empty, live - 1)) { ok = false; break; }
+          tc_fence_after();
+          if (issuer) {
 #pragma unroll
-          for (int kk = 0; kk < 8; ++kk)               // dK += dS^T Q
-            umma_f16(tmem_base + kColDK, dS_k + koff16(kk), dQ_mn + tq + mnoff16(kk), idesc_kmn, (it == 0 && kk == 0) ? 0u : 1u);
-          umma_commit(&q_empty[it & 1]);
-          if (it + 1 == n_it) umma_commit(all_done);
+            for (int kk = 0; kk < 8; ++kk)               // dV += P^T dO; P^T of 64 queries over the left of its half of S^T
+              umma_f16_ts(tmem_base + kColDV, tmem_base + kColS + (uint32_t)((kk >> 2) * 64 + (kk & 3) * 8), dO_mn + mnoff16(kk),
+                          idesc_kmn, (it == 0 && kk == 0) ? 0u : 1u);
+            umma_commit(do_empty);
+          }
+          if (it + 1 < n_it) {
+            if (!wait(&q_full[(gi + 1) & 1], (gi + 1) >> 1)) { ok = false; break; }
+            if constexpr (kWin) {
+              if (++mi == n_i) mi = 0;
+              if (p.cu_q && own_rows() < BQ) zero_tail(sQ + ((gi + 1) & 1) * kTile, own_rows(), lane);
+            }
+            tc_fence_after();
+            if (issuer) {
+#pragma unroll
+              for (int kk = 0; kk < 8; ++kk)             // S^T of the next pair, over P^T of this one
+                umma_f16(tmem_base + kColS, dK_k + koff16(kk), dQ_k + tq_next + koff16(kk), idesc_kk, kk != 0 ? 1u : 0u);
+              umma_commit(s_full);
+            }
+          }
+          if (!wait(ds_ready, gi)) { ok = false; break; }
+          tc_fence_after();
+          if (issuer) {
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk)               // dQ = dS K over the consumed dP^T
+              umma_f16(tmem_base + kColDP, dS_mn + mnoff16(kk), dK_mn + mnoff16(kk), idesc_mnmn, kk != 0 ? 1u : 0u);
+            umma_commit(dq_full);
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk)               // dK += dS^T Q
+              umma_f16(tmem_base + kColDK, dS_k + koff16(kk), dQ_mn + tq + mnoff16(kk), idesc_kmn, (it == 0 && kk == 0) ? 0u : 1u);
+            umma_commit(&q_empty[gi & 1]);
+            if (it + 1 == n_it) umma_commit(all_done);
+          }
         }
-      }
+        base += n_it;
+        ++live;
+        return ok;
+      });
       __syncwarp();
     } else if (warp == 14) {
       // ------------------------------------------------------------ lse (log2 domain, negated: an addend of the exponent) and
       // delta (times the softmax scale, negated) of every query block; an lse of -inf switches a row off
       // (read one block ahead, all eight loads in flight at once)
-      int h = h0, i = istart;
+      int h, i, gi = 0;
       float l[4], d[4];
       auto fetch = [&]() {
         const int64_t base = p.cu_q ? (int64_t)h * p.total_q + qoff : ((int64_t)b * p.H + h) * p.Sq;
@@ -344,20 +400,25 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
           d[e] = qi < Sq ? __ldg(p.delta + base + qi) : 0.f;
         }
       };
-      if (n_it > 0) fetch();
-      for (int it = 0; it < n_it; ++it) {
-        const int st = it & 1;
-        if (!mbar_wait_warp(&ld_empty[st], (uint32_t)(((it >> 1) & 1) ^ 1), abort_flag)) break;
+      each_unit([&]() -> bool {
+        h = h0;
+        i = istart;
+        if (n_it > 0) fetch();
+        for (int it = 0; it < n_it; ++it, ++gi) {
+          const int st = gi & 1;
+          if (!mbar_wait_warp(&ld_empty[st], (uint32_t)(((gi >> 1) & 1) ^ 1), abort_flag)) return false;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s_lse[st * 128 + e * 32 + lane] = l[e] > -INFINITY ? -l[e] * 1.4426950408889634f : -INFINITY;
-          s_dlt[st * 128 + e * 32 + lane] = -d[e] * p.scale;
+          for (int e = 0; e < 4; ++e) {
+            s_lse[st * 128 + e * 32 + lane] = l[e] > -INFINITY ? -l[e] * 1.4426950408889634f : -INFINITY;
+            s_dlt[st * 128 + e * 32 + lane] = -d[e] * p.scale;
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ld_full[st]);
+          if (++i == n_i) { i = 0; ++h; }
+          if (it + 1 < n_it) fetch();
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&ld_full[st]);
-        if (++i == n_i) { i = 0; ++h; }
-        if (it + 1 < n_it) fetch();
-      }
+        return true;
+      });
     }
   } else if (warp >= 8) {
     regs_inc<kDqRegs>();
@@ -365,10 +426,12 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
     const int qw = warp & 3;
     const int r = qw * 32 + lane;                 // query row inside the block = TMEM lane
     const uint32_t addr = tmem_base + ((uint32_t)(qw * 32) << 16) + kColDP;
+    int gi = 0;
+    each_unit([&]() -> bool {
     int h = h0, i = istart;
-    for (int it = 0; it < n_it; ++it) {
+    for (int it = 0; it < n_it; ++it, ++gi) {
       const int q0 = (i0 + i) * BQ;
-      bool ok = mbar_wait_warp(dq_full, (uint32_t)(it & 1), abort_flag);
+      bool ok = mbar_wait_warp(dq_full, (uint32_t)(gi & 1), abort_flag);
       tc_fence_after();
       uint32_t raw[4][32];
 #pragma unroll
@@ -395,9 +458,11 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
           asm volatile("cp.async.bulk.commit_group;" ::: "memory");
         }
       }
-      if (!ok) break;
+      if (!ok) return false;
       if (++i == n_i) { i = 0; ++h; }
     }
+    return true;
+    });
     // every reduction must have completed before the CTA exits
     if (threadIdx.x == 8 * 32) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   } else {
@@ -406,25 +471,27 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
     const int wg = warp >> 2;
     const int qw = warp & 3;
     const int r = qw * 32 + lane;                 // key row inside the block = TMEM lane
-    const int kj = k0 + r;
     const uint32_t lane_base = ((uint32_t)(qw * 32) << 16);
     const uint32_t s_addr = tmem_base + lane_base + kColS + (uint32_t)(wg * 64);
     const uint32_t dp_addr = tmem_base + lane_base + kColDP + (uint32_t)(wg * 64);
     uint8_t* srow = sS + (size_t)wg * (kTile / 2) + (size_t)r * 128;   // this warpgroup's 64 query columns = atom `wg`
+    auto wait_all = [&](uint64_t* bar, uint32_t parity) { return mbar_wait_warp(bar, parity, abort_flag); };
+    int gi = 0, live = 0;
+    each_unit([&]() -> bool {
+    const int kj = k0 + r;
     const bool key_off = kj >= Sk;
     const bool block_off = k0 + BK > Sk;
     const int far = kWin && kj >= p.sinks ? kj + p.window : 0x7fffffff;      // the first query that no longer sees this key
     bool ok = true;
-    auto wait_all = [&](uint64_t* bar, uint32_t parity) { return mbar_wait_warp(bar, parity, abort_flag); };
     int i = istart;
-    for (int it = 0; it < n_it; ++it) {
-      const uint32_t par = (uint32_t)(it & 1);
-      const int st = it & 1, q0 = (i0 + i) * BQ;
+    for (int it = 0; it < n_it; ++it, ++gi) {
+      const uint32_t par = (uint32_t)(gi & 1);
+      const int st = gi & 1, q0 = (i0 + i) * BQ;
       const float4* nlse4 = reinterpret_cast<const float4*>(s_lse + st * 128 + wg * 64);
       const float4* ndlt4 = reinterpret_cast<const float4*>(s_dlt + st * 128 + wg * 64);
       // only then can a query be older than a key of this block, a key be past the end or in front of a window
       const bool masked = (p.causal && q0 < k0 + BK) || block_off || (kWin && q0 + BQ - k0 > p.window);
-      if (!wait_all(&ld_full[st], (uint32_t)((it >> 1) & 1)) || !wait_all(s_full, par)) { ok = false; break; }
+      if (!wait_all(&ld_full[st], (uint32_t)((gi >> 1) & 1)) || !wait_all(s_full, par)) { ok = false; break; }
       tc_fence_after();
       float pf[64];
       auto probs = [&](auto mask) {
@@ -512,7 +579,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
       }
       if (++i == n_i) i = 0;
     }
-    if (ok && n_it > 0) ok = wait_all(all_done, 0);
+    if (ok && n_it > 0) ok = wait_all(all_done, (uint32_t)(live & 1));
     // ---- dK, dV of this key block
     if (ok) {
       tc_fence_after();
@@ -551,6 +618,12 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
         }
       }
     }
+    if (kWin && n_it > 0) {
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(acc_empty);
+      ++live;
+    }
     if constexpr (kWin) {
       if (p.cu_q && b == p.B - 1 && chunk == 0) {       // packed rows past the last sequence: the CTAs of a head share them
         Vec16<T> zero;
@@ -563,6 +636,8 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
         }
       }
     }
+    return ok;
+    });
   }
 
   tc_fence_before();
@@ -763,7 +838,10 @@ extern "C" int b200_flash_attn_bwd(const b200_attn_t* a, float* dq_accum, void* 
   p.sink_ws = a->workspace;
   if (a->window > 0 && (!a->causal || a->window > (1 << 30) || a->sinks < 0 || (p.sink_chunks > 1 && !p.sink_ws)))
     return (int)cudaErrorNotSupported;
-  const long long grid = (long long)a->B * a->Hkv * (p.kv_blocks + p.sink_blocks * (p.sink_chunks - 1));
+  const long long units = (long long)a->B * a->Hkv * (p.kv_blocks + p.sink_blocks * (p.sink_chunks - 1));
+  if (units > 2147483647ll - kSMs) return (int)cudaErrorNotSupported;
+  p.units = (int)units;
+  const long long grid = a->window > 0 ? std::min<long long>(units, gemm_sm_count()) : units;
   if (grid > 2147483647ll || rows / 8 + 1 > 2147483647ll) return (int)cudaErrorNotSupported;
   const int row_blocks = (dS + kDeltaRows - 1) / kDeltaRows;
   const unsigned delta_grid = (unsigned)((long long)dB * a->H * row_blocks);
