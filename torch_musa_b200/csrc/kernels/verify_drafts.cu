@@ -13,8 +13,6 @@
 // Parity: the reference has no speculative decoding.
 #include "common.cuh"
 
-#include <algorithm>
-
 namespace b200k {
 namespace {
 
@@ -92,8 +90,11 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_drafts_kernel(int64_t* 
       w[e] = w[e] > 0.0 ? w[e] : 0.0;          // NaN weighs nothing
     }
   };
-  auto cluster_sync = [&]() {
-    if (p.split > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  auto cluster_arrive = [&]() {
+    if (p.split > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  };
+  auto cluster_wait = [&]() {
+    if (p.split > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     else __syncthreads();
   };
   if (rank == 0)
@@ -110,7 +111,8 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_drafts_kernel(int64_t* 
     }
     s = warp_sum(s);
     if (lane == 0) s_mine[warp] = s;
-    cluster_sync();
+    cluster_arrive();
+    cluster_wait();
     for (int c = threadIdx.x; c < pieces; c += kVerifyThreads) {
       double v;
       if (p.split > 1) {
@@ -121,7 +123,9 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_drafts_kernel(int64_t* 
       }
       s_all[c] = v;
     }
-    cluster_sync();      // everyone has read everyone: s_mine may be written again, and a CTA may leave
+    // a CTA leaves, or writes s_mine again, when all have read it: waited for at the end
+    cluster_arrive();
+    __syncthreads();
     // The running sum at the piece borders: one function of the border, evaluated the same way by both its neighbours, and it never
     // falls (sums of what is not negative, in a fixed order).  So exactly one warp finds the limit in its piece.
     double before = 0.0, upto = 0.0, total = 0.0;
@@ -173,8 +177,11 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_drafts_kernel(int64_t* 
         if (lane == 0) out[(int64_t)b * (p.n + 1) + r] = token;
       }
       if (rank == 0 && threadIdx.x == 0) taken_out[b] = r;
+      __syncwarp();
+      cluster_wait();
       return;
     }
+    cluster_wait();
   }
   if (rank == 0 && threadIdx.x == 0) {
     out[(int64_t)b * (p.n + 1) + r] = -1;
@@ -185,13 +192,21 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_drafts_kernel(int64_t* 
 template <typename T>
 int launch_verify(int64_t* taken, int64_t* out, const T* target, const T* draft, const int64_t* tokens, const float* uniforms, VerifyParams p,
                   cudaStream_t stream) {
-  // CTAs of a cluster: a load or two for every lane, while there are places for all
+  // CTAs of a cluster: as many as leave every thread a load or two, up to eight while there are places for all of them, sixteen only
+  // where each gets an SM (four drafts, 32000 words, us in a graph for 2 / 4 / 8 / 16: one sequence 10.6 / 7.7 / 6.3 / 5.4; with seven
+  // drafts 64 sequences 19.6 / 12.2 / 9.0 / 14.8)
   const int loads = (int)cdiv(p.V, (int64_t)kVerifyThreads * Vec16<T>::N);
   p.split = 1;
-  while (p.split < 8 && p.split < loads && (long long)p.B * p.split < 4 * kSMs) p.split *= 2;
+  while (p.split < 16 && p.split < loads && 2ll * p.B * p.split <= (p.split < 8 ? 4 : 1) * kSMs) p.split *= 2;
   if ((long long)p.B * p.split > 2147483647ll) return (int)cudaErrorNotSupported;
   auto on16 = [](const T* x, int64_t s0, int64_t s1) { return aligned16(x) && s0 % Vec16<T>::N == 0 && s1 % Vec16<T>::N == 0; };
   const bool vec = on16(target, p.p_sb, p.p_sn) && (!draft || on16(draft, p.q_sb, p.q_sn));
+  static OncePerDevice once;
+  if (int e = once([] {
+        if (int r = (int)cudaFuncSetAttribute(verify_drafts_kernel<T, true>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) return r;
+        return (int)cudaFuncSetAttribute(verify_drafts_kernel<T, false>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+      }))
+    return e;
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
