@@ -5,6 +5,9 @@ Bounds: with u = eps / 2 of the type, attention keeps its sums and statistics in
 probabilities are carried to 2^-16): |o - o'| <= u |o| + 2^-13 sum p |v|.  A rotation is two 32-bit products and a sum, rounded
 once: u |y| + 2^-22 (|x0 c| + |x1 s|).  Whole numbers are equal."""
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -185,6 +188,91 @@ def test_replay_follows_the_lengths_and_graphs_do_not_share(bw, dev):
         bw.synchronize()
         for x, o in zip(on, outs):
             assert torch.equal(o, paged_attention(*x))
+
+
+def test_capture_is_the_first_thing_a_program_does(bw, dev):
+    """Nothing has run before: torch's CUDA allocator is not set up, and the words that kernels report to are not there."""
+    code = """
+import torch, torch_musa_b200 as bw
+from torch_musa_b200.ops import paged_attention, paged_rope_cache, verify_drafts, window_attention
+put = lambda t: t.to("blackwell")
+q, pool = put(torch.zeros(1, 1, 2, 64, dtype=torch.float16)), put(torch.ones(4, 2, 16, 64, dtype=torch.float16))
+table, lens = put(torch.tensor([[2, 1]], dtype=torch.int32)), put(torch.tensor([20], dtype=torch.int32))
+angles, p = put(torch.ones(32, 32)), put(torch.tensor([[[0.0, 1.0]]]))
+none, u, x = put(torch.zeros(1, 0, dtype=torch.long)), put(torch.zeros(1, 1)), put(torch.ones(1, 40, 1, 128, dtype=torch.float16))
+x.requires_grad_()
+graph = bw.BlackwellGraph()
+with bw.graph(graph):
+    a = paged_rope_cache(q[0], pool[0, :, :1].transpose(0, 1), pool[0, :, :1].transpose(0, 1), angles, angles, pool, pool, table, lens)
+    b = paged_attention(q, pool, pool, table, lens)
+    c = verify_drafts(p, none, u)[1]
+    d = window_attention(x, x, x, 8, 1)
+    e = torch.autograd.grad(d, x, d.detach())[0]
+graph.replay()
+bw.synchronize()
+assert bool((a.cpu() == 0).all()) and bool((b.cpu() == 1).all()) and c.tolist() == [[1]] and bool((d.cpu() == 1).all()) and bool(torch.isfinite(e.cpu()).all())
+"""
+    subprocess.run([sys.executable, "-c", code], check=True, timeout=300, cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+
+
+def test_very_long_sequences_at_once(bw, dev):
+    """Past 16384 keys several clusters share a key head and a second kernel joins their parts: two such calls on two streams, captured
+    ones replayed together, lengths that leave most parts without a key."""
+    cases = [case(s, [20000], 1, 4, 1, 64, 64, torch.float16) for s in (13, 14)]
+    on = [[t.to(dev) for t in c] for c in cases]
+    want = [want_attention(*c) for c in cases]
+    streams, graphs, outs = [bw.Stream(), bw.Stream()], [], []
+    eager = []
+    for s, x in zip(streams, on):
+        s.wait_stream(bw.current_stream())
+        with bw.stream(s):
+            eager = eager + [paged_attention(*x)]
+    bw.synchronize()
+    for e, w in zip(eager, want):
+        check(e, *w)
+    for x in on:
+        graph = bw.BlackwellGraph()
+        with bw.graph(graph):
+            outs.append(paged_attention(*x))
+        graphs.append(graph)
+    bw.synchronize()
+    for _ in range(10):
+        for s, graph in zip(streams, graphs):
+            with bw.stream(s):
+                graph.replay()
+    bw.synchronize()
+    for o, e in zip(outs, eager):
+        assert torch.equal(o, e)
+    q, k, v, table, _ = cases[0]
+    for n in (0, 1, 70, 700):
+        lens = torch.tensor([n], dtype=torch.int32)
+        keep = on[0][2].clone().nan_to_num_(0.0, 0.0, 0.0)      # rows past the new end are clean, whatever the case put there
+        check(paged_attention(on[0][0], on[0][1], keep, on[0][3], lens.to(dev)), *want_attention(q, k, v, table, lens))
+
+
+def test_windows_and_sinks_of_any_size(bw, dev):
+    q, k, v, table, lens = case(15, [90, 3], 5, 4, 2, 128, 16, torch.bfloat16)
+    want = want_attention(q, k, v, table, lens)
+    on = [t.to(dev) for t in (q, k, v, table, lens)]
+    for window, sinks in ((2 ** 62, 0), (2 ** 31 - 1, 2 ** 31 - 1), (1, 2 ** 40)):
+        check(paged_attention(*on, window=window, sinks=sinks), *want)
+
+
+def test_captured_verification(bw, dev):
+    p, x, u, q = probs(5, 3, 4, 5000, torch.float32)
+    on = [t.to(dev) for t in (p, x, u, q)]
+    graph = bw.BlackwellGraph()
+    verify_drafts(*on)
+    with bw.graph(graph):
+        held = verify_drafts(*on)
+    for seed in (6, 7):
+        new = probs(seed, 3, 4, 5000, torch.float32)
+        for a, b in zip(on, new):
+            a.copy_(b)
+        graph.replay()
+        bw.synchronize()
+        want = verify_drafts(*new)
+        assert torch.equal(held[0].cpu(), want[0]) and torch.equal(held[1].cpu(), want[1])
 
 
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])

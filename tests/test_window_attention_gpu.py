@@ -233,3 +233,83 @@ def test_llama_with_a_window_trains_like_the_plain_model(bw, dev):
     # 16 roundings of 2^-8 along the way (norms, projections, residuals of two layers), each at most the values' own size
     assert float((got - want).abs().max()) <= 16 * 2 ** -8 * float(want.abs().max())
     assert all(p.grad is not None and bool(torch.isfinite(p.grad).all()) for p in model.parameters())
+
+
+def test_backward_is_refused_where_determinism_is_asked_for(bw, dev):
+    from torch_musa_b200.ops import flash_attn_varlen_func, window_attention
+
+    q, k, v, do = (t.to(dev) for t in inputs(torch.bfloat16, (1, 40, 2, D), (1, 40, 1, D)))
+    q.requires_grad_()
+    cu = torch.tensor([0, 40], dtype=torch.int32).to(dev)
+    outs = [window_attention(q, k, v, 8), flash_attn_varlen_func(q[0], k[0], v[0], cu, cu, 40, 40, causal=True, window=8)]
+    torch.use_deterministic_algorithms(True)
+    try:
+        for out in outs:
+            with pytest.raises(RuntimeError, match="deterministic"):
+                out.sum().backward()
+    finally:
+        torch.use_deterministic_algorithms(False)
+
+
+def test_refusals(bw, dev):
+    from torch_musa_b200.ops import window_attention
+
+    op = torch.ops.blackwell
+    q, k, v, do = (t.to(dev) for t in inputs(torch.bfloat16, (1, 40, 4, D), (1, 40, 2, D)))
+    out, lse = op.window_attention(q, k, v, 8)
+    for bad in (lambda: op.window_attention(q, k, v, 0), lambda: op.window_attention(q, k, v, 8, -1), lambda: op.window_attention(q, k, v, 8, 0, 0.0),
+                lambda: op.window_attention(q, k, v[:, :30], 8), lambda: op.window_attention(q, k.half(), v, 8), lambda: op.window_attention(q, k.cpu(), v, 8),
+                lambda: op.window_attention(q[:, :, :3], k, v, 8), lambda: op.window_attention(q[..., :64], k[..., :64], v[..., :64], 8),
+                lambda: op.window_attention_backward(do[:, :20], q, k, v, out, lse, 8), lambda: op.window_attention_backward(do, q, k, v, out, lse.half(), 8),
+                lambda: op.varlen_attention(q[0], k[0], v[0], *[torch.tensor([0, 40], dtype=torch.int32).to(dev)] * 2, 40, 40, False, None, 8)):
+        with pytest.raises(RuntimeError):
+            bad()
+    with pytest.raises(ValueError):
+        window_attention(q, k, v, 8, softmax_scale=-1.0)
+    leaf = q.clone().requires_grad_()
+    grad = torch.autograd.grad(window_attention(leaf, k, v, 8).sum(), leaf, create_graph=True)[0]
+    with pytest.raises(RuntimeError):           # no second order
+        grad.sum().backward()
+    for shape_q, shape_k in (((1, 0, 4, D), (1, 5, 2, D)), ((0, 5, 4, D), (0, 5, 2, D)), ((2, 5, 4, D), (2, 0, 2, D))):
+        e = [torch.zeros(s, dtype=torch.float16).to(dev).requires_grad_() for s in (shape_q, shape_k, shape_k)]
+        o = window_attention(*e, 3)
+        assert o.shape == shape_q and bool((o == 0).all())
+        assert [g.shape for g in torch.autograd.grad(o, e, torch.zeros_like(o))] == [t.shape for t in e]
+
+
+def test_two_streams_and_two_graphs(bw, dev):
+    """Forward and backward of two problems at once, each on a stream of its own, eager and replayed: scratch is not shared.  (The last
+    bits of dq follow the order of arrival.)"""
+    from torch_musa_b200.ops import window_attention
+
+    cases = [inputs(torch.bfloat16, (1, 700, 4, D), (1, 700, 2, D), s) for s in (1, 2)]
+    cases = [[t.to(dev) for t in c] for c in cases]
+    leaves = [[t.clone().requires_grad_() for t in c[:3]] for c in cases]
+    step = lambda i: (lambda o: [o.detach(), *torch.autograd.grad(o, leaves[i], cases[i][3])])(window_attention(*leaves[i], 100, 5))  # noqa: E731
+    want = [step(i) for i in range(2)]
+    streams = [bw.Stream(), bw.Stream()]
+    bw.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with bw.stream(s):
+                got[i] = step(i)
+    graphs, held = [], []
+    for i in range(2):
+        graph = bw.BlackwellGraph()
+        with bw.graph(graph):
+            held.append(step(i))
+        graphs.append(graph)
+    bw.synchronize()
+    for _ in range(5):
+        for s, graph in zip(streams, graphs):
+            with bw.stream(s):
+                graph.replay()
+    bw.synchronize()
+    for i in range(2):
+        for result in (got[i], held[i]):
+            for n, (a, b) in enumerate(zip(result, want[i])):
+                if n == 1:
+                    assert float((a.double() - b.double()).abs().max()) <= float(2 ** -8 * b.double().abs().max())
+                else:
+                    assert torch.equal(a, b)

@@ -13,6 +13,7 @@
 #include "aten/FallbackCall.h"
 #include "aten/Ops.h"
 
+#include <ATen/Context.h>
 #include <ATen/Functions.h>
 #include <ATen/native/DispatchStub.h>
 #include <ATen/native/transformers/attention.h>
@@ -315,6 +316,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> varlen_attention_backward(
              l = lse.contiguous();
   b200_attn_t a{};
   varlen_desc(a, q, k, v, cu_q, cu_k, max_q, max_k, causal, scale, window, sinks);
+  if (window.has_value()) at::globalContext().alertNotDeterministic("varlen_attention_backward with a window");
   TORCH_CHECK(l.scalar_type() == at::kFloat && l.numel() == q.size(0) * q.size(1), "varlen_attention_backward: lse must be [H, total_q]");
   a.o_ss = o.stride(0); a.o_sh = o.stride(1);
   at::Tensor dq32 = at::empty({q.size(1), q.size(0), 128}, q.options().dtype(at::kFloat));
@@ -399,6 +401,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> window_attention_backward(const a
   const char* op = "window_attention_backward";
   check_window_operands(op, q_, k_, v_);
   check_devices(op, q_, k_, v_, grad_out, out, lse);
+  at::globalContext().alertNotDeterministic(op);      // dq is summed in the order in which key blocks arrive
   TORCH_CHECK(grad_out.sizes() == q_.sizes() && out.sizes() == q_.sizes() && grad_out.scalar_type() == q_.scalar_type() &&
                   out.scalar_type() == q_.scalar_type() && lse.scalar_type() == at::kFloat && lse.numel() == q_.size(0) * q_.size(1) * q_.size(2),
               op, ": grad_out and out must be like q, lse float32 [B, H, Sq]");

@@ -74,7 +74,7 @@ at::Tensor paged_attention(const at::Tensor& q_, const at::Tensor& k_pages, cons
   TORCH_CHECK(!window.has_value() || *window > 0, op, ": window must be positive");
   TORCH_CHECK(sinks >= 0, op, ": sinks must not be negative");
   TORCH_CHECK(!scale.has_value() || (*scale > 0 && std::isfinite(*scale)), op, ": the scale must be positive, got ", scale.value_or(0.0));
-  TORCH_CHECK(block_table.size(1) <= INT_MAX / k_pages.size(2), op, ": block_table covers more than 2^31 tokens");
+  TORCH_CHECK(block_table.size(1) <= (1 << 30) / k_pages.size(2), op, ": block_table covers more than 2^30 tokens");
   if (block_table.size(1) == 0) return at::zeros({B, n, H, D}, q_.options());
   at::Tensor out = at::empty({B, n, H, D}, q_.options());
   if (out.numel() == 0) return out;
@@ -86,8 +86,8 @@ at::Tensor paged_attention(const at::Tensor& q_, const at::Tensor& k_pages, cons
   a.num_pages = fit_int(op, k_pages.size(0));
   a.page_size = fit_int(op, k_pages.size(2));
   a.table_width = (int)block_table.size(1);
-  a.window = window.has_value() ? (int)std::min<int64_t>(*window, INT_MAX) : 0;
-  a.sinks = (int)std::min<int64_t>(sinks, INT_MAX);
+  a.window = window.has_value() ? (int)std::min<int64_t>(*window, 1 << 30) : 0;      // differences of positions stay in 32 bits
+  a.sinks = (int)std::min<int64_t>(sinks, 1 << 30);
   a.scale = (float)scale.value_or(1.0 / std::sqrt((double)D));
   a.q_sb = stride_of(q, 0); a.q_sn = stride_of(q, 1); a.q_sh = stride_of(q, 2);
   a.k_sp = stride_of(k_pages, 0); a.k_sh = stride_of(k_pages, 1); a.k_sr = k_pages.stride(2);
@@ -126,7 +126,7 @@ at::Tensor paged_rope_cache(const at::Tensor& q_, const at::Tensor& k_, const at
   check_int32(op, "seq_lens", seq_lens, 1);
   const int64_t B = seq_lens.size(0);
   TORCH_CHECK(block_table.size(0) == B, op, ": block_table and seq_lens must have a row per sequence");
-  TORCH_CHECK(block_table.size(1) <= INT_MAX / k_pages.size(2), op, ": block_table covers more than 2^31 tokens");
+  TORCH_CHECK(block_table.size(1) <= (1 << 30) / k_pages.size(2), op, ": block_table covers more than 2^30 tokens");
   const bool packed = cu_seqlens.has_value() && cu_seqlens->defined();
   if (packed) {
     check_int32(op, "cu_seqlens", *cu_seqlens, 1);

@@ -1,7 +1,10 @@
 #include "core/Graph.h"
 
+#include "core/DeviceAssert.h"
 #include "core/Generator.h"
+#include "kernels/b200_kernels.h"
 
+#include <ATen/Context.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 
 #include <atomic>
@@ -38,6 +41,12 @@ void Graph::capture_begin(alloc::MempoolId pool, cudaStreamCaptureMode mode) {
                                 "(use torch.blackwell.graph(...) or a side stream)");
   capture_stream_ = stream.stream();
 
+  // torch's own CUDA allocator takes part below (what the library fallback allocates inside a capture); a program that has not
+  // used the fallback yet has not set it up
+  at::globalContext().lazyInitDevice(c10::DeviceType::CUDA);
+  // and the host-mapped words that kernels report to cannot be allocated any more once the stream is capturing
+  device_assert_word(device_);
+  (void)b200_gemm_status(0);
   auto* a = alloc::get();
   if (pool.first != 0 || pool.second != 0) {
     pool_ = pool;

@@ -591,7 +591,7 @@ B200_API int b200_decode_rope_cache(int dtype, void* q_out, const void* q, const
  * and 16-byte aligned); block_table int32 [B, table_width], seq_lens int32 [B]: tokens of a sequence in the cache, the newest
  * included.  Token i stands at position len - n + i and sees key j when j <= its position and, with window > 0, its position
  * minus j < window or j < sinks.  Keys on a page number outside the pool are hidden and noted in *status (may be NULL); a
- * token that sees no key gets zeros.  D is 64 or 128, page_size a multiple of 16.  workspace: as many floats as
+ * token that sees no key gets zeros.  D is 64 or 128, page_size a multiple of 16, a table row covers at most 2^30 tokens.  workspace: as many floats as
  * b200_paged_attention_workspace says for the same description (NULL when that is 0). */
 typedef struct {
   int dtype, head_dim;

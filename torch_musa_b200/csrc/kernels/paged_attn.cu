@@ -736,7 +736,7 @@ int launch_paged(const PagedPlan& plan, void* out, const void* q, const void* kp
 bool paged_sizes_ok(const b200_paged_attn_t* a) {
   return (a->dtype == B200_BF16 || a->dtype == B200_F16) && (a->head_dim == 64 || a->head_dim == 128) && a->B > 0 && a->n > 0 && a->H > 0 &&
          a->Hkv > 0 && a->H % a->Hkv == 0 && a->page_size > 0 && a->page_size % kPageRows == 0 && a->num_pages >= 0 && a->table_width > 0 &&
-         (long long)a->table_width * a->page_size <= 2147483647ll && a->sinks >= 0 && a->B <= 65535 && a->Hkv <= 65535 &&
+         (long long)a->table_width * a->page_size <= (1 << 30) && a->n <= (1 << 29) && a->sinks >= 0 && a->B <= 65535 && a->Hkv <= 65535 &&
          (long long)a->n * (a->H / a->Hkv) <= (1 << 24);
 }
 
@@ -760,7 +760,8 @@ extern "C" int b200_paged_attention(const b200_paged_attn_t* a, void* out, const
   PagedParams p{};
   p.B = a->B; p.n = a->n; p.H = a->H; p.Hkv = a->Hkv;
   p.num_pages = a->num_pages; p.page_size = a->page_size; p.table_width = a->table_width;
-  p.window = a->window; p.sinks = a->window > 0 ? a->sinks : 0;
+  p.window = std::min(a->window, 1 << 30);             // differences of positions stay in 32 bits
+  p.sinks = a->window > 0 ? std::min(a->sinks, 1 << 30) : 0;
   p.scale_log2 = a->scale * 1.4426950408889634f;
   p.q_sb = a->q_sb; p.q_sn = a->q_sn; p.q_sh = a->q_sh;
   p.k_sp = a->k_sp; p.k_sh = a->k_sh; p.k_sr = a->k_sr;

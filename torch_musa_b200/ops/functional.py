@@ -398,8 +398,10 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     """Causal attention with a sliding window and a few first tokens that stay visible: query i sees key j when
     ``j <= i and (i - j < window or j < sinks)``.  ``q`` [B, Sq, H, D], ``k`` / ``v`` [B, Sk, Hkv, D] (Hkv divides H);
     returns [B, Sq, H, D], zeros for a query that sees no key.  On the blackwell device with D = 128 and bf16 / fp16 the
-    tensor-core kernels skip the blocks of keys outside the mask, in both directions (gradients of dq are summed in
-    fp32 in the order in which blocks arrive); otherwise it is ``scaled_dot_product_attention`` with the mask."""
+    tensor-core kernels skip the blocks of keys outside the mask, in both directions; otherwise it is
+    ``scaled_dot_product_attention`` with the mask.  There the gradient of ``q`` is summed in 32 bits in the order in which
+    blocks of keys arrive, which ``torch.use_deterministic_algorithms`` refuses, and a key or value that is not finite
+    reaches every query that shares a block of 128 keys with it, whether it sees it or not."""
     _check_window(True, window, sinks, softmax_scale)
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3] or k.shape[2] == 0 or q.shape[2] % k.shape[2]:
         raise ValueError(f"window_attention: q [B, Sq, H, D] and k, v [B, Sk, Hkv, D] with Hkv a divisor of H expected, got "
