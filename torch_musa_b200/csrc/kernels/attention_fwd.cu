@@ -37,6 +37,7 @@ struct AttnParams {
   const int* cu_k;
   int total_q;
   int* status;
+  int units;                  // pairs of query tiles of all (batch, head) instances
   int window, sinks;          // kWin: key j is visible when j <= i and (i - j < window or j < sinks)
 };
 
@@ -67,6 +68,16 @@ struct AttnParams {
 // rest of tile 1's window.  So tile 0 takes a prefix of the list and tile 1 a suffix, and every block is loaded once.  Packed
 // rows of the next sequence, or of nobody, are set to zero in the last block of V: their probability is zero, but zero times
 // what lies there need not be.
+// One unit of work: a pair of query tiles of one (batch, head); heavy (late) tiles first, across all (batch, head) instances.
+struct FwdUnit {
+  int qp, b, h, hk, Sq, Sk, qoff, koff, bt;
+  int nb0, nb1, nbmax;        // tile t ends before item nb<t> of the list of key blocks
+  __device__ __forceinline__ int nb(int t) const { return t ? nb1 : nb0; }
+  // kWin: the list that the tiles share is [lo0, lo0 + n_pre), then the sinks' [0, n_sink), then [lo1, ...); tile 1 begins at item
+  // second_first
+  int second_first, lo0, lo1, n_pre, n_sink;
+};
+
 template <typename T, bool kWin>
 __global__ void __launch_bounds__(kAttnThreads, 1)
 attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
@@ -81,61 +92,80 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
   uint64_t* r_empty = bars + 2 + kRing;        // [kRing]  tcgen05.commit
   uint64_t* mma_done = bars + 2 + 2 * kRing;   // [2]      tcgen05.commit: P V of block j - 1 and S of block j
   uint64_t* p_ready = mma_done + 2;            // [2][2]   four softmax warps: first / second part of P of block j is in TMEM
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(p_ready + 4);
+  uint64_t* q_empty = p_ready + 4;             // [2]      tcgen05.commit: the last S of a unit's tile (kWin)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // heavy (late) query tiles first, across all (batch, head) instances
   const int n_bh = p.B * p.H;
-  const int qp = p.q_pairs - 1 - (int)(blockIdx.x / n_bh);
-  const int bh = (int)(blockIdx.x % n_bh);
-  const int b = bh / p.H, h = bh - b * p.H;
-  const int hk = h / (p.H / p.Hkv);
-  // this instance's sequence: lengths, first packed rows and the batch coordinate of the tensor maps.  Rows past a
-  // packed sequence's end belong to the next sequence: they are loaded, masked by index and never stored.
-  int Sq = p.Sq, Sk = p.Sk, qoff = 0, koff = 0, bt = b;
-  if (p.cu_q) {
-    qoff = p.cu_q[b];
-    Sq = p.cu_q[b + 1] - qoff;
-    koff = p.cu_k[b];
-    Sk = p.cu_k[b + 1] - koff;
-    bt = 0;
-  }
-  int nb[2];
+  auto make_unit = [&](int unit) {
+    FwdUnit u{};
+    u.qp = p.q_pairs - 1 - unit / n_bh;
+    const int bh = unit % n_bh;
+    u.b = bh / p.H;
+    u.h = bh - u.b * p.H;
+    u.hk = u.h / (p.H / p.Hkv);
+    // this instance's sequence: lengths, first packed rows and the batch coordinate of the tensor maps.  Rows past a
+    // packed sequence's end belong to the next sequence: they are loaded, masked by index and never stored.
+    u.Sq = p.Sq;
+    u.Sk = p.Sk;
+    u.bt = u.b;
+    if (p.cu_q) {
+      u.qoff = p.cu_q[u.b];
+      u.Sq = p.cu_q[u.b + 1] - u.qoff;
+      u.koff = p.cu_k[u.b];
+      u.Sk = p.cu_k[u.b + 1] - u.koff;
+      u.bt = 0;
+    }
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    const int q0 = (2 * qp + t) * AQ;
-    int k_end = Sk;
-    if (p.causal) k_end = min(Sk, q0 + AQ);
-    nb[t] = q0 < Sq ? (k_end + AK - 1) / AK : 0;
-  }
-  // kWin: the shared list of blocks is [lo0, lo0 + n_pre), then the sinks' [0, n_sink), then [lo1, ...); tile t takes its
-  // items [first_of(t), nb[t])
-  int second_first = 0, lo0 = 0, lo1 = 0, n_pre = 0, n_sink = 0;
-  if constexpr (kWin) {
-    const int sb = (min(p.sinks, Sk) + AK - 1) / AK, q0 = 2 * qp * AQ;
-    const bool second = q0 + AQ < Sq;
-    lo0 = max(max(0, q0 - p.window + 1) / AK, sb);
-    lo1 = second ? max(max(0, q0 + AQ - p.window + 1) / AK, sb) : lo0;
-    const int end0 = nb[0], end1 = nb[1];
-    n_pre = max(0, min(lo1, end0) - lo0);
-    n_sink = min(sb, max(end0, end1));
-    nb[0] = n_pre + min(sb, end0) + max(0, end0 - lo1);
-    nb[1] = second ? n_pre + n_sink + max(0, end1 - lo1) : 0;
-    if (nb[1] == n_pre) nb[1] = 0;      // no key at all
-    second_first = nb[1] > 0 ? n_pre : 0;
-  }
-  auto first_of = [&](int t) { return kWin && t == 1 ? second_first : 0; };
-  auto block_of = [&](int j) {
-    if constexpr (!kWin) return j;
-    else return j < n_pre ? lo0 + j : (j - n_pre < n_sink ? j - n_pre : lo1 + (j - n_pre - n_sink));
+    for (int t = 0; t < 2; ++t) {
+      const int q0 = (2 * u.qp + t) * AQ;
+      int k_end = u.Sk;
+      if (p.causal) k_end = min(u.Sk, q0 + AQ);
+      (t ? u.nb1 : u.nb0) = q0 < u.Sq ? (k_end + AK - 1) / AK : 0;
+    }
+    if constexpr (kWin) {
+      const int sb = (min(p.sinks, u.Sk) + AK - 1) / AK, q0 = 2 * u.qp * AQ;
+      const bool second = q0 + AQ < u.Sq;
+      u.lo0 = max(max(0, q0 - p.window + 1) / AK, sb);
+      u.lo1 = second ? max(max(0, q0 + AQ - p.window + 1) / AK, sb) : u.lo0;
+      const int end0 = u.nb0, end1 = u.nb1;
+      u.n_pre = max(0, min(u.lo1, end0) - u.lo0);
+      u.n_sink = min(sb, max(end0, end1));
+      u.nb0 = u.n_pre + min(sb, end0) + max(0, end0 - u.lo1);
+      u.nb1 = second ? u.n_pre + u.n_sink + max(0, end1 - u.lo1) : 0;
+      if (u.nb1 == u.n_pre) u.nb1 = 0;      // no key at all
+      u.second_first = u.nb1 > 0 ? u.n_pre : 0;
+    }
+    u.nbmax = max(u.nb0, u.nb1);
+    return u;
   };
-  const int nbmax = max(nb[0], nb[1]);
+  // Calls f() for every unit of this CTA until it returns false.  Without a window a CTA has one unit.  With one the units are short (ten
+  // blocks at a window of 1024): a CTA then stays on its SM and takes every 148th unit, turning round at either end so that long and
+  // short ones even out; the loads and the first products of a unit run while the one before it is stored.
+  const FwdUnit only = kWin ? FwdUnit{} : make_unit((int)blockIdx.x);
+  auto each_unit = [&](auto f) {
+    if constexpr (!kWin) {
+      f(only);
+    } else {
+      for (int round = 0; round * (int)gridDim.x < p.units; ++round) {
+        const int unit = round * (int)gridDim.x + (round & 1 ? (int)(gridDim.x - 1 - blockIdx.x) : (int)blockIdx.x);
+        if (unit >= p.units) continue;
+        if (!f(make_unit(unit))) break;
+      }
+    }
+  };
+  auto first_of = [](const FwdUnit& u, int t) { return kWin && t == 1 ? u.second_first : 0; };
+  auto block_of = [](const FwdUnit& u, int j) {
+    if constexpr (!kWin) return j;
+    else return j < u.n_pre ? u.lo0 + j : (j - u.n_pre < u.n_sink ? j - u.n_pre : u.lo1 + (j - u.n_pre - u.n_sink));
+  };
 
   if (threadIdx.x == 0) {
     *abort_flag = 0;
     for (int t = 0; t < 2; ++t) {
       mbar_init(&q_full[t], 1);
+      mbar_init(&q_empty[t], 1);
       mbar_init(&mma_done[t], 1);
       mbar_init(&p_ready[2 * t], 4);
       mbar_init(&p_ready[2 * t + 1], 4);
@@ -163,22 +193,30 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
     if (warp == 8) {
       // ------------------------------------------------------------ TMA producer
       if (lane == 0) {
-        for (int t = 0; t < 2; ++t) {
-          if (nb[t] == 0) continue;
-          const int q0 = (2 * qp + t) * AQ;
-          mbar_expect_tx(&q_full[t], kTile);
-          tma_load_4d(sQ + t * kTile, &tmap_q, &q_full[t], 0, qoff + q0, h, bt);                 // d 0..63
-          tma_load_4d(sQ + t * kTile + kTile / 2, &tmap_q, &q_full[t], 64, qoff + q0, h, bt);    // d 64..127
-        }
-        for (int n = 0; n < 2 * nbmax; ++n) {
-          const int st = n % kRing;
-          if (!mbar_wait(&r_empty[st], (uint32_t)(((n / kRing) & 1) ^ 1), abort_flag)) break;
-          mbar_expect_tx(&r_full[st], kTile);
-          const int k0 = block_of(n >> 1) * AK;
-          const CUtensorMap* map = (n & 1) ? &tmap_v : &tmap_k;   // V is read as an MN-major B operand: same boxes
-          tma_load_4d(sR + st * kTile, map, &r_full[st], 0, koff + k0, hk, bt);
-          tma_load_4d(sR + st * kTile + kTile / 2, map, &r_full[st], 64, koff + k0, hk, bt);
-        }
+        int ring = 0;                    // items of the ring so far
+        uint32_t loaded[2] = {0, 0};     // Q tiles so far, for the phases
+        each_unit([&](const FwdUnit& u) -> bool {
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (u.nb(t) == 0) continue;
+            const int q0 = (2 * u.qp + t) * AQ;
+            if (kWin && !mbar_wait(&q_empty[t], (loaded[t] & 1) ^ 1, abort_flag)) return false;
+            ++loaded[t];
+            mbar_expect_tx(&q_full[t], kTile);
+            tma_load_4d(sQ + t * kTile, &tmap_q, &q_full[t], 0, u.qoff + q0, u.h, u.bt);                 // d 0..63
+            tma_load_4d(sQ + t * kTile + kTile / 2, &tmap_q, &q_full[t], 64, u.qoff + q0, u.h, u.bt);    // d 64..127
+          }
+          for (int n = 0; n < 2 * u.nbmax; ++n, ++ring) {
+            const int st = ring % kRing;
+            if (!mbar_wait(&r_empty[st], (uint32_t)(((ring / kRing) & 1) ^ 1), abort_flag)) return false;
+            mbar_expect_tx(&r_full[st], kTile);
+            const int k0 = block_of(u, n >> 1) * AK;
+            const CUtensorMap* map = (n & 1) ? &tmap_v : &tmap_k;   // V is read as an MN-major B operand: same boxes
+            tma_load_4d(sR + st * kTile, map, &r_full[st], 0, u.koff + k0, u.hk, u.bt);
+            tma_load_4d(sR + st * kTile + kTile / 2, map, &r_full[st], 64, u.koff + k0, u.hk, u.bt);
+          }
+          return true;
+        });
       }
       __syncwarp();
     } else if (warp == 9) {
@@ -210,66 +248,80 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
           umma_f16_ts(tmem_base + 256u + (uint32_t)(t * 128), pa + (uint32_t)(kk * 8), va + (uint32_t)(kk * (2048 >> 4)), idesc_o,
                       (first && kk == 0) ? 0u : 1u);
       };
-      bool ok = true;
-      for (int t = 0; t < 2 && ok; ++t)
-        if (nb[t] > 0) ok = wait(&q_full[t], 0);
-      if (ok && nbmax > 0) ok = ring_wait(0);
-      if (ok && nbmax > 0) {
-        tc_fence_after();
-        if (leader) {
-          for (int t = 0; t < 2; ++t)
-            if (nb[t] > 0 && first_of(t) == 0) {
-              issue_s(t, 0);
-              umma_commit(&mma_done[t]);
-            }
-          umma_commit(&r_empty[0]);
-        }
-      }
-      for (int j = 0; j < nbmax && ok; ++j) {
-        const int nv = 2 * j + 1, nk = 2 * j + 2;
-        if (!ring_wait(nv)) { ok = false; break; }
-        if (j + 1 < nbmax && !ring_wait(nk)) { ok = false; break; }
-        if constexpr (kWin) {
-          const int rows = Sk - block_of(j) * AK;      // of this block that are the sequence's own
-          if (p.cu_q && rows < AK) {
-            uint8_t* tile = sR + (nv % kRing) * kTile;
-            for (int x = rows * 8 + lane; x < AK * 8; x += 32) {
-              *reinterpret_cast<uint4*>(tile + x * 16) = make_uint4(0, 0, 0, 0);
-              *reinterpret_cast<uint4*>(tile + kTile / 2 + x * 16) = make_uint4(0, 0, 0, 0);
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-          }
-        }
-        for (int t = 0; t < 2; ++t) {
-          const int j0 = first_of(t);
-          const bool next = j + 1 < nb[t] && j + 1 >= j0;
-          if (j >= nb[t]) continue;
-          if (j < j0) {
-            if (next && leader) {
-              issue_s(t, nk);
-              umma_commit(&mma_done[t]);
-            }
-            continue;
-          }
-          const uint32_t par = (uint32_t)((j - j0) & 1);
-          if (!wait(&p_ready[2 * t], par)) { ok = false; break; }
-          tc_fence_after();
-          if (leader) issue_pv(t, nv, j == j0, 0, kFirstPart / 16);
-          if (!wait(&p_ready[2 * t + 1], par)) { ok = false; break; }
+      int ring = 0;                      // items of the ring before this unit's
+      uint32_t q_seen[2] = {0, 0}, p_seen[2] = {0, 0};     // Q tiles and blocks of P so far, for the phases
+      each_unit([&](const FwdUnit& u) -> bool {
+        bool ok = true;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          if (u.nb(t) > 0 && ok) ok = wait(&q_full[t], kWin ? q_seen[t]++ & 1 : 0u);
+        if (ok && u.nbmax > 0) ok = ring_wait(ring);
+        if (ok && u.nbmax > 0) {
           tc_fence_after();
           if (leader) {
-            issue_pv(t, nv, false, kFirstPart / 16, AK / 16);
-            if (next) issue_s(t, nk);              // over P of block j: the tensor core works in issue order
-            umma_commit(&mma_done[t]);
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+              if (u.nb(t) > 0 && first_of(u, t) == 0) {
+                issue_s(t, ring);
+                if (kWin && u.nb(t) == 1) umma_commit(&q_empty[t]);
+                umma_commit(&mma_done[t]);
+              }
+            umma_commit(&r_empty[ring % kRing]);
           }
         }
-        if (!ok) break;
-        if (leader) {
-          umma_commit(&r_empty[nv % kRing]);
-          if (j + 1 < nbmax) umma_commit(&r_empty[nk % kRing]);
+        for (int j = 0; j < u.nbmax && ok; ++j) {
+          const int nv = ring + 2 * j + 1, nk = ring + 2 * j + 2;
+          if (!ring_wait(nv)) { ok = false; break; }
+          if (j + 1 < u.nbmax && !ring_wait(nk)) { ok = false; break; }
+          if constexpr (kWin) {
+            const int rows = u.Sk - block_of(u, j) * AK;      // of this block that are the sequence's own
+            if (p.cu_q && rows < AK) {
+              uint8_t* tile = sR + (nv % kRing) * kTile;
+              for (int x = rows * 8 + lane; x < AK * 8; x += 32) {
+                *reinterpret_cast<uint4*>(tile + x * 16) = make_uint4(0, 0, 0, 0);
+                *reinterpret_cast<uint4*>(tile + kTile / 2 + x * 16) = make_uint4(0, 0, 0, 0);
+              }
+              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+              __syncwarp();
+            }
+          }
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const int j0 = first_of(u, t);
+            const bool next = j + 1 < u.nb(t) && j + 1 >= j0, last = kWin && j + 2 == u.nb(t);
+            if (j >= u.nb(t) || !ok) continue;
+            if (j < j0) {
+              if (next && leader) {
+                issue_s(t, nk);
+                if (last) umma_commit(&q_empty[t]);
+                umma_commit(&mma_done[t]);
+              }
+              continue;
+            }
+            const uint32_t par = kWin ? p_seen[t]++ & 1 : (uint32_t)(j & 1);
+            if (!wait(&p_ready[2 * t], par)) { ok = false; continue; }
+            tc_fence_after();
+            if (leader) issue_pv(t, nv, j == j0, 0, kFirstPart / 16);
+            if (!wait(&p_ready[2 * t + 1], par)) { ok = false; continue; }
+            tc_fence_after();
+            if (leader) {
+              issue_pv(t, nv, false, kFirstPart / 16, AK / 16);
+              if (next) {
+                issue_s(t, nk);              // over P of block j: the tensor core works in issue order
+                if (last) umma_commit(&q_empty[t]);
+              }
+              umma_commit(&mma_done[t]);
+            }
+          }
+          if (!ok) break;
+          if (leader) {
+            umma_commit(&r_empty[nv % kRing]);
+            if (j + 1 < u.nbmax) umma_commit(&r_empty[nk % kRing]);
+          }
         }
-      }
+        ring += 2 * u.nbmax;
+        return ok;
+      });
       __syncwarp();
     }
   } else {
@@ -278,174 +330,185 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
     const int t = warp >> 2;
     const int qw = warp & 3;                 // TMEM lane quarter of this warp
     const int r = qw * 32 + lane;            // query row inside the tile = TMEM lane
-    const int qi = (2 * qp + t) * AQ + r;
     const uint32_t lane_base = ((uint32_t)(qw * 32) << 16);
     const uint32_t s_addr = tmem_base + lane_base + (uint32_t)(t * 128);
     const uint32_t o_addr = tmem_base + lane_base + 256u + (uint32_t)(t * 128);
-    float m_ref = -INFINITY;                 // maximum the exponents refer to (raised lazily)
-    float l_run = 0.f;
-    bool ok = true;
-    const int n_blocks = nb[t] - first_of(t);
     // warp-uniform wait: the warp-collective TMEM accesses and votes below need all 32 lanes to take the same path
     auto wait_all = [&](uint64_t* bar, uint32_t parity) {
       const bool w = mbar_wait(bar, parity, abort_flag);
       return __all_sync(0xffffffffu, w);
     };
-    for (int j = 0; j < n_blocks; ++j) {
-      if (!wait_all(&mma_done[t], (uint32_t)(j & 1))) { ok = false; break; }
-      tc_fence_after();
-      const int k0 = block_of(j + first_of(t)) * AK;
-      // the row's visible keys: [0, lim), without [hide0, hide1) in front of the window
-      int lim = Sk - k0;
-      if (p.causal) lim = min(lim, qi - k0 + 1);
-      lim = max(0, min(lim, AK));
-      const int hide0 = kWin ? max(0, p.sinks - k0) : 0, hide1 = kWin ? qi - p.window + 1 - k0 : 0;
-      const bool full = __all_sync(0xffffffffu, lim == AK && hide0 >= hide1);
-      // the whole row of scores in registers
-      uint32_t raw[4][32];
+    uint32_t done = 0;                       // phases of mma_done[t] so far
+    each_unit([&](const FwdUnit& u) -> bool {
+      const int qi = (2 * u.qp + t) * AQ + r;
+      float m_ref = -INFINITY;                 // maximum the exponents refer to (raised lazily)
+      float l_run = 0.f;
+      bool ok = true;
+      const int n_blocks = u.nb(t) - first_of(u, t);
+      for (int j = 0; j < n_blocks; ++j) {
+        if (!wait_all(&mma_done[t], kWin ? done++ & 1 : (uint32_t)(j & 1))) { ok = false; break; }
+        tc_fence_after();
+        const int k0 = block_of(u, j + first_of(u, t)) * AK;
+        // the row's visible keys: [0, lim), without [hide0, hide1) in front of the window
+        int lim = u.Sk - k0;
+        if (p.causal) lim = min(lim, qi - k0 + 1);
+        lim = max(0, min(lim, AK));
+        const int hide0 = kWin ? max(0, p.sinks - k0) : 0, hide1 = kWin ? qi - p.window + 1 - k0 : 0;
+        const bool full = __all_sync(0xffffffffu, lim == AK && hide0 >= hide1);
+        // the whole row of scores in registers
+        uint32_t raw[4][32];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + (uint32_t)(c * 32), raw[c]);
-      tmem_ld_wait();
-      // kWin: what the row does not see becomes -inf here, two instructions an element, and the block goes the common way.  The tests
-      // inside the loops below, three times for each element, are four times the code, and a windowed CTA meets a masked block so
-      // often that it waits for instructions: 32 heads x 4096, window 64, 174 us with them.
-      if constexpr (kWin) {
-        if (!full) {
+        for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + (uint32_t)(c * 32), raw[c]);
+        tmem_ld_wait();
+        // kWin: what the row does not see becomes -inf here, two instructions an element, and the block goes the common way.  The tests
+        // inside the loops below, three times for each element, are four times the code, and a windowed CTA meets a masked block so
+        // often that it waits for instructions: 32 heads x 4096, window 64, 174 us with them.
+        if constexpr (kWin) {
+          if (!full) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const uint32_t seen = low_bits(lim - c * 32) & ~(low_bits(hide1 - c * 32) & ~low_bits(hide0 - c * 32));
+            for (int c = 0; c < 4; ++c) {
+              const uint32_t seen = low_bits(lim - c * 32) & ~(low_bits(hide1 - c * 32) & ~low_bits(hide0 - c * 32));
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (!((seen >> e) & 1u)) raw[c][e] = 0xff800000u;
+              for (int e = 0; e < 32; ++e)
+                if (!((seen >> e) & 1u)) raw[c][e] = 0xff800000u;
+            }
           }
         }
-      }
-      // P = exp2(S * scale - m) as bf16 / fp16 pairs over the first 64 columns of S; packed fp32 arithmetic, one
-      // special-function instruction per exponential, one conversion per pair.  Two instantiations: with the mask test
-      // inside one, every element pays a compare and a select.
-      float l0, l1;
-      uint32_t pk[4][16];
-      auto chunk_p = [&](auto masked, int c, float neg_m) {
-#pragma unroll
-        for (int e = 0; e < 32; e += 2) {
-          float x0, x1;
-          fma2(x0, x1, __uint_as_float(raw[c][e]), __uint_as_float(raw[c][e + 1]), p.scale_log2, neg_m);
-          float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
-          if constexpr (decltype(masked)::value) {
-            if (c * 32 + e >= lim) p0 = 0.f;
-            if (c * 32 + e + 1 >= lim) p1 = 0.f;
-          }
-          add2(l0, l1, p0, p1);
-          pk[c][e >> 1] = pack2<T>(p0, p1);
-        }
-      };
-      auto block = [&](auto masked) {
-        // The first part is computed against the reference maximum as it stands, while the block's own maximum is found
-        // beside it (four chains of three-input maxima under the special-function unit's shadow): m is raised in the first
-        // block and hardly ever after it, and only then is the first part computed again.
-        l0 = l1 = 0.f;
-        const float m_old = m_ref == -INFINITY ? 0.f : m_ref;
-#pragma unroll
-        for (int c = 0; c < kFirstPart / 32; ++c) chunk_p(masked, c, -m_old);
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
+        // P = exp2(S * scale - m) as bf16 / fp16 pairs over the first 64 columns of S; packed fp32 arithmetic, one
+        // special-function instruction per exponential, one conversion per pair.  Two instantiations: with the mask test
+        // inside one, every element pays a compare and a select.
+        float l0, l1;
+        uint32_t pk[4][16];
+        auto chunk_p = [&](auto masked, int c, float neg_m) {
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
-            float a = __uint_as_float(raw[c][e]), b2 = __uint_as_float(raw[c][e + 1]);
+            float x0, x1;
+            fma2(x0, x1, __uint_as_float(raw[c][e]), __uint_as_float(raw[c][e + 1]), p.scale_log2, neg_m);
+            float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
             if constexpr (decltype(masked)::value) {
-              if (c * 32 + e >= lim) a = -INFINITY;
-              if (c * 32 + e + 1 >= lim) b2 = -INFINITY;
+              if (c * 32 + e >= lim) p0 = 0.f;
+              if (c * 32 + e + 1 >= lim) p1 = 0.f;
             }
-            mx[(e >> 1) & 3] = max3(mx[(e >> 1) & 3], a, b2);
+            add2(l0, l1, p0, p1);
+            pk[c][e >> 1] = pack2<T>(p0, p1);
           }
-        const float m_blk = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-        const float m_new = fmaxf(m_ref, m_blk * p.scale_log2);
-        const bool raise = m_new - m_ref > kRescaleThreshold;      // also true for the first finite maximum
-        if (__any_sync(0xffffffffu, raise)) {
-          const float alpha = raise ? exp2f(m_ref - m_new) : 1.f;   // 0 when m_ref = -inf
-          if (j > 0) {
-#pragma unroll
-            for (int c = 0; c < AD / 16; ++c) {
-              uint32_t o16[16];
-              tmem_ld16(o_addr + (uint32_t)(c * 16), o16);
-              tmem_ld_wait();
-#pragma unroll
-              for (int e = 0; e < 16; ++e) o16[e] = __float_as_uint(__uint_as_float(o16[e]) * alpha);
-              tmem_st16(o_addr + (uint32_t)(c * 16), o16);
-            }
-          }
-          if (raise) {
-            l_run *= alpha;
-            m_ref = m_new;
-          }
+        };
+        auto block = [&](auto masked) {
+          // The first part is computed against the reference maximum as it stands, while the block's own maximum is found
+          // beside it (four chains of three-input maxima under the special-function unit's shadow): m is raised in the first
+          // block and hardly ever after it, and only then is the first part computed again.
           l0 = l1 = 0.f;
-          const float m_use = m_ref == -INFINITY ? 0.f : m_ref;     // row without any visible key so far
+          const float m_old = m_ref == -INFINITY ? 0.f : m_ref;
 #pragma unroll
-          for (int c = 0; c < kFirstPart / 32; ++c) chunk_p(masked, c, -m_use);
+          for (int c = 0; c < kFirstPart / 32; ++c) chunk_p(masked, c, -m_old);
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              float a = __uint_as_float(raw[c][e]), b2 = __uint_as_float(raw[c][e + 1]);
+              if constexpr (decltype(masked)::value) {
+                if (c * 32 + e >= lim) a = -INFINITY;
+                if (c * 32 + e + 1 >= lim) b2 = -INFINITY;
+              }
+              mx[(e >> 1) & 3] = max3(mx[(e >> 1) & 3], a, b2);
+            }
+          const float m_blk = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          const float m_new = fmaxf(m_ref, m_blk * p.scale_log2);
+          const bool raise = m_new - m_ref > kRescaleThreshold;      // also true for the first finite maximum
+          if (__any_sync(0xffffffffu, raise)) {
+            const float alpha = raise ? exp2f(m_ref - m_new) : 1.f;   // 0 when m_ref = -inf
+            if (j > 0) {
+#pragma unroll
+              for (int c = 0; c < AD / 16; ++c) {
+                uint32_t o16[16];
+                tmem_ld16(o_addr + (uint32_t)(c * 16), o16);
+                tmem_ld_wait();
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o16[e] = __float_as_uint(__uint_as_float(o16[e]) * alpha);
+                tmem_st16(o_addr + (uint32_t)(c * 16), o16);
+              }
+            }
+            if (raise) {
+              l_run *= alpha;
+              m_ref = m_new;
+            }
+            l0 = l1 = 0.f;
+            const float m_use = m_ref == -INFINITY ? 0.f : m_ref;     // row without any visible key so far
+#pragma unroll
+            for (int c = 0; c < kFirstPart / 32; ++c) chunk_p(masked, c, -m_use);
+          }
+#pragma unroll
+          for (int c = 0; c < kFirstPart / 32; ++c) tmem_st16(s_addr + (uint32_t)(c * 16), pk[c]);
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_ready[2 * t]);
+          const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
+#pragma unroll
+          for (int c = kFirstPart / 32; c < 4; ++c) {
+            chunk_p(masked, c, -m_use);
+            tmem_st16(s_addr + (uint32_t)(c * 16), pk[c]);
+          }
+        };
+        if constexpr (kWin) {
+          block(std::false_type{});
+        } else {
+          if (full) block(std::false_type{});
+          else block(std::true_type{});
         }
-#pragma unroll
-        for (int c = 0; c < kFirstPart / 32; ++c) tmem_st16(s_addr + (uint32_t)(c * 16), pk[c]);
+        l_run += l0 + l1;
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_ready[2 * t]);
-        const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
-#pragma unroll
-        for (int c = kFirstPart / 32; c < 4; ++c) {
-          chunk_p(masked, c, -m_use);
-          tmem_st16(s_addr + (uint32_t)(c * 16), pk[c]);
-        }
-      };
-      if constexpr (kWin) {
-        block(std::false_type{});
-      } else {
-        if (full) block(std::false_type{});
-        else block(std::true_type{});
+        if (lane == 0) mbar_arrive(&p_ready[2 * t + 1]);
       }
-      l_run += l0 + l1;
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&p_ready[2 * t + 1]);
-    }
-    if (ok && n_blocks > 0) ok = wait_all(&mma_done[t], (uint32_t)(n_blocks & 1));
-    if (ok && n_blocks > 0) {
-      tc_fence_after();
-      const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
-      T* orow = out + (int64_t)bt * p.o_sb + (int64_t)h * p.o_sh + (int64_t)(qoff + qi) * p.o_ss;
+      if (ok && n_blocks > 0) ok = wait_all(&mma_done[t], kWin ? done++ & 1 : (uint32_t)(n_blocks & 1));
+      if (ok && n_blocks > 0) {
+        tc_fence_after();
+        const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
+        T* orow = out + (int64_t)u.bt * p.o_sb + (int64_t)u.h * p.o_sh + (int64_t)(u.qoff + qi) * p.o_ss;
 #pragma unroll
-      for (int c = 0; c < AD / 32; ++c) {
-        uint32_t raw[32];
-        tmem_ld32(o_addr + (uint32_t)(c * 32), raw);
-        tmem_ld_wait();
-        if (qi < Sq) {
+        for (int c = 0; c < AD / 32; ++c) {
+          uint32_t raw[32];
+          tmem_ld32(o_addr + (uint32_t)(c * 32), raw);
+          tmem_ld_wait();
+          if (qi < u.Sq) {
 #pragma unroll
-          for (int g8 = 0; g8 < 4; ++g8) {
-            Vec16<T> v;
+            for (int g8 = 0; g8 < 4; ++g8) {
+              Vec16<T> v;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v.v[e] = ToF<T>::from(__uint_as_float(raw[g8 * 8 + e]) * inv);
-            st16(orow + c * 32 + g8 * 8, v);
+              for (int e = 0; e < 8; ++e) v.v[e] = ToF<T>::from(__uint_as_float(raw[g8 * 8 + e]) * inv);
+              st16(orow + c * 32 + g8 * 8, v);
+            }
           }
         }
+        if (qi < u.Sq && p.lse)
+          p.lse[p.cu_q ? (int64_t)u.h * p.total_q + u.qoff + qi : ((int64_t)u.b * p.H + u.h) * p.Sq + qi] = l_run > 0.f ? (m_ref + log2f(l_run)) * 0.6931471805599453f : -INFINITY;
       }
-      if (qi < Sq && p.lse)
-        p.lse[p.cu_q ? (int64_t)h * p.total_q + qoff + qi : ((int64_t)b * p.H + h) * p.Sq + qi] = l_run > 0.f ? (m_ref + log2f(l_run)) * 0.6931471805599453f : -INFINITY;
-    }
-    if constexpr (kWin) {
-      Vec16<T> zero;
+      if constexpr (kWin) {
+        Vec16<T> zero;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) zero.v[e] = ToF<T>::from(0.f);
-      if (n_blocks == 0 && qi < Sq) {                  // a query that sees no key
-        T* orow = out + (int64_t)bt * p.o_sb + (int64_t)h * p.o_sh + (int64_t)(qoff + qi) * p.o_ss;
-        for (int c = 0; c < AD; c += 8) st16(orow + c, zero);
-        if (p.lse) p.lse[p.cu_q ? (int64_t)h * p.total_q + qoff + qi : ((int64_t)b * p.H + h) * p.Sq + qi] = -INFINITY;
-      }
-      if (p.cu_q && b == p.B - 1)                      // packed rows past the last sequence: the CTAs of a head share them
-        for (int x = qp * 16 + (threadIdx.x >> 4); x < p.total_q - (qoff + Sq); x += p.q_pairs * 16) {
-          st16(out + (int64_t)h * p.o_sh + (int64_t)(qoff + Sq + x) * p.o_ss + (threadIdx.x & 15) * 8, zero);
-          if (p.lse && (threadIdx.x & 15) == 0) p.lse[(int64_t)h * p.total_q + qoff + Sq + x] = -INFINITY;
+        for (int e = 0; e < 8; ++e) zero.v[e] = ToF<T>::from(0.f);
+        if (n_blocks == 0 && qi < u.Sq) {                  // a query that sees no key
+          T* orow = out + (int64_t)u.bt * p.o_sb + (int64_t)u.h * p.o_sh + (int64_t)(u.qoff + qi) * p.o_ss;
+          for (int c = 0; c < AD; c += 8) st16(orow + c, zero);
+          if (p.lse) p.lse[p.cu_q ? (int64_t)u.h * p.total_q + u.qoff + qi : ((int64_t)u.b * p.H + u.h) * p.Sq + qi] = -INFINITY;
         }
+      }
+      return ok;
+    });
+    if constexpr (kWin) {
+      if (p.cu_q) {                                    // packed rows past the last sequence: zeros, the CTAs share them
+        Vec16<T> zero;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) zero.v[e] = ToF<T>::from(0.f);
+        for (int x = p.cu_q[p.B] + blockIdx.x * 16 + (threadIdx.x >> 4); x < p.total_q; x += gridDim.x * 16)
+          for (int y = 0; y < p.H; ++y) {
+            st16(out + (int64_t)y * p.o_sh + (int64_t)x * p.o_ss + (threadIdx.x & 15) * 8, zero);
+            if (p.lse && (threadIdx.x & 15) == 0) p.lse[(int64_t)y * p.total_q + x] = -INFINITY;
+          }
+      }
     }
   }
 
@@ -515,12 +578,14 @@ extern "C" int b200_flash_attn_fwd(const b200_attn_t* a, void* out, float* lse, 
   p.q_pairs = (p.q_blocks + 1) / 2;
   p.status = gemm_status_word_device();
   const long long grid = (long long)a->B * a->H * p.q_pairs;
-  if (grid > 2147483647ll) return (int)cudaErrorNotSupported;
+  if (grid > 2147483647ll - 1024) return (int)cudaErrorNotSupported;
+  p.units = (int)grid;
   p.window = a->window;
   p.sinks = a->sinks;
   auto launch = [&](auto kern, OncePerDevice& once, auto* o) -> int {
     if (int e = once([&] { return fwd_setup(kern); })) return e;
-    kern<<<(unsigned)grid, kAttnThreads, kAttnSmem, stream>>>(mq, mk, mv, o, p);
+    const unsigned ctas = a->window > 0 ? (unsigned)std::min<long long>(grid, gemm_sm_count()) : (unsigned)grid;
+    kern<<<ctas, kAttnThreads, kAttnSmem, stream>>>(mq, mk, mv, o, p);
     B200K_LAUNCH_RET();
   };
   static OncePerDevice once[4];

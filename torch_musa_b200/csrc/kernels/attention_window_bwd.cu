@@ -1,0 +1,691 @@
+// Flash-attention backward under a sliding window with sinks (head_dim 128, bf16 / fp16, grouped-query heads): key j is visible to query i
+// when j <= i and (i - j < window or j < sinks).
+//
+// The products, the layouts and the roles of the warps are those of attention_bwd.cu, whose comment has them: everything is computed
+// transposed, keys along the TMEM lanes; dK and dV accumulate in TMEM over the query blocks of a unit, dQ leaves by TMA reductions into
+// fp32.  What differs:
+//   * The queries that see a block of keys are a contiguous range, window + 127 long behind the block's first key, or all that follow when
+//     it holds sinks.  A block with sinks meets many more query blocks than the others (at 4096 tokens and a window of 1024: 32 against
+//     9, times the heads of a group), so its range is cut into chunks of about the others' length; their dV and dK go to fp32 buffers
+//     that a small kernel adds up in order.
+//   * Units are short, and starting and ending a CTA cost as much as three or four pairs of blocks: a CTA stays on its SM and takes every
+//     148th unit, turning round at either end so that long and short ones even out.  The loads of a unit's queries, and the waits for its
+//     first products, run while the one before it is stored.  What a change of units still costs, about 5 us of 27 for nine pairs, is
+//     the chain K -> S^T -> P -> dS that starts afresh: K and V of the next unit have no place before the last product of this one.
+//   * Hidden scores become -inf before the exponentials, two instructions an element, instead of tests inside the loops, whose second
+//     copy of the code cost more than they did (instructions came late).
+//   * Packed rows that are not the sequence's own are zeros in shared memory before a product reads them: their probabilities are zero,
+//     but zero times what lies there need not be.
+// Measured (whole calls: row dots, this kernel, sums of the chunks, conversion of dQ): 32 heads x 4096, window 1024, four sinks 273 us (289
+// with a CTA per unit); with 8 key heads 260 us.  Tried and not kept: cutting the list of pairs into 148 equal shares, so that units are
+// cut anywhere (32 heads x 4096: 484 us; neighbouring CTAs no longer read the same rows, and twice as many units begin afresh).
+//
+// Parity: no counterpart in the reference (its vendor flash backward takes a causal flag only: reference
+// torch_musa/csrc/aten/ops/attention/mudnn/SDP.cpp:678-845).
+#include "attention_bwd_common.cuh"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace b200k {
+namespace {
+using namespace gemmdev;
+using namespace attndev;
+
+struct WindowParams {
+  int B, H, Hkv, Sq, Sk;
+  float scale, scale_log2;
+  const float* lse;       // [B, H, Sq] natural log
+  const float* delta;     // [B, H, Sq]
+  float* dq;              // [B, H, Sq, 128] fp32
+  int64_t dk_sb, dk_sh, dk_ss, dv_sb, dv_sh, dv_ss;
+  int kv_blocks, q_blocks;
+  int* status;
+  // packed variable-length sequences (NULL: dense batch), as in the forward kernel; lse / delta are then [H, total_q]
+  // and dq [H, total_q, 128]
+  const int* cu_q;
+  const int* cu_k;
+  int total_q;
+  int window, sinks, total_k;
+  int units;                      // units of work that the CTAs share
+  int sink_blocks, sink_chunks;   // key blocks with sinks, CTAs that share the query blocks of one of them
+  float* sink_ws;                 // sink_chunks > 1: fp32 [B * Hkv][sink_blocks][sink_chunks][dV, dK][128][128]
+};
+
+// The query blocks [first, end) that see key block kb.
+__device__ __forceinline__ void window_queries(const WindowParams& p, int kb, int Sq, int Sk, int q_blocks, int& first, int& end) {
+  const int k0 = kb * BK;
+  first = min(q_blocks, k0 / BQ);
+  end = k0 < p.sinks ? q_blocks : min(q_blocks, (min(k0 + BK, Sk) - 1 + p.window - 1) / BQ + 1);
+  if (k0 >= Sk || end < first) end = first;
+}
+
+// Rows [rows, 128) of a tile that a copy brought into shared memory become zero (called by a converged warp, before its products
+// read the tile): they belong to another sequence, or to nobody.
+__device__ __forceinline__ void zero_tail(uint8_t* tile, int rows, int lane) {
+  for (int x = rows * 8 + lane; x < 128 * 8; x += 32) {
+    *reinterpret_cast<uint4*>(tile + x * 16) = make_uint4(0, 0, 0, 0);
+    *reinterpret_cast<uint4*>(tile + kTile / 2 + x * 16) = make_uint4(0, 0, 0, 0);
+  }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncwarp();
+}
+
+// One unit of work: a key block of one (batch, kv head), or a chunk of one.  All (batch, head) instances of the earliest key block come
+// first: under a causal mask it meets the most query blocks.
+struct BwdUnit {
+  int kb, chunk, bh, b, hk, k0, Sq, Sk, qoff, koff, bt;
+  int i0, n_i, n_it, h0, istart;      // first query block, query blocks, pairs of query block and head, where the pairs start
+  bool partial;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kBwdThreads, 1)
+attn_window_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
+                const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ CUtensorMap tmap_do,
+                const __grid_constant__ CUtensorMap tmap_dq, T* __restrict__ dk, T* __restrict__ dv, const WindowParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  if (smem - smem_raw > kBwdSlack) {        // cannot happen while the kernel has no static shared memory
+    if (threadIdx.x == 0 && p.status) atomicExch(p.status, 1);
+    return;
+  }
+  uint8_t* sK = smem;
+  uint8_t* sV = smem + kTile;
+  uint8_t* sQ = smem + 2 * kTile;                    // [2][kTile]
+  uint8_t* sdO = smem + 4 * kTile;
+  uint8_t* sS = smem + 5 * kTile;                    // dS^T [keys x queries]
+  uint8_t* sStage = smem + 6 * kTile;                // [2][kStage] fp32 dQ
+  float* s_lse = reinterpret_cast<float*>(smem + 6 * kTile + 2 * kStage);   // [2][128]
+  float* s_dlt = s_lse + 2 * 128;                                             // [2][128]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(s_dlt + 2 * 128);
+  uint64_t* kv_full = bars;                  // 1
+  uint64_t* q_full = bars + 1;               // [2]
+  uint64_t* q_empty = bars + 3;              // [2]  tcgen05.commit after dK
+  uint64_t* do_full = bars + 5;              // 1
+  uint64_t* do_empty = bars + 6;             // tcgen05.commit after dV
+  uint64_t* s_full = bars + 7;               // tcgen05.commit: S^T
+  uint64_t* dp_full = bars + 8;              // tcgen05.commit: dP^T (and with it everything issued before)
+  uint64_t* p_ready = bars + 9;              // 8 warps: P^T in TMEM
+  uint64_t* ds_ready = bars + 10;            // 8 warps: dS^T in shared memory, dP^T read
+  uint64_t* dq_full = bars + 11;             // tcgen05.commit: dQ
+  uint64_t* dq_drained = bars + 12;          // 4 warps: dQ is in registers
+  uint64_t* all_done = bars + 13;            // tcgen05.commit: dV, dK complete
+  uint64_t* ld_full = bars + 14;             // [2]  lse and delta of a query block are there
+  uint64_t* ld_empty = bars + 16;            // [2]  8 warps
+  uint64_t* acc_empty = bars + 18;           // 8 warps: dV and dK of the unit are in registers
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 19);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n_bh = p.B * p.Hkv, G = p.H / p.Hkv;
+  auto make_unit = [&](int unit) {
+    BwdUnit u{};
+    u.kb = unit / n_bh;
+    // counts (block with sinks, chunk) pairs first
+    const int pairs = p.sink_blocks * p.sink_chunks;
+    if (u.kb < pairs) {
+      u.chunk = u.kb % p.sink_chunks;
+      u.kb /= p.sink_chunks;
+    } else {
+      u.kb -= pairs - p.sink_blocks;
+    }
+    u.bh = unit % n_bh;
+    u.b = u.bh / p.Hkv;
+    u.hk = u.bh - u.b * p.Hkv;
+    u.k0 = u.kb * BK;
+    // this instance's sequence (see the forward kernel): rows past a packed sequence's end are loaded, masked by index
+    // (their probabilities and score gradients are exact zeros) and never stored
+    u.Sq = p.Sq;
+    u.Sk = p.Sk;
+    u.bt = u.b;
+    int q_blocks = p.q_blocks;
+    if (p.cu_q) {
+      u.qoff = p.cu_q[u.b];
+      u.Sq = p.cu_q[u.b + 1] - u.qoff;
+      u.koff = p.cu_k[u.b];
+      u.Sk = p.cu_k[u.b + 1] - u.koff;
+      u.bt = 0;
+      q_blocks = (u.Sq + BQ - 1) / BQ;
+    }
+    int end;
+    window_queries(p, u.kb, u.Sq, u.Sk, q_blocks, u.i0, end);
+    u.n_i = end - u.i0;
+    u.n_it = u.n_i * G;
+    u.h0 = u.hk * G;
+    u.partial = u.kb < p.sink_blocks && p.sink_chunks > 1;
+    if (u.partial) {                                  // pairs [chunk * per, (chunk + 1) * per) of this block's
+      const int per = (u.n_it + p.sink_chunks - 1) / p.sink_chunks, from = min(u.n_it, u.chunk * per);
+      u.n_it = min(u.n_it, from + per) - from;
+      if (u.n_i > 0) {
+        u.h0 += from / u.n_i;
+        u.istart = from % u.n_i;
+      }
+    }
+    return u;
+  };
+  // calls f() for every unit of this CTA until it returns false
+  auto each_unit = [&](auto f) {
+    for (int round = 0; round * (int)gridDim.x < p.units; ++round) {
+      const int unit = round * (int)gridDim.x + (round & 1 ? (int)(gridDim.x - 1 - blockIdx.x) : (int)blockIdx.x);
+      if (unit >= p.units) continue;
+      if (!f(make_unit(unit))) break;
+    }
+  };
+
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    mbar_init(kv_full, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], 1);
+      mbar_init(&ld_full[i], 1);
+      mbar_init(&ld_empty[i], 8);
+    }
+    mbar_init(do_full, 1);
+    mbar_init(do_empty, 1);
+    mbar_init(s_full, 1);
+    mbar_init(dp_full, 1);
+    mbar_init(p_ready, 8);
+    mbar_init(ds_ready, 8);
+    mbar_init(dq_full, 1);
+    mbar_init(dq_drained, 4);
+    mbar_init(all_done, 1);
+    mbar_init(acc_empty, 8);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    prefetch_tmap(&tmap_q);
+    prefetch_tmap(&tmap_k);
+    prefetch_tmap(&tmap_v);
+    prefetch_tmap(&tmap_do);
+    prefetch_tmap(&tmap_dq);
+  }
+  if (warp == 13) {
+    tmem_alloc(tmem_slot, kBwdTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  constexpr uint32_t kColS = 0, kColDP = 128, kColDV = 256, kColDK = 384;
+
+  if (warp >= 12) {
+    regs_dec<kOtherRegs>();
+    if (warp == 12) {
+      // ------------------------------------------------------------ TMA producer
+      if (lane == 0) {
+        int gi = 0, live = 0;            // pairs and units with pairs so far: the phases of the barriers
+        auto load_kv = [&](const BwdUnit& u) {
+          mbar_expect_tx(kv_full, 2 * kTile);
+          tma_load_4d(sK, &tmap_k, kv_full, 0, u.koff + u.k0, u.hk, u.bt);
+          tma_load_4d(sK + kTile / 2, &tmap_k, kv_full, 64, u.koff + u.k0, u.hk, u.bt);
+          tma_load_4d(sV, &tmap_v, kv_full, 0, u.koff + u.k0, u.hk, u.bt);
+          tma_load_4d(sV + kTile / 2, &tmap_v, kv_full, 64, u.koff + u.k0, u.hk, u.bt);
+        };
+        each_unit([&](const BwdUnit& u) -> bool {
+          if (u.n_it == 0) return true;
+          if (live == 0) load_kv(u);
+          int h = u.h0, i = u.istart;
+          for (int it = 0; it < u.n_it; ++it, ++gi) {
+            const int q0 = (u.i0 + i) * BQ, st = gi & 1;
+            if (!mbar_wait(&q_empty[st], (uint32_t)(((gi >> 1) & 1) ^ 1), abort_flag)) return false;
+            mbar_expect_tx(&q_full[st], kTile);
+            tma_load_4d(sQ + st * kTile, &tmap_q, &q_full[st], 0, u.qoff + q0, h, u.bt);
+            tma_load_4d(sQ + st * kTile + kTile / 2, &tmap_q, &q_full[st], 64, u.qoff + q0, h, u.bt);
+            if (!mbar_wait(do_empty, (uint32_t)((gi & 1) ^ 1), abort_flag)) return false;
+            mbar_expect_tx(do_full, kTile);
+            tma_load_4d(sdO, &tmap_do, do_full, 0, u.qoff + q0, h, u.bt);
+            tma_load_4d(sdO + kTile / 2, &tmap_do, do_full, 64, u.qoff + q0, h, u.bt);
+            if (it == 0 && live > 0) {       // K and V are free when every product of the unit before is done
+              if (!mbar_wait(all_done, (uint32_t)((live - 1) & 1), abort_flag)) return false;
+              load_kv(u);
+            }
+            if (++i == u.n_i) { i = 0; ++h; }
+          }
+          ++live;
+          return true;
+        });
+      }
+      __syncwarp();
+    } else if (warp == 13) {
+      // ------------------------------------------------------------ MMA issuer (the whole warp waits, one lane issues)
+      constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+      constexpr uint32_t idesc_kk = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(128 >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+      constexpr uint32_t idesc_kmn = idesc_kk | (1u << 16);                 // B read MN-major
+      constexpr uint32_t idesc_mnmn = idesc_kk | (1u << 15) | (1u << 16);   // A and B read MN-major
+      const bool issuer = elect_one();
+      auto wait = [&](uint64_t* bar, int n) { return mbar_wait_warp(bar, (uint32_t)(n & 1), abort_flag); };
+      auto kdesc = [&](const uint8_t* tile) { return make_desc(smem_u32(tile), 16, 1024); };            // read K-major
+      auto mndesc = [&](const uint8_t* tile) { return make_desc(smem_u32(tile), kTile / 2, 1024); };    // read MN-major
+      const uint64_t dK_k = kdesc(sK), dV_k = kdesc(sV), dO_k = kdesc(sdO), dQ_k = kdesc(sQ), dS_k = kdesc(sS);
+      const uint64_t dK_mn = mndesc(sK), dO_mn = mndesc(sdO), dQ_mn = mndesc(sQ), dS_mn = mndesc(sS);
+      auto koff16 = [](int kk) { return (uint32_t)(((kk >> 2) * (kTile / 2) + (kk & 3) * 32) >> 4); };   // K-major: two 64-column atoms
+      auto mnoff16 = [](int kk) { return (uint32_t)((kk * 2048) >> 4); };                                // MN-major: 16 rows of 128 bytes
+      int base = 0, live = 0;              // pairs before this unit's, units with pairs so far
+      each_unit([&](const BwdUnit& u) -> bool {
+        if (u.n_it == 0) return true;
+        bool ok = wait(kv_full, live) && wait(&q_full[base & 1], base >> 1);
+        // the rows of the current and the next query block that are the sequence's own (128 or more: all)
+        int mi = u.istart;
+        auto own_rows = [&]() { return u.Sq - (u.i0 + mi) * BQ; };
+        if (ok && p.cu_q) {
+          if (u.k0 + BK > u.Sk) {
+            zero_tail(sK, u.Sk - u.k0, lane);
+            zero_tail(sV, u.Sk - u.k0, lane);
+          }
+          if (own_rows() < BQ) zero_tail(sQ + (base & 1) * kTile, own_rows(), lane);
+        }
+        if (ok) {
+          tc_fence_after();
+          if (issuer) {
+            const uint32_t tq = (uint32_t)((base & 1) * (kTile >> 4));
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk) umma_f16(tmem_base + kColS, dK_k + koff16(kk), dQ_k + tq + koff16(kk), idesc_kk, kk != 0 ? 1u : 0u);
+            umma_commit(s_full);
+          }
+        }
+        for (int it = 0; it < u.n_it && ok; ++it) {
+          const int gi = base + it;
+          const uint32_t tq = (uint32_t)((gi & 1) * (kTile >> 4)), tq_next = (uint32_t)(((gi + 1) & 1) * (kTile >> 4));
+          if (!wait(do_full, gi)) { ok = false; break; }
+          if (p.cu_q && own_rows() < BQ) zero_tail(sdO, own_rows(), lane);
+          if (gi > 0 && !wait(dq_drained, gi - 1)) { ok = false; break; }
+          tc_fence_after();
+          if (issuer) {
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk) umma_f16(tmem_base + kColDP, dV_k + koff16(kk), dO_k + koff16(kk), idesc_kk, kk != 0 ? 1u : 0u);
+            umma_commit(dp_full);                        // dP^T = V dO^T
+          }
+          if (!wait(p_ready, gi)) { ok = false; break; }
+          if (it == 0 && live > 0 && !wait(acc_empty, live - 1)) { ok = false; break; }
+          tc_fence_after();
+          if (issuer) {
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk)               // dV += P^T dO; P^T of 64 queries over the left of its half of S^T
+              umma_f16_ts(tmem_base + kColDV, tmem_base + kColS + (uint32_t)((kk >> 2) * 64 + (kk & 3) * 8), dO_mn + mnoff16(kk),
+                          idesc_kmn, (it == 0 && kk == 0) ? 0u : 1u);
+            umma_commit(do_empty);
+          }
+          if (it + 1 < u.n_it) {
+            if (!wait(&q_full[(gi + 1) & 1], (gi + 1) >> 1)) { ok = false; break; }
+            if (++mi == u.n_i) mi = 0;
+            if (p.cu_q && own_rows() < BQ) zero_tail(sQ + ((gi + 1) & 1) * kTile, own_rows(), lane);
+            tc_fence_after();
+            if (issuer) {
+#pragma unroll
+              for (int kk = 0; kk < 8; ++kk)             // S^T of the next pair, over P^T of this one
+                umma_f16(tmem_base + kColS, dK_k + koff16(kk), dQ_k + tq_next + koff16(kk), idesc_kk, kk != 0 ? 1u : 0u);
+              umma_commit(s_full);
+            }
+          }
+          if (!wait(ds_ready, gi)) { ok = false; break; }
+          tc_fence_after();
+          if (issuer) {
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk)               // dQ = dS K over the consumed dP^T
+              umma_f16(tmem_base + kColDP, dS_mn + mnoff16(kk), dK_mn + mnoff16(kk), idesc_mnmn, kk != 0 ? 1u : 0u);
+            umma_commit(dq_full);
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk)               // dK += dS^T Q
+              umma_f16(tmem_base + kColDK, dS_k + koff16(kk), dQ_mn + tq + mnoff16(kk), idesc_kmn, (it == 0 && kk == 0) ? 0u : 1u);
+            umma_commit(&q_empty[gi & 1]);
+            if (it + 1 == u.n_it) umma_commit(all_done);
+          }
+        }
+        base += u.n_it;
+        ++live;
+        return ok;
+      });
+      __syncwarp();
+    } else if (warp == 14) {
+      // ------------------------------------------------------------ lse (log2 domain, negated: an addend of the exponent) and
+      // delta (times the softmax scale, negated) of every query block; an lse of -inf switches a row off
+      // (read one block ahead, all eight loads in flight at once)
+      int h, i, gi = 0;
+      float l[4], d[4];
+      auto fetch = [&](const BwdUnit& u) {
+        const int64_t base = p.cu_q ? (int64_t)h * p.total_q + u.qoff : ((int64_t)u.b * p.H + h) * p.Sq;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int qi = (u.i0 + i) * BQ + e * 32 + lane;
+          l[e] = qi < u.Sq ? __ldg(p.lse + base + qi) : -INFINITY;
+          d[e] = qi < u.Sq ? __ldg(p.delta + base + qi) : 0.f;
+        }
+      };
+      each_unit([&](const BwdUnit& u) -> bool {
+        h = u.h0;
+        i = u.istart;
+        if (u.n_it > 0) fetch(u);
+        for (int it = 0; it < u.n_it; ++it, ++gi) {
+          const int st = gi & 1;
+          if (!mbar_wait_warp(&ld_empty[st], (uint32_t)(((gi >> 1) & 1) ^ 1), abort_flag)) return false;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            s_lse[st * 128 + e * 32 + lane] = l[e] > -INFINITY ? -l[e] * 1.4426950408889634f : -INFINITY;
+            s_dlt[st * 128 + e * 32 + lane] = -d[e] * p.scale;
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ld_full[st]);
+          if (++i == u.n_i) { i = 0; ++h; }
+          if (it + 1 < u.n_it) fetch(u);
+        }
+        return true;
+      });
+    }
+  } else if (warp >= 8) {
+    regs_inc<kDqRegs>();
+    // ------------------------------------------------------------ dQ warpgroup: TMEM -> registers -> shared memory -> global
+    const int qw = warp & 3;
+    const int r = qw * 32 + lane;                 // query row inside the block = TMEM lane
+    const uint32_t addr = tmem_base + ((uint32_t)(qw * 32) << 16) + kColDP;
+    int gi = 0;
+    each_unit([&](const BwdUnit& u) -> bool {
+      int h = u.h0, i = u.istart;
+      for (int it = 0; it < u.n_it; ++it, ++gi) {
+        const int q0 = (u.i0 + i) * BQ;
+        bool ok = mbar_wait_warp(dq_full, (uint32_t)(gi & 1), abort_flag);
+        tc_fence_after();
+        uint32_t raw[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32(addr + (uint32_t)(c * 32), raw[c]);
+        tmem_ld_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(dq_drained);
+        const int row0 = p.cu_q ? (int)((int64_t)h * p.total_q + u.qoff + q0) : (int)(((int64_t)u.b * p.H + h) * p.Sq + q0);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          // the reduction that read this box two chunks ago has finished with it
+          if (threadIdx.x == 8 * 32) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+          if (!named_bar_and(1, 128, ok)) { ok = false; break; }     // one answer for the four warps
+          uint8_t* box = sStage + (c & 1) * kStage + (size_t)r * 128;
+#pragma unroll
+          for (int ch = 0; ch < 8; ++ch)
+            *reinterpret_cast<uint4*>(box + (size_t)((ch ^ (r & 7)) * 16)) =
+                make_uint4(raw[c][ch * 4], raw[c][ch * 4 + 1], raw[c][ch * 4 + 2], raw[c][ch * 4 + 3]);
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          named_bar_sync(1, 128);
+          if (threadIdx.x == 8 * 32) {
+            tma_reduce_add_2d(&tmap_dq, sStage + (c & 1) * kStage, c * 32, row0);
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          }
+        }
+        if (!ok) return false;
+        if (++i == u.n_i) { i = 0; ++h; }
+      }
+      return true;
+    });
+    // every reduction must have completed before the CTA exits
+    if (threadIdx.x == 8 * 32) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  } else {
+    regs_inc<kComputeRegs>();
+    // ------------------------------------------------------------ two compute warpgroups (warps 0-3, 4-7)
+    const int wg = warp >> 2;
+    const int qw = warp & 3;
+    const int r = qw * 32 + lane;                 // key row inside the block = TMEM lane
+    const uint32_t lane_base = ((uint32_t)(qw * 32) << 16);
+    const uint32_t s_addr = tmem_base + lane_base + kColS + (uint32_t)(wg * 64);
+    const uint32_t dp_addr = tmem_base + lane_base + kColDP + (uint32_t)(wg * 64);
+    uint8_t* srow = sS + (size_t)wg * (kTile / 2) + (size_t)r * 128;   // this warpgroup's 64 query columns = atom `wg`
+    auto wait_all = [&](uint64_t* bar, uint32_t parity) { return mbar_wait_warp(bar, parity, abort_flag); };
+    int gi = 0, live = 0;
+    each_unit([&](const BwdUnit& u) -> bool {
+      const int kj = u.k0 + r;
+      const bool key_off = kj >= u.Sk;
+      const bool block_off = u.k0 + BK > u.Sk;
+      const int far = kj >= p.sinks ? kj + p.window : 0x7fffffff;      // the first query that no longer sees this key
+      bool ok = true;
+      int i = u.istart;
+      for (int it = 0; it < u.n_it; ++it, ++gi) {
+        const uint32_t par = (uint32_t)(gi & 1);
+        const int st = gi & 1, q0 = (u.i0 + i) * BQ;
+        const float4* nlse4 = reinterpret_cast<const float4*>(s_lse + st * 128 + wg * 64);
+        const float4* ndlt4 = reinterpret_cast<const float4*>(s_dlt + st * 128 + wg * 64);
+        // only then can a query be older than a key of this block, a key be past the end or in front of a window
+        const bool masked = q0 < u.k0 + BK || block_off || q0 + BQ - u.k0 > p.window;
+        if (!wait_all(&ld_full[st], (uint32_t)((gi >> 1) & 1)) || !wait_all(s_full, par)) { ok = false; break; }
+        tc_fence_after();
+        float pf[64];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t raw[32], pk[16];
+          tmem_ld32(s_addr + (uint32_t)(c * 32), raw);
+          tmem_ld_wait();
+          if (masked) {              // what is not seen becomes -inf
+            const int q = q0 + wg * 64 + c * 32;
+            const uint32_t seen = key_off ? 0u : low_bits(far - q) & ~low_bits(kj - q);
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (!((seen >> e) & 1u)) raw[e] = 0xff800000u;
+          }
+#pragma unroll
+          for (int e4 = 0; e4 < 8; ++e4) {
+            const float4 nl = nlse4[c * 8 + e4];
+            const float nls[4] = {nl.x, nl.y, nl.z, nl.w};
+#pragma unroll
+            for (int e2 = 0; e2 < 4; e2 += 2) {
+              const int e = e4 * 4 + e2, cc = c * 32 + e;
+              float x0, x1;
+              fma2v(x0, x1, __uint_as_float(raw[e]), __uint_as_float(raw[e + 1]), p.scale_log2, nls[e2], nls[e2 + 1]);
+              float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
+              pf[cc] = p0;
+              pf[cc + 1] = p1;
+              pk[e >> 1] = pack2<T>(p0, p1);
+            }
+          }
+          tmem_st16(s_addr + (uint32_t)(c * 16), pk);   // over columns of S^T that this thread has read
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_ready);
+        // dP^T; its commit also says that the products which read the previous dS^T have completed
+        if (!wait_all(dp_full, par)) { ok = false; break; }
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t raw[32], pk[16];
+          tmem_ld32(dp_addr + (uint32_t)(c * 32), raw);
+          tmem_ld_wait();
+#pragma unroll
+          for (int e4 = 0; e4 < 8; ++e4) {
+            const float4 nd = ndlt4[c * 8 + e4];
+            const float nds[4] = {nd.x, nd.y, nd.z, nd.w};
+#pragma unroll
+            for (int e2 = 0; e2 < 4; e2 += 2) {
+              const int e = e4 * 4 + e2, cc = c * 32 + e;
+              float t0, t1, d0, d1;
+              fma2v(t0, t1, __uint_as_float(raw[e]), __uint_as_float(raw[e + 1]), p.scale, nds[e2], nds[e2 + 1]);
+              mul2(d0, d1, pf[cc], pf[cc + 1], t0, t1);
+              pk[e >> 1] = pack2<T>(d0, d1);
+            }
+          }
+#pragma unroll
+          for (int g8 = 0; g8 < 4; ++g8) {
+            const int ch = c * 4 + g8;
+            *reinterpret_cast<uint4*>(srow + (size_t)((ch ^ (r & 7)) * 16)) =
+                make_uint4(pk[g8 * 4], pk[g8 * 4 + 1], pk[g8 * 4 + 2], pk[g8 * 4 + 3]);
+          }
+        }
+        tc_fence_before();
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(ds_ready);
+          mbar_arrive(&ld_empty[st]);
+        }
+        if (++i == u.n_i) i = 0;
+      }
+      if (ok && u.n_it > 0) ok = wait_all(all_done, (uint32_t)(live & 1));
+      // ---- dK, dV of this key block
+      if (ok) {
+        tc_fence_after();
+        const bool row_ok = kj < u.Sk;
+        T* dk_row = dk + (int64_t)u.bt * p.dk_sb + (int64_t)u.hk * p.dk_sh + (int64_t)(u.koff + kj) * p.dk_ss + wg * 64;
+        T* dv_row = dv + (int64_t)u.bt * p.dv_sb + (int64_t)u.hk * p.dv_sh + (int64_t)(u.koff + kj) * p.dv_ss + wg * 64;
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            uint32_t raw[32];
+            if (u.n_it > 0) {
+              tmem_ld32(tmem_base + lane_base + (which ? kColDK : kColDV) + (uint32_t)(wg * 64 + c * 32), raw);
+              tmem_ld_wait();
+            } else {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) raw[e] = 0u;
+            }
+            if (u.partial) {
+              float* dst = p.sink_ws + ((((int64_t)u.bh * p.sink_blocks + u.kb) * p.sink_chunks + u.chunk) * 2 + which) * (BK * BD) + r * BD +
+                           wg * 64 + c * 32;
+              if (u.n_it > 0) {
+#pragma unroll
+                for (int g4 = 0; g4 < 8; ++g4)
+                  *reinterpret_cast<uint4*>(dst + g4 * 4) = make_uint4(raw[g4 * 4], raw[g4 * 4 + 1], raw[g4 * 4 + 2], raw[g4 * 4 + 3]);
+              }
+            } else if (row_ok) {
+              T* dst = (which ? dk_row : dv_row) + c * 32;
+#pragma unroll
+              for (int g8 = 0; g8 < 4; ++g8) {
+                Vec16<T> v;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v.v[e] = ToF<T>::from(__uint_as_float(raw[g8 * 8 + e]));
+                st16(dst + g8 * 8, v);
+              }
+            }
+          }
+        }
+      }
+      if (u.n_it > 0) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(acc_empty);
+        ++live;
+      }
+      if (p.cu_q && u.b == p.B - 1 && u.chunk == 0) {       // packed rows past the last sequence: the CTAs of a head share them
+        Vec16<T> zero;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) zero.v[e] = ToF<T>::from(0.f);
+        for (int x = u.kb * 16 + (threadIdx.x >> 4); x < p.total_k - (u.koff + u.Sk); x += p.kv_blocks * 16) {
+          const int64_t row = u.koff + u.Sk + x;
+          st16(dk + (int64_t)u.hk * p.dk_sh + row * p.dk_ss + (threadIdx.x & 15) * 8, zero);
+          st16(dv + (int64_t)u.hk * p.dv_sh + row * p.dv_ss + (threadIdx.x & 15) * 8, zero);
+        }
+      }
+      return ok;
+    });
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 13) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, kBwdTmemCols);
+  }
+  settle_abort(abort_flag, p.status);
+}
+
+// dV and dK of the blocks with sinks: the chunks' sums, added in order (the same for every run) and rounded once.  A thread owns
+// eight dimensions of a row.
+template <typename T>
+__global__ void __launch_bounds__(256) attn_sink_sum_kernel(T* __restrict__ dk, T* __restrict__ dv, const WindowParams p) {
+  const int which = blockIdx.y, r = (int)(blockIdx.x % 8) * 16 + (threadIdx.x >> 4), c = (threadIdx.x & 15) * 8;
+  const int unit = (int)(blockIdx.x / 8), kb = unit % p.sink_blocks, bh = unit / p.sink_blocks;
+  const int b = bh / p.Hkv, hk = bh - b * p.Hkv, kj = kb * BK + r;
+  int Sq = p.Sq, Sk = p.Sk, koff = 0, bt = b, q_blocks = p.q_blocks;
+  if (p.cu_q) {
+    Sq = p.cu_q[b + 1] - p.cu_q[b];
+    koff = p.cu_k[b];
+    Sk = p.cu_k[b + 1] - koff;
+    bt = 0;
+    q_blocks = (Sq + BQ - 1) / BQ;
+  }
+  if (kj >= Sk) return;
+  int first, end;
+  window_queries(p, kb, Sq, Sk, q_blocks, first, end);
+  const int n_it = (end - first) * (p.H / p.Hkv), per = (n_it + p.sink_chunks - 1) / p.sink_chunks;
+  float s[8] = {};
+  const float* src = p.sink_ws + (((int64_t)unit * p.sink_chunks) * 2 + which) * (BK * BD) + r * BD + c;
+  for (int ch = 0; ch * per < n_it; ++ch, src += 2 * BK * BD) {
+    const float4 x = *reinterpret_cast<const float4*>(src), y = *reinterpret_cast<const float4*>(src + 4);
+    s[0] += x.x; s[1] += x.y; s[2] += x.z; s[3] += x.w;
+    s[4] += y.x; s[5] += y.y; s[6] += y.z; s[7] += y.w;
+  }
+  Vec16<T> o;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) o.v[e] = ToF<T>::from(s[e]);
+  if (which) st16(dk + (int64_t)bt * p.dk_sb + (int64_t)hk * p.dk_sh + (int64_t)(koff + kj) * p.dk_ss + c, o);
+  else st16(dv + (int64_t)bt * p.dv_sb + (int64_t)hk * p.dv_sh + (int64_t)(koff + kj) * p.dv_ss + c, o);
+}
+
+// How many CTAs share the query blocks of a key block with sinks: as many as make their ranges about as long as the others'.
+int sink_chunks(const b200_attn_t* a) {
+  if (a->window <= 0 || a->sinks <= 0) return 1;
+  const int q_blocks = (a->Sq + BQ - 1) / BQ;
+  const int others = std::min<long long>(q_blocks, (a->window + BK - 2ll) / BQ + 1);
+  return std::max(1, std::min(64, (q_blocks + others - 1) / std::max(1, others)));
+}
+int sink_blocks(const b200_attn_t* a) { return a->window > 0 ? (std::min(a->sinks, a->Sk) + BK - 1) / BK : 0; }
+
+}  // namespace
+}  // namespace b200k
+
+using namespace b200k;
+
+extern "C" int64_t b200_flash_attn_bwd_workspace(const b200_attn_t* a) {
+  const int chunks = sink_chunks(a);
+  return chunks > 1 ? (int64_t)a->B * a->Hkv * sink_blocks(a) * chunks * 2 * BK * BD : 0;
+}
+
+namespace b200k {
+
+int attn_window_bwd(const b200_attn_t* a, float* dq_accum, void* dk, void* dv, float* delta, const void* q, const void* k, const void* v,
+                    const void* o, const void* d_o, const float* lse, const int64_t* extra_strides, cudaStream_t stream) {
+  BwdMaps m;
+  if (int e = bwd_maps(&m, a, dq_accum, dk, dv, q, k, v, o, d_o, extra_strides)) return e;
+  const int64_t* x = extra_strides;
+  WindowParams p{};
+  p.B = a->B; p.H = a->H; p.Hkv = a->Hkv; p.Sq = a->Sq; p.Sk = a->Sk;
+  p.scale = a->scale;
+  p.scale_log2 = a->scale * 1.4426950408889634f;
+  p.lse = lse;
+  p.delta = delta;
+  p.dq = dq_accum;
+  p.dk_sb = x[3]; p.dk_sh = x[4]; p.dk_ss = x[5];
+  p.dv_sb = x[6]; p.dv_sh = x[7]; p.dv_ss = x[8];
+  p.kv_blocks = (a->Sk + BK - 1) / BK;
+  p.q_blocks = (a->Sq + BQ - 1) / BQ;
+  p.status = gemm_status_word_device();
+  p.cu_q = a->cu_seqlens_q;
+  p.cu_k = a->cu_seqlens_k;
+  p.total_q = a->total_q;
+  p.window = a->window;
+  p.sinks = a->sinks;
+  p.total_k = a->total_k;
+  p.sink_blocks = sink_blocks(a);
+  p.sink_chunks = sink_chunks(a);
+  p.sink_ws = a->workspace;
+  if (!a->causal || a->window > (1 << 30) || a->sinks < 0 || (p.sink_chunks > 1 && !p.sink_ws)) return (int)cudaErrorNotSupported;
+  const long long units = (long long)a->B * a->Hkv * (p.kv_blocks + p.sink_blocks * (p.sink_chunks - 1));
+  if (units > 2147483647ll - 1024) return (int)cudaErrorNotSupported;
+  p.units = (int)units;
+  const unsigned grid = (unsigned)std::min<long long>(units, gemm_sm_count());
+  auto launch = [&](auto kern, OncePerDevice& once, auto* gk, auto* gv) -> int {
+    using T = std::remove_pointer_t<decltype(gk)>;
+    if (int e = once([&] { return bwd_setup(kern); })) return e;
+    attn_delta_kernel<T><<<m.delta_grid, 256, 0, stream>>>((const T*)o, (const T*)d_o, delta, dq_accum, a->H, m.delta_rows, (int)m.row_blocks,
+                                                           a->o_sb, a->o_sh, a->o_ss, x[0], x[1], x[2]);
+    kern<<<grid, kBwdThreads, kBwdSmem, stream>>>(m.q, m.k, m.v, m.d_o, m.dq, gk, gv, p);
+    note_launch(2);
+    if (p.sink_blocks > 0 && p.sink_chunks > 1) {
+      attn_sink_sum_kernel<T><<<dim3((unsigned)(a->B * a->Hkv * p.sink_blocks * 8), 2), 256, 0, stream>>>(gk, gv, p);
+      note_launch();
+    }
+    return (int)cudaGetLastError();
+  };
+  static OncePerDevice once[2];
+  return a->dtype == B200_BF16 ? launch(attn_window_bwd_kernel<__nv_bfloat16>, once[0], (__nv_bfloat16*)dk, (__nv_bfloat16*)dv)
+                               : launch(attn_window_bwd_kernel<__half>, once[1], (__half*)dk, (__half*)dv);
+}
+
+}  // namespace b200k
