@@ -122,6 +122,16 @@ def test_unary_integer_and_bool(bw, dev):
     assert not bw.fallback_counts(), bw.fallback_counts()
 
 
+def test_bitwise_not_of_bool(bw, dev):
+    bw.reset_fallback_counts()
+    x = _rand((4, 9), torch.bool)
+    for t in (x, x.t(), x[:, ::2], x[:, :1].expand(4, 9)):
+        _check(torch.bitwise_not, (t,), dev)
+    _check(lambda t: t.clone().bitwise_not_(), (x,), dev)
+    _check(lambda t: torch.bitwise_not(t, out=torch.empty(4, 9, dtype=torch.bool, device=t.device)), (x,), dev)
+    assert not bw.fallback_counts(), bw.fallback_counts()
+
+
 def test_where_clamp_masked_fill_addc_lerp(bw, dev):
     bw.reset_fallback_counts()
     for dt in (torch.float32, torch.bfloat16, torch.int64):

@@ -226,7 +226,8 @@ B200_PW_UNARY(asinh, "asinh", B200_EW_ASINH, kFloat)
 B200_PW_UNARY(acosh, "acosh", B200_EW_ACOSH, kFloat)
 B200_PW_UNARY(atanh, "atanh", B200_EW_ATANH, kFloat)
 B200_PW_UNARY(erfc, "erfc", B200_EW_ERFC, kFloat)
-B200_PW_UNARY(bitwise_not, "bitwise_not", B200_EW_BITWISE_NOT, kSame)
+// ~1 is not zero, and so would be stored as true
+B200_PW_UNARY(bitwise_not, "bitwise_not", a.scalar_type() == at::kBool ? B200_EW_LOGICAL_NOT : B200_EW_BITWISE_NOT, kSame)
 // .out forms of the operators whose functional / in-place forms live in Elementwise.cpp
 B200_PW_UNARY(exp_g, "exp", B200_EW_EXP, kFloat)
 B200_PW_UNARY(sqrt_g, "sqrt", B200_EW_SQRT, kFloat)
