@@ -91,6 +91,36 @@ def test_paged_attention(bw, dev, dt, lens, n, H, Hkv, D, page, window, sinks):
     check(out, *want_attention(*args, window, sinks))
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("n", [1, 3])
+def test_pages_without_a_visible_key_are_not_asked_for(bw, dev, D, n):
+    """Every place of a window's and the sinks' edge within pages of 16, which are shorter than a step of the kernel: the table's other
+    entries are out of range, and nothing is reported."""
+    for window in (1, 2, 15, 16, 17, 31, 32, 33, 40):
+        for sinks in (0, 1, 15, 16, 17, 20):
+            lens = [100 + 7 * window % 33, 64, 49, n]
+            args = case(window, lens, n, 4, 2, D, 16, torch.float16, window, sinks)
+            out = paged_attention(*(t.to(dev) for t in args), window=window, sinks=sinks)
+            bw.synchronize()
+            check(out, *want_attention(*args, window, sinks), f"window {window}, sinks {sinks}")
+
+
+def test_other_types_and_head_sizes_take_the_plain_way(bw, dev):
+    for dt, D in ((torch.float32, 64), (torch.float16, 32)):
+        args = case(20, [40, 3, 0], 2, 4, 2, D, 16, dt, 10, 1)
+        out = paged_attention(*(t.to(dev) for t in args), window=10, sinks=1)
+        check(out, *want_attention(*args, 10, 1))
+    cos, sin = precompute_rope_cache(64, 32)
+    _, k, v, table, lens = case(21, [40, 3], 1, 2, 1, 32, 16, torch.float32)
+    k.zero_(), v.zero_()
+    new = torch.randn(2, 4, 32, generator=torch.Generator().manual_seed(1))
+    on = [t.to(dev) for t in (new, cos, sin, k, v, table, lens)]
+    out = paged_rope_cache(on[0][:, :2], on[0][:, 2:3], on[0][:, 3:], *on[1:])
+    want = paged_rope_cache(new[:, :2], new[:, 2:3], new[:, 3:], cos, sin, k, v, table, lens)
+    for a, b in ((out, want), (on[3], k), (on[4], v)):
+        assert float((a.cpu() - b).abs().max()) <= 2.0 ** -20      # products of values below 4, each side rounded in 32 bits
+
+
 def test_keys_of_later_tokens_do_not_reach_earlier_ones(bw, dev):
     """n tokens at once with infinities and NaN in the newest keys and values, and in those that only the oldest token still sees."""
     n, window = 4, 50

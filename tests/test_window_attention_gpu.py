@@ -277,6 +277,24 @@ def test_refusals(bw, dev):
         assert [g.shape for g in torch.autograd.grad(o, e, torch.zeros_like(o))] == [t.shape for t in e]
 
 
+def test_other_types_and_head_sizes_take_the_plain_way(bw, dev):
+    from torch_musa_b200.ops import flash_attn_varlen_func, window_attention
+
+    g = torch.Generator().manual_seed(9)
+    for dt, size in ((torch.float32, 128), (torch.bfloat16, 64)):
+        q, k, v, do = (torch.randn(1, 50, h, size, generator=g).to(dt) for h in (4, 2, 2, 4))
+        sides = []
+        for where in (dev, torch.device("cpu")):
+            leaves = [t.to(where).requires_grad_() for t in (q, k, v)]
+            out = window_attention(*leaves, 9, 2)
+            flat = [t[0].to(where) for t in (q, k, v)]
+            cu = torch.tensor([0, 20, 50], dtype=torch.int32).to(where)
+            packed = flash_attn_varlen_func(*flat, cu, cu, 30, 30, causal=True, window=9, sinks=2)
+            sides.append([t.detach().cpu().float() for t in (out, packed, *torch.autograd.grad(out, leaves, do.to(where)))])
+        for a, b in zip(*sides):      # both ways round to the type a few times, values of a few
+            assert float((a - b).abs().max()) <= 16 * torch.finfo(dt).eps * max(1.0, float(b.abs().max()))
+
+
 def test_two_streams_and_two_graphs(bw, dev):
     """Forward and backward of two problems at once, each on a stream of its own, eager and replayed: scratch is not shared.  (The last
     bits of dq follow the order of arrival.)"""

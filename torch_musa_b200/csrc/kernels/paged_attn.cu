@@ -137,6 +137,15 @@ __device__ __forceinline__ bool not_finite(uint32_t w) {
 // A lane's columns are rows 2 t and 2 t + 1 in both, so a row's maximum and sum stay with the lanes that hold its outputs.  P goes in as
 // a 16-bit value plus the 16-bit remainder of its rounding (2^-16 or better).  The maximum that exponents refer to is raised only
 // when a score exceeds it by 2^8: then eight lanes have to be asked, which most steps leave out.
+//
+// What bounds it: memory, where the batch fills the machine -- 32 sequences of 1100 to 2048 keys with 32 key heads: 126 us, 830 MB read once,
+// 6.6 TB/s, warps waiting for their copies (long scoreboard 5.3 of 10.9 clocks an instruction); two of 50001 to 65536 keys with 8 key heads:
+// 82 us, 5.8 TB/s, on 384 of 444 places.  Where it is small, the way from the launch through length, table and keys to the joins: 3.4 us
+// for 32 keys, 5.1 for 500.  With several tokens at once, issue: 20 rows a key head, D 64, take 190 instructions for 16 keys (4 KB), so
+// 16 sequences, window 1024, five tokens take 14.3 us where one token takes 8.5.
+// On the way here (us, the first two of these cases): a warp per row and scalar products 2262 / 72680; the tensor core with operands
+// copied piece by piece into a lane's own slots 181 / 156 (600, then 400 instructions for 16 keys); whole rows and ldmatrix 127 / 93; keys as
+// the long side of the products 124 / 82, and D 64 with four rows a key head, 64 sequences of up to 4000 keys, 62 -> 50.
 // kDense: the rows of a page follow one another (the layout of the pools as they are made), so that a copy's address is a constant
 // away from the page's.
 template <typename T, int D, int NT, bool kDense>
@@ -190,12 +199,19 @@ __global__ void __launch_bounds__(kPagedWarps * 32, NT * D <= 256 ? 3 : 2) paged
     vaddr[x] = ring + (uint32_t)(kHalves * kHalf + ((mi >> 1) * 8 + mr) * D * 2) + (((uint32_t)x * 32) ^ (uint32_t)(((mi & 1) ^ mr) * 16));
   }
 
+  // A step's page numbers, read one step before they are needed; kNoPage for a half in which nobody sees a key: the table's entry may then
+  // be anything.
+  constexpr int kNoPage = -0x7fffffff - 1;
   struct Pages { int n[kHalves]; };
-  auto entry = [&](int s) {          // the page numbers of a step, read one step before they are needed
+  auto entry = [&](int s) {
     Pages e;
     const int k0 = key_of(s);
 #pragma unroll
-    for (int x = 0; x < kHalves; ++x) e.n[x] = s < s1 && k0 + x * kPageRows <= pos1 ? __ldg(table + p.by_page(k0 + x * kPageRows)) : -1;
+    for (int x = 0; x < kHalves; ++x) {
+      const int kx = k0 + x * kPageRows;
+      const bool seen = s < s1 && kx <= pos1 && (kHalves == 1 || kx + kPageRows > wlo || kx < p.sinks);
+      e.n[x] = seen ? max(__ldg(table + p.by_page(kx)), -1) : kNoPage;
+    }
     return e;
   };
   uint32_t found = 0;                // one bit a stage and half: whether its page is in the pool
@@ -205,7 +221,7 @@ __global__ void __launch_bounds__(kPagedWarps * 32, NT * D <= 256 ? 3 : 2) paged
       for (int x = 0; x < kHalves; ++x) {
         const int k0 = key_of(s) + x * kPageRows, number = e.n[x];
         const bool there = (unsigned)number < (unsigned)p.num_pages;
-        if (!there && k0 <= pos1 && lane == 0 && p.status) atomicExch(p.status, 1);
+        if (!there && number != kNoPage && lane == 0 && p.status) atomicExch(p.status, 1);
         const uint32_t bit = 1u << (stage * kHalves + x);
         found = there ? found | bit : found & ~bit;
         const uint32_t page = there ? (uint32_t)number : 0u, row = (uint32_t)(k0 - p.by_page(k0) * p.page_size);
@@ -589,9 +605,9 @@ struct PagedWriteParams {
 
 // q_out = rotate(q); rotate(k) and v go to their rows of the cache.  A thread owns eight adjacent dimensions of the first half of one
 // row and their partners in the second half.  Its two loads are on their way before the position and the page are looked up, one
-// load after the other.  Bound by memory: 17.4 us for 4096 prompt tokens with 32 + 2 x 8 heads (101 MB, 5.8 TB/s); a block per
-// token, whose threads share the look-up and go over several heads, was slower (19.4: fewer loads in flight), and so were divisions
-// in place of the multiplications (17.6).
+// load after the other.  Bound by memory: 14.8 us for 4096 prompt tokens with 32 + 2 x 8 heads replayed from a graph (101 MB, 6.8 TB/s, a
+// part of it in the L2 cache), 20.4 with other inputs each time.  A block per token, whose threads share the look-up and go over
+// several heads, was slower (19.4 in a graph: fewer loads in flight), and so were 64-bit divisions in place of the multiplications (17.6).
 template <typename T, int D>
 __global__ void __launch_bounds__(256) paged_rope_kernel(T* __restrict__ q_out, const T* __restrict__ q, const T* __restrict__ k,
                                                          const T* __restrict__ v, T* __restrict__ kp, T* __restrict__ vp,
@@ -674,6 +690,8 @@ PagedPlan paged_plan(const b200_paged_attn_t* a) {
   const long long slots = kSMs * (p.tiles * a->head_dim <= 256 ? 3 : 2);      // CTAs that are resident at once
   const long long most = std::max(1ll, keys / 64);            // a step for every warp of a share
   p.outer = 1;
+  // Few rows over a long length: sixteen CTAs a unit would leave SMs idle.  (One sequence of 65536 keys with one key head: 64 us with one
+  // cluster, 18 with 32 of eight; but 4000 keys with eight key heads 9 us with clusters of 16, 12 with three a unit, for the second kernel.)
   if (units * 16 < 2 * kSMs && keys > 16 * 1024) {
     const long long shares = std::max(1ll, std::min(slots / units, keys / 256));
     p.outer = (int)((shares + 7) / 8);
@@ -681,6 +699,8 @@ PagedPlan paged_plan(const b200_paged_attn_t* a) {
   } else {
     // clusters of more than eight leave about a quarter of the places empty (a cluster lies within one group of SMs)
     const long long one_wave = std::max(std::min(slots / units, 8ll), slots * 3 / 4 / units);
+    // one wave where it fits, else two CTAs a unit while that is less than four waves: shorter pieces even out different lengths (512 units of
+    // 100 to 4000 keys: 95 us whole, 88 halved, 98 in fours; 256 units with 20 rows: 86 / 77 / 80)
     p.split = (int)std::min({std::max(one_wave, units < 2 * slots ? 2ll : 1ll), most, 16ll});
   }
   return p;

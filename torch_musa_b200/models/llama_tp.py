@@ -32,7 +32,7 @@ class TPAttention(nn.Module):
         qkv = self.wqkv(x_shard).view(B, S, self.h_l + 2 * self.kv_l, hd)
         q, k, v = qkv.split([self.h_l, self.kv_l, self.kv_l], dim=2)
         q, k = BF.rope(q, cos, sin), BF.rope(k, cos, sin)
-        return self.wo(causal_attention(q, k, v, self.cfg).view(B * S, self.h_l * hd))
+        return self.wo(causal_attention(q, k, v, self.cfg).reshape(B * S, self.h_l * hd))
 
 
 class TPFeedForward(nn.Module):
