@@ -3,6 +3,7 @@
 replayed from a device graph.
 
   python benchmark/decode_bench.py [--batch 32] [--kv 2048] [--layers 32] [--tokens 32]
+  python benchmark/decode_bench.py --paged [--window 1024 --sinks 4] [--page 64]     (paged cache: PagedLlamaDecoder)
   python -m torch.distributed.run --nproc-per-node 8 --master-addr 127.0.0.1 benchmark/decode_bench.py   (tensor parallel:
       every rank holds 1/W of the heads and of the KV cache, two all-reduces per layer inside the captured step)
 
@@ -23,8 +24,33 @@ if ROOT not in sys.path:
 import torch  # noqa: E402
 
 import torch_musa_b200 as bw  # noqa: E402
-from torch_musa_b200.models import Llama, LlamaConfig  # noqa: E402
+from torch_musa_b200.models import Llama, LlamaConfig, PagedLlamaDecoder  # noqa: E402
 from torch_musa_b200.models.decode import LlamaDecoder, shard_for_tensor_parallel  # noqa: E402
+
+
+def paged(a, cfg, model, prompt):
+    """The same step over a paged cache, the step alone timed (the host's part, one token per sequence, included)."""
+    def timed(graph):
+        dec = PagedLlamaDecoder(model, a.batch, a.batch * -(-cfg.max_seq_len // a.page), a.page, device=prompt.device)
+        if graph:
+            dec.capture()
+        for row in prompt:
+            dec.add([row])
+        for _ in range(4):
+            dec.step()
+        bw.synchronize()
+        s, e = bw.Event(enable_timing=True), bw.Event(enable_timing=True)
+        s.record()
+        for _ in range(a.tokens):
+            dec.step()
+        e.record()
+        bw.synchronize()
+        return s.elapsed_time(e) / a.tokens
+
+    eager, graph = timed(False), timed(True)
+    print(json.dumps({"op": "paged_decode", "model": f"llama-7b dims, {a.layers} layers", "batch": a.batch, "kv_len": a.kv, "page": a.page,
+                      "window": a.window, "sinks": a.sinks, "eager_ms_per_token": round(eager, 3), "graph_ms_per_token": round(graph, 3),
+                      "graph_tokens_per_s": round(a.batch / graph * 1e3, 1), "speedup": round(eager / graph, 2)}))
 
 
 def main():
@@ -33,7 +59,12 @@ def main():
     ap.add_argument("--kv", type=int, default=2048)
     ap.add_argument("--layers", type=int, default=32)
     ap.add_argument("--tokens", type=int, default=32)
+    ap.add_argument("--paged", action="store_true")
+    ap.add_argument("--page", type=int, default=64)
+    ap.add_argument("--window", type=int, default=None)
+    ap.add_argument("--sinks", type=int, default=0)
     a = ap.parse_args()
+    assert a.paged or a.window is None, "a window needs the paged cache"
     world, rank = int(os.environ.get("WORLD_SIZE", "1")), int(os.environ.get("RANK", "0"))
     local = int(os.environ.get("LOCAL_RANK", "0"))
     dev = torch.device("blackwell", local)
@@ -44,8 +75,9 @@ def main():
         bw.set_device(local)
         dist.init_process_group("bccl", rank=rank, world_size=world)
         group = dist.group.WORLD
+    assert not (a.paged and world > 1), "the paged cache is not sharded"
     cfg = LlamaConfig(n_layers=a.layers, max_seq_len=a.kv + a.tokens * 3 + 8, fused_qkv=world == 1,
-                      fused_gate_up=world == 1)
+                      fused_gate_up=world == 1, window=a.window, attention_sinks=a.sinks)
     torch.manual_seed(0)
     with torch.device(dev):
         model = Llama(cfg).to(torch.bfloat16).eval()
@@ -58,6 +90,9 @@ def main():
         shard_for_tensor_parallel(model, rank, world)
     torch.manual_seed(1)
     prompt = torch.randint(0, cfg.vocab_size, (a.batch, a.kv)).to(dev)
+    if a.paged:
+        paged(a, cfg, model, prompt)
+        return
     dec = LlamaDecoder(model, a.batch, cfg.max_seq_len, device=dev, tp_group=group)
     dec.prefill(prompt)
 
