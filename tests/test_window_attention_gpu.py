@@ -120,6 +120,36 @@ def test_packed_sequences(bw, dev, dt, lens, klens, H, Hkv, window, sinks, extra
         assert bool((t[sum(n):] == 0).all())
 
 
+@pytest.mark.parametrize("bad", [0, 1])
+@pytest.mark.parametrize("packed", [False, True])
+def test_infinities_and_nan_stay_in_their_sequence(bw, dev, packed, bad):
+    """One of two sequences holds infinities and NaN near its ends; nothing of the other changes.  (dq is a sum of at most three blocks in
+    any order: its 32-bit values differ by 2^-22 of the sum of their sizes, which is below 2^-18 of the largest value here, and by a step
+    of the type when that moves a rounding.)"""
+    from torch_musa_b200.ops import flash_attn_varlen_func, window_attention
+
+    S, H, Hkv, dt = 200, 2, 1, torch.bfloat16
+    clean = inputs(dt, (2, S, H, D), (2, S, Hkv, D), 31)
+    dirty = [t.clone() for t in clean]
+    for t in dirty:
+        t[bad, S - 1], t[bad, S - 3], t[bad, 0] = math.inf, math.nan, -math.inf
+    cu = torch.tensor([0, S, 2 * S], dtype=torch.int32).to(dev)
+
+    def run(tensors):
+        q, k, v, do = (t.flatten(0, 1).to(dev) if packed else t.to(dev) for t in tensors)
+        for t in (q, k, v):
+            t.requires_grad_()
+        o = flash_attn_varlen_func(q, k, v, cu, cu, S, S, causal=True, window=50, sinks=3) if packed else window_attention(q, k, v, 50, 3)
+        return [t.detach().cpu().view(2, S, -1, D)[1 - bad].float() for t in (o, *torch.autograd.grad(o, (q, k, v), do))]
+
+    want, got = run(clean), run(dirty)
+    for name, a, b in zip(("o", "dq", "dk", "dv"), want, got):
+        if name == "dq":
+            assert bool(((a - b).abs() <= 2.0 ** -7 * a.abs() + 2.0 ** -18 * a.abs().max()).all())
+        else:
+            assert torch.equal(a, b), name
+
+
 def test_a_window_longer_than_the_sequence_is_the_causal_mask(bw, dev):
     """Bit for bit: the same blocks in the same order."""
     import torch.nn.functional as F

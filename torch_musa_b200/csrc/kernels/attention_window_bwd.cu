@@ -392,6 +392,12 @@ attn_window_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(dq_drained);
+        if (q0 + r >= u.Sq) {        // a row of the next sequence or head: zero, also where this one's keys are not finite
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int e = 0; e < 32; ++e) raw[c][e] = 0u;
+        }
         const int row0 = p.cu_q ? (int)((int64_t)h * p.total_q + u.qoff + q0) : (int)(((int64_t)u.b * p.H + h) * p.Sq + q0);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
