@@ -276,3 +276,21 @@ def test_paged_decoder_refusals():
     dec.remove(0)
     with pytest.raises(ValueError, match="not in use"):
         dec.remove(0)
+
+
+def test_paged_decoder_is_unchanged_by_a_call_that_fails():
+    model = Llama(llama_tiny_config(vocab_size=61)).eval()
+    dec = PagedLlamaDecoder(model, sequences=2, pages=6, page_size=16, max_len=48)
+    with pytest.raises(IndexError):
+        dec.add([torch.zeros(3, dtype=torch.long), torch.tensor([61])])      # no such token: the model fails
+    assert sorted(dec.free) == list(range(6)) and dec.lens == [None, None] and not dec.active.any()
+    dec.add([torch.zeros(3, dtype=torch.long)])
+    good = (torch.zeros(2, 2, dtype=torch.long), torch.zeros(2, 3), torch.zeros(2, 2, 61))
+    for which, bad in ((0, good[0][:1]), (0, good[0][0]), (1, good[1][:, :2]), (1, good[1].double()), (2, good[2][:, :1]), (2, good[2].bfloat16())):
+        args = list(good)
+        args[which] = bad
+        with pytest.raises(ValueError):
+            dec.check(*args)
+        assert dec.seq_lens.tolist() == [3, 0] and dec.lens == [3, None]
+    taken, _ = dec.check(*good)
+    assert dec.lens[0] == 4 + int(taken[0])

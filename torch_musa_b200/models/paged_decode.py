@@ -114,12 +114,18 @@ class PagedLlamaDecoder:
         for b in slots:
             self.lens[b] = 0
         try:
-            for b, n in zip(slots, sizes):
-                self._reserve([b], n)
-        except (RuntimeError, ValueError):
+            self._prefill(slots, prompts, sizes)
+        except Exception:
             for b in slots:
                 self.remove(b)
             raise
+        for b, n in zip(slots, sizes):
+            self.lens[b] = n
+        return slots
+
+    def _prefill(self, slots: List[int], prompts: Sequence[torch.Tensor], sizes: List[int]) -> None:
+        for b, n in zip(slots, sizes):
+            self._reserve([b], n)
         rows = torch.tensor(slots, device=self.device)
         table, lens = self.block_table[rows], torch.tensor(sizes, dtype=torch.int32, device=self.device)
         cu = torch.tensor([0] + sizes).cumsum(0).to(torch.int32).to(self.device)
@@ -135,9 +141,6 @@ class PagedLlamaDecoder:
         self.tokens[rows] = self.model.lm_head(last).argmax(-1, keepdim=True)
         self.seq_lens[rows] = lens
         self.active[rows] = 1
-        for b, n in zip(slots, sizes):
-            self.lens[b] = n
-        return slots
 
     def _new_tokens(self, tokens: torch.Tensor) -> torch.Tensor:
         """Hidden rows [B, n, dim] of n new tokens per slot; ``seq_lens`` counts them already."""
@@ -176,7 +179,12 @@ class PagedLlamaDecoder:
         ``tokens`` becomes the drawn ones.  Returns (taken [B], tokens [B, n + 1]); rows of slots not in use mean nothing."""
         if temperature <= 0:
             raise ValueError(f"temperature must be positive, got {temperature}")
-        n = drafts.shape[1]
+        n = drafts.shape[-1]
+        if (tuple(drafts.shape) != (self.B, n) or tuple(uniforms.shape) != (self.B, n + 1) or uniforms.dtype != torch.float32
+                or (draft_probs is not None and (tuple(draft_probs.shape) != (self.B, n, self.cfg.vocab_size)
+                                                 or draft_probs.dtype != torch.float32))):
+            raise ValueError("drafts [sequences, n], float32 uniforms [sequences, n + 1] and float32 draft_probs "
+                             "[sequences, n, vocabulary] expected")
         used = [b for b in range(self.B) if self.lens[b] is not None]
         self._reserve(used, n + 1)
         self.seq_lens.add_(self.active * (n + 1))
