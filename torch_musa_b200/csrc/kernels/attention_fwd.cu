@@ -63,12 +63,12 @@ struct AttnParams {
 // The MMA warp alternates between the tiles (P V and next S of tile 0, then of tile 1), so one tile's softmax runs while
 // the tensor core works for the other; K and V tiles stream through a five-slot TMA ring.
 //
-// kWin (sliding window of W keys and s sinks): 32 heads x 4096, window 1024: 88 us (680 TFLOP/s of what is visible, tensor
-// core 39 % busy); one prompt of 8192, window 4096: 352 us (1170; 56 %).  The blocks without a visible key are left out.  The list of blocks that the two
+// kWin (sliding window of W keys and s sinks): the blocks without a visible key are left out.  The list of blocks that the two
 // tiles share is, in this order: the blocks that only tile 0's window reaches (one, or none), the blocks of the sinks, the
 // rest of tile 1's window.  So tile 0 takes a prefix of the list and tile 1 a suffix, and every block is loaded once.  Packed
 // rows of the next sequence, or of nobody, are set to zero in the last block of V: their probability is zero, but zero times
-// what lies there need not be.
+// what lies there need not be.  Measured: 32 heads x 4096, window 1024: 88 us (680 TFLOP/s of what is visible, tensor core
+// 39 % busy; 96 us with a CTA per unit); one prompt of 8192, window 4096: 352 us (1170 TFLOP/s, 56 %).
 // One unit of work: a pair of query tiles of one (batch, head); heavy (late) tiles first, across all (batch, head) instances.
 struct FwdUnit {
   int qp, b, h, hk, Sq, Sk, qoff, koff, bt;
@@ -485,7 +485,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
           }
         }
         if (qi < u.Sq && p.lse)
-          p.lse[p.cu_q ? (int64_t)u.h * p.total_q + u.qoff + qi : ((int64_t)u.b * p.H + u.h) * p.Sq + qi] = l_run > 0.f ? (m_ref + log2f(l_run)) * 0.6931471805599453f : -INFINITY;
+          p.lse[p.cu_q ? (int64_t)u.h * p.total_q + u.qoff + qi : ((int64_t)u.b * p.H + u.h) * p.Sq + qi] =
+              l_run > 0.f ? (m_ref + log2f(l_run)) * 0.6931471805599453f : -INFINITY;
       }
       if constexpr (kWin) {
         Vec16<T> zero;

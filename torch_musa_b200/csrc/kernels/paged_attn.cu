@@ -67,7 +67,8 @@ __device__ __forceinline__ uint4 ldmatrix(uint32_t a) {
 }
 __device__ __forceinline__ uint4 ldmatrix_t(uint32_t a) {
   uint4 r;
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a) : "memory");
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a) : "memory");
   return r;
 }
 // from the shared memory of another CTA of the cluster
@@ -149,8 +150,8 @@ __device__ __forceinline__ bool not_finite(uint32_t w) {
 // kDense: the rows of a page follow one another (the layout of the pools as they are made), so that a copy's address is a constant
 // away from the page's.
 template <typename T, int D, int NT, bool kDense>
-__global__ void __launch_bounds__(kPagedWarps * 32, NT * D <= 256 ? 3 : 2) paged_attn_kernel(T* __restrict__ out, const T* __restrict__ q, const T* __restrict__ kp,
-                                                                         const T* __restrict__ vp, const PagedParams p) {
+__global__ void __launch_bounds__(kPagedWarps * 32, NT * D <= 256 ? 3 : 2)
+paged_attn_kernel(T* __restrict__ out, const T* __restrict__ q, const T* __restrict__ kp, const T* __restrict__ vp, const PagedParams p) {
   constexpr int kRows = 8 * NT, kHalves = D == 64 && NT <= 2 ? 2 : 1, kKeys = kHalves * kPageRows, kHalf = kPageRows * D * 2;
   constexpr int kStageBytes = 2 * kHalves * kHalf, kStages = kWarpRing / kStageBytes;
   constexpr int kPad = D + 4;            // floats of a row of a part: the four lanes' rows then lie in different banks
@@ -320,7 +321,8 @@ __global__ void __launch_bounds__(kPagedWarps * 32, NT * D <= 256 ? 3 : 2) paged
       if (unseen) {
 #pragma unroll
         for (int i = 0; i < kKeys / kPerCopy; ++i)
-          if ((unseen >> (i * kPerCopy + crow)) & 1u) zero16(ring + at + kHalves * kHalf + (uint32_t)(crow * D * 2 + cpiece * 16 + i * kPerCopy * D * 2));
+          if ((unseen >> (i * kPerCopy + crow)) & 1u)
+            zero16(ring + at + kHalves * kHalf + (uint32_t)(crow * D * 2 + cpiece * 16 + i * kPerCopy * D * 2));
         __syncwarp();
       }
 #pragma unroll

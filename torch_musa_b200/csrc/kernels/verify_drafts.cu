@@ -117,7 +117,8 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_drafts_kernel(int64_t* 
       double v;
       if (p.split > 1) {
         uint32_t a = (uint32_t)__cvta_generic_to_shared(&s_mine[c % kVerifyWarps]);
-        asm volatile("{\n\t.reg .u32 r;\n\tmapa.shared::cluster.u32 r, %1, %2;\n\tld.shared::cluster.f64 %0, [r];\n\t}" : "=d"(v) : "r"(a), "r"(c / kVerifyWarps) : "memory");
+        asm volatile("{\n\t.reg .u32 r;\n\tmapa.shared::cluster.u32 r, %1, %2;\n\tld.shared::cluster.f64 %0, [r];\n\t}"
+                     : "=d"(v) : "r"(a), "r"(c / kVerifyWarps) : "memory");
       } else {
         v = s_mine[c];
       }
