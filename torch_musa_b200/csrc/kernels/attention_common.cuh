@@ -106,6 +106,41 @@ __device__ __forceinline__ void mul2(float& d0, float& d1, float x0, float x1, f
 }
 // the n lowest bits, for any n
 __device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u); }
+// A warp's walk over the units of work of packed sequences, numbered sequence after sequence: only those that exist are dealt, however
+// the lengths differ.  A lane holds one of 32 sequences at a time.
+struct UnitWalk {
+  int base, before, mine, upto;        // first sequence in hand, units in front of it, this lane's, those of all up to this lane's
+  template <typename F>
+  __device__ __forceinline__ void take(int first, int units_before, int B, int lane, F count) {
+    base = first;
+    before = units_before;
+    mine = base + lane < B ? count(base + lane) : 0;
+    upto = mine;
+#pragma unroll
+    for (int w = 1; w < 32; w <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, upto, w);
+      if (lane >= w) upto += y;
+    }
+    upto += before;
+  }
+  // Sequence b and number `within` of unit x (never less than at the last call); false behind the last one: `before` counts them all.
+  template <typename F>
+  __device__ __forceinline__ bool find(int x, int B, int lane, int& b, int& within, F count) {
+    for (;;) {
+      const uint32_t past = __ballot_sync(0xffffffffu, upto > x);
+      if (past) {
+        const int at = __ffs(past) - 1;
+        b = base + at;
+        within = x - __shfl_sync(0xffffffffu, upto - mine, at);
+        return true;
+      }
+      const int all = __shfl_sync(0xffffffffu, upto, 31);
+      take(min(base + 32, B), all, B, lane, count);
+      if (base >= B) return false;
+    }
+  }
+};
+
 // two floats to one packed pair of 16-bit values (one conversion instruction)
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float a, float b);

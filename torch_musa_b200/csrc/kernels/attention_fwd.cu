@@ -16,8 +16,9 @@ using namespace attndev;
 constexpr int AQ = 128, AK = 128, AD = 128;          // query rows per tile, keys per block, head dim
 constexpr int kTile = 128 * 128 * 2;                  // 32 KB: any of Q, K, V
 constexpr int kRing = 5;                              // K / V tiles in flight
-constexpr int kAttnSmem = 2 * kTile /*Q0,Q1*/ + kRing * kTile + 1024 + 256;
-constexpr int kAttnThreads = 384;                     // 2 softmax warpgroups; one with the TMA warp and the MMA warp
+constexpr int kAttnSmem = 2 * kTile /*Q0,Q1*/ + kRing * kTile + 1024 + 512 /*barriers, units*/;
+constexpr int kAttnThreads = 384;                     // 2 softmax warpgroups; one with the TMA, the MMA and the unit warp
+constexpr int kUnitReaders = 10;                      // kWin: the TMA, MMA and softmax warps, which the unit warp tells what to do
 constexpr int kSoftmaxRegs = 216, kOtherRegs = 72;    // after the split: a row of scores stays in registers
 constexpr int kLaunchRegs = (2 * kSoftmaxRegs + kOtherRegs + 2) / 3;   // what the launch has to bring for that split
 constexpr uint32_t kAttnTmemCols = 512;               // S0, S1, O0, O1
@@ -69,7 +70,8 @@ struct AttnParams {
 // rows of the next sequence, or of nobody, are set to zero in the last block of V: their probability is zero, but zero times
 // what lies there need not be.  Measured: 32 heads x 4096, window 1024: 88 us (680 TFLOP/s of what is visible, tensor core
 // 39 % busy; 96 us with a CTA per unit); one prompt of 8192, window 4096: 352 us (1170 TFLOP/s, 56 %).
-// One unit of work: a pair of query tiles of one (batch, head); heavy (late) tiles first, across all (batch, head) instances.
+// One unit of work: a pair of query tiles of one (batch, head); heavy (late) tiles first, across all (batch, head) instances, or within each
+// sequence where they are packed and windowed.
 struct FwdUnit {
   int qp, b, h, hk, Sq, Sk, qoff, koff, bt;
   int nb0, nb1, nbmax;        // tile t ends before item nb<t> of the list of key blocks
@@ -94,17 +96,16 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
   uint64_t* mma_done = bars + 2 + 2 * kRing;   // [2]      tcgen05.commit: P V of block j - 1 and S of block j
   uint64_t* p_ready = mma_done + 2;            // [2][2]   four softmax warps: first / second part of P of block j is in TMEM
   uint64_t* q_empty = p_ready + 4;             // [2]      tcgen05.commit: the last S of a unit's tile (kWin)
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_empty + 2);
+  uint64_t* u_full = q_empty + 2;              // [2]      a unit's description is there (kWin)
+  uint64_t* u_empty = u_full + 2;              // [2]      all have read it
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(u_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  FwdUnit* s_unit = reinterpret_cast<FwdUnit*>(tmem_slot + 2);      // [2]
+  static_assert(24 * 8 + 8 + 2 * sizeof(FwdUnit) <= 512, "barriers and units share 512 bytes");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int n_bh = p.B * p.H;
-  auto make_unit = [&](int unit) {
-    FwdUnit u{};
-    u.qp = p.q_pairs - 1 - unit / n_bh;
-    const int bh = unit % n_bh;
-    u.b = bh / p.H;
-    u.h = bh - u.b * p.H;
+  auto complete = [&](FwdUnit& u) {      // from qp, b and h
     u.hk = u.h / (p.H / p.Hkv);
     // this instance's sequence: lengths, first packed rows and the batch coordinate of the tensor maps.  Rows past a
     // packed sequence's end belong to the next sequence: they are loaded, masked by index and never stored.
@@ -139,20 +140,35 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
       u.second_first = u.nb1 > 0 ? u.n_pre : 0;
     }
     u.nbmax = max(u.nb0, u.nb1);
+  };
+  auto make_unit = [&](int unit) {
+    FwdUnit u{};
+    u.qp = p.q_pairs - 1 - unit / n_bh;
+    const int bh = unit % n_bh;
+    u.b = bh / p.H;
+    u.h = bh - u.b * p.H;
+    complete(u);
     return u;
   };
   // Calls f() for every unit of this CTA until it returns false.  Without a window a CTA has one unit.  With one the units are short (ten
   // blocks at a window of 1024): a CTA then stays on its SM and takes every 148th unit, turning round at either end so that long and
-  // short ones even out; the loads and the first products of a unit run while the one before it is stored.
+  // short ones even out; the loads and the first products of a unit run while the one before it is stored.  A warp of its own finds the
+  // units, two ahead, and hands them over: each role for itself would pay for the search in time and in registers.
   const FwdUnit only = kWin ? FwdUnit{} : make_unit((int)blockIdx.x);
-  auto each_unit = [&](auto f) {
+  auto each_unit = [&](auto whole_warp, auto f) {
     if constexpr (!kWin) {
       f(only);
     } else {
-      for (int round = 0; round * (int)gridDim.x < p.units; ++round) {
-        const int unit = round * (int)gridDim.x + (round & 1 ? (int)(gridDim.x - 1 - blockIdx.x) : (int)blockIdx.x);
-        if (unit >= p.units) continue;
-        if (!f(make_unit(unit))) break;
+      for (uint32_t n = 0;; ++n) {
+        if constexpr (decltype(whole_warp)::value) {
+          if (!mbar_wait_warp(&u_full[n & 1], (n >> 1) & 1, abort_flag)) break;
+        } else {
+          if (!mbar_wait(&u_full[n & 1], (n >> 1) & 1, abort_flag)) break;
+        }
+        const FwdUnit u = s_unit[n & 1];
+        if constexpr (decltype(whole_warp)::value) __syncwarp();
+        if (!decltype(whole_warp)::value || lane == 0) mbar_arrive(&u_empty[n & 1]);
+        if (u.qp < 0 || !f(u)) break;
       }
     }
   };
@@ -167,6 +183,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
     for (int t = 0; t < 2; ++t) {
       mbar_init(&q_full[t], 1);
       mbar_init(&q_empty[t], 1);
+      mbar_init(&u_full[t], 1);
+      mbar_init(&u_empty[t], kUnitReaders);
       mbar_init(&mma_done[t], 1);
       mbar_init(&p_ready[2 * t], 4);
       mbar_init(&p_ready[2 * t + 1], 4);
@@ -184,6 +202,9 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
     tmem_alloc(tmem_slot, kAttnTmemCols);
     tmem_relinquish();
   }
+  auto tile_pairs = [&](int b) { return min(p.q_pairs, (max(0, p.cu_q[b + 1] - p.cu_q[b]) + 2 * AQ - 1) / (2 * AQ)); };
+  UnitWalk walk;
+  if (kWin && warp == 10 && p.cu_q) walk.take(0, 0, p.B, lane, tile_pairs);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -196,7 +217,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
       if (lane == 0) {
         int ring = 0;                    // items of the ring so far
         uint32_t loaded[2] = {0, 0};     // Q tiles so far, for the phases
-        each_unit([&](const FwdUnit& u) -> bool {
+        each_unit(std::false_type{}, [&](const FwdUnit& u) -> bool {
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
             if (u.nb(t) == 0) continue;
@@ -251,7 +272,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
       };
       int ring = 0;                      // items of the ring before this unit's
       uint32_t q_seen[2] = {0, 0}, p_seen[2] = {0, 0};     // Q tiles and blocks of P so far, for the phases
-      each_unit([&](const FwdUnit& u) -> bool {
+      each_unit(std::true_type{}, [&](const FwdUnit& u) -> bool {
         bool ok = true;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
@@ -324,6 +345,33 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
         return ok;
       });
       __syncwarp();
+    } else if (kWin && warp == 10) {
+      // ------------------------------------------------------------ the units, one after the other; qp < 0 behind the last
+      for (uint32_t n = 0;; ++n) {
+        const int unit = (int)(n * gridDim.x + (n & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x));
+        FwdUnit u{};
+        bool there;
+        if (p.cu_q) {
+          int behind;
+          there = walk.find(unit / p.H, p.B, lane, u.b, behind, tile_pairs);
+          if (there) {
+            u.h = unit % p.H;
+            u.qp = tile_pairs(u.b) - 1 - behind;
+            complete(u);
+          }
+        } else {
+          there = unit < p.units;
+          if (there) u = make_unit(unit);
+        }
+        if (!there) u.qp = -1;
+        if (!mbar_wait_warp(&u_empty[n & 1], ((n >> 1) & 1) ^ 1, abort_flag)) break;
+        if (lane == 0) {
+          s_unit[n & 1] = u;
+          mbar_arrive(&u_full[n & 1]);
+        }
+        __syncwarp();
+        if (!there) break;
+      }
     }
   } else {
     regs_inc<kSoftmaxRegs>();
@@ -340,7 +388,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
       return __all_sync(0xffffffffu, w);
     };
     uint32_t done = 0;                       // phases of mma_done[t] so far
-    each_unit([&](const FwdUnit& u) -> bool {
+    each_unit(std::true_type{}, [&](const FwdUnit& u) -> bool {
       const int qi = (2 * u.qp + t) * AQ + r;
       float m_ref = -INFINITY;                 // maximum the exponents refer to (raised lazily)
       float l_run = 0.f;

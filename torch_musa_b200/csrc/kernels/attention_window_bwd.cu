@@ -10,7 +10,7 @@
 //     that a small kernel adds up in order.
 //   * Units are short, and starting and ending a CTA cost as much as three or four pairs of blocks: a CTA stays on its SM and takes every
 //     148th unit, turning round at either end so that long and short ones even out.  The loads of a unit's queries, and the waits for its
-//     first products, run while the one before it is stored.  What a change of units still costs, about 5 us of 27 for nine pairs, is
+//     first products, run while the one before it is stored.  A warp of its own finds the units and hands them over.  What a change of units still costs, about 5 us of 27 for nine pairs, is
 //     the chain K -> S^T -> P -> dS that starts afresh: K and V of the next unit have no place before the last product of this one.
 //   * Hidden scores become -inf before the exponentials, two instructions an element, instead of tests inside the loops, whose second
 //     copy of the code cost more than they did (instructions came late).
@@ -71,8 +71,11 @@ __device__ __forceinline__ void zero_tail(uint8_t* tile, int rows, int lane) {
   __syncwarp();
 }
 
+constexpr int kUnitReaders = 15;         // every other warp of the kernel
+constexpr int kUnitBytes = 128;          // of their descriptions, beyond the common layout's: from the slack
+
 // One unit of work: a key block of one (batch, kv head), or a chunk of one.  All (batch, head) instances of the earliest key block come
-// first: under a causal mask it meets the most query blocks.
+// first (under a causal mask it meets the most query blocks); of packed sequences all that hold sinks.
 struct BwdUnit {
   int kb, chunk, bh, b, hk, k0, Sq, Sk, qoff, koff, bt;
   int i0, n_i, n_it, h0, istart;      // first query block, query blocks, pairs of query block and head, where the pairs start
@@ -86,7 +89,7 @@ attn_window_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                 const __grid_constant__ CUtensorMap tmap_dq, T* __restrict__ dk, T* __restrict__ dv, const WindowParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  if (smem - smem_raw > kBwdSlack) {        // cannot happen while the kernel has no static shared memory
+  if (smem - smem_raw > kBwdSlack - kUnitBytes) {        // cannot happen while the kernel has no static shared memory
     if (threadIdx.x == 0 && p.status) atomicExch(p.status, 1);
     return;
   }
@@ -114,25 +117,17 @@ attn_window_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
   uint64_t* ld_full = bars + 14;             // [2]  lse and delta of a query block are there
   uint64_t* ld_empty = bars + 16;            // [2]  8 warps
   uint64_t* acc_empty = bars + 18;           // 8 warps: dV and dK of the unit are in registers
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 19);
+  uint64_t* u_full = bars + 19;              // [2]  a unit's description is there
+  uint64_t* u_empty = bars + 21;             // [2]  all have read it
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 23);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  BwdUnit* s_unit = reinterpret_cast<BwdUnit*>(tmem_slot + 2);     // [2]
+  static_assert(23 * 8 + 8 + 2 * sizeof(BwdUnit) <= 256 + kUnitBytes, "barriers and units share this space");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int n_bh = p.B * p.Hkv, G = p.H / p.Hkv;
-  auto make_unit = [&](int unit) {
-    BwdUnit u{};
-    u.kb = unit / n_bh;
-    // counts (block with sinks, chunk) pairs first
-    const int pairs = p.sink_blocks * p.sink_chunks;
-    if (u.kb < pairs) {
-      u.chunk = u.kb % p.sink_chunks;
-      u.kb /= p.sink_chunks;
-    } else {
-      u.kb -= pairs - p.sink_blocks;
-    }
-    u.bh = unit % n_bh;
-    u.b = u.bh / p.Hkv;
-    u.hk = u.bh - u.b * p.Hkv;
+  auto complete = [&](BwdUnit& u) {        // from kb, chunk, b and hk
+    u.bh = u.b * p.Hkv + u.hk;
     u.k0 = u.kb * BK;
     // this instance's sequence (see the forward kernel): rows past a packed sequence's end are loaded, masked by index
     // (their probabilities and score gradients are exact zeros) and never stored
@@ -162,14 +157,19 @@ attn_window_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         u.istart = from % u.n_i;
       }
     }
-    return u;
   };
   // calls f() for every unit of this CTA until it returns false
-  auto each_unit = [&](auto f) {
-    for (int round = 0; round * (int)gridDim.x < p.units; ++round) {
-      const int unit = round * (int)gridDim.x + (round & 1 ? (int)(gridDim.x - 1 - blockIdx.x) : (int)blockIdx.x);
-      if (unit >= p.units) continue;
-      if (!f(make_unit(unit))) break;
+  auto each_unit = [&](auto whole_warp, auto f) {
+    for (uint32_t n = 0;; ++n) {
+      if constexpr (decltype(whole_warp)::value) {
+        if (!mbar_wait_warp(&u_full[n & 1], (n >> 1) & 1, abort_flag)) break;
+      } else {
+        if (!mbar_wait(&u_full[n & 1], (n >> 1) & 1, abort_flag)) break;
+      }
+      const BwdUnit u = s_unit[n & 1];
+      if constexpr (decltype(whole_warp)::value) __syncwarp();
+      if (!decltype(whole_warp)::value || lane == 0) mbar_arrive(&u_empty[n & 1]);
+      if (u.kb < 0 || !f(u)) break;
     }
   };
 
@@ -181,6 +181,8 @@ attn_window_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       mbar_init(&q_empty[i], 1);
       mbar_init(&ld_full[i], 1);
       mbar_init(&ld_empty[i], 8);
+      mbar_init(&u_full[i], 1);
+      mbar_init(&u_empty[i], kUnitReaders);
     }
     mbar_init(do_full, 1);
     mbar_init(do_empty, 1);
@@ -203,6 +205,11 @@ attn_window_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     tmem_alloc(tmem_slot, kBwdTmemCols);
     tmem_relinquish();
   }
+  auto key_blocks = [&](int b) { return min(p.kv_blocks, (max(0, p.cu_k[b + 1] - p.cu_k[b]) + BK - 1) / BK); };
+  auto sink_units = [&](int b) { return min(key_blocks(b), p.sink_blocks) * p.sink_chunks; };
+  auto other_units = [&](int b) { return max(0, key_blocks(b) - p.sink_blocks); };
+  UnitWalk walk;
+  if (warp == 15 && p.cu_q) walk.take(0, 0, p.B, lane, sink_units);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -222,7 +229,7 @@ attn_window_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
           tma_load_4d(sV, &tmap_v, kv_full, 0, u.koff + u.k0, u.hk, u.bt);
           tma_load_4d(sV + kTile / 2, &tmap_v, kv_full, 64, u.koff + u.k0, u.hk, u.bt);
         };
-        each_unit([&](const BwdUnit& u) -> bool {
+        each_unit(std::false_type{}, [&](const BwdUnit& u) -> bool {
           if (u.n_it == 0) return true;
           if (live == 0) load_kv(u);
           int h = u.h0, i = u.istart;
@@ -262,7 +269,7 @@ attn_window_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       auto koff16 = [](int kk) { return (uint32_t)(((kk >> 2) * (kTile / 2) + (kk & 3) * 32) >> 4); };   // K-major: two 64-column atoms
       auto mnoff16 = [](int kk) { return (uint32_t)((kk * 2048) >> 4); };                                // MN-major: 16 rows of 128 bytes
       int base = 0, live = 0;              // pairs before this unit's, units with pairs so far
-      each_unit([&](const BwdUnit& u) -> bool {
+      each_unit(std::true_type{}, [&](const BwdUnit& u) -> bool {
         if (u.n_it == 0) return true;
         bool ok = wait(kv_full, live) && wait(&q_full[base & 1], base >> 1);
         // the rows of the current and the next query block that are the sequence's own (128 or more: all)
@@ -352,7 +359,7 @@ attn_window_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
           d[e] = qi < u.Sq ? __ldg(p.delta + base + qi) : 0.f;
         }
       };
-      each_unit([&](const BwdUnit& u) -> bool {
+      each_unit(std::true_type{}, [&](const BwdUnit& u) -> bool {
         h = u.h0;
         i = u.istart;
         if (u.n_it > 0) fetch(u);
@@ -371,6 +378,47 @@ attn_window_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         }
         return true;
       });
+    } else {
+      // ------------------------------------------------------------ the units, one after the other; kb < 0 behind the last
+      bool in_sinks = true;
+      int with_sinks = 0;
+      for (uint32_t n = 0;; ++n) {
+        const int unit = (int)(n * gridDim.x + (n & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x));
+        BwdUnit u{};
+        bool there;
+        if (p.cu_q) {
+          const int x = unit / p.Hkv;
+          if (in_sinks && !walk.find(x, p.B, lane, u.b, u.kb, sink_units)) {
+            in_sinks = false;
+            with_sinks = walk.before;
+            walk.take(0, 0, p.B, lane, other_units);
+          }
+          there = in_sinks || walk.find(x - with_sinks, p.B, lane, u.b, u.kb, other_units);
+          u.hk = unit % p.Hkv;
+          if (!in_sinks) u.kb += p.sink_blocks;
+        } else {
+          const int pairs = p.sink_blocks * p.sink_chunks, bh = unit % n_bh;
+          there = unit < p.units;
+          u.kb = unit / n_bh;
+          u.b = bh / p.Hkv;
+          u.hk = bh - u.b * p.Hkv;
+          in_sinks = u.kb < pairs;
+          if (!in_sinks) u.kb -= pairs - p.sink_blocks;
+        }
+        if (in_sinks) {                       // numbers of (block, chunk) pairs
+          u.chunk = u.kb % p.sink_chunks;
+          u.kb /= p.sink_chunks;
+        }
+        if (there) complete(u);
+        else u.kb = -1;
+        if (!mbar_wait_warp(&u_empty[n & 1], ((n >> 1) & 1) ^ 1, abort_flag)) break;
+        if (lane == 0) {
+          s_unit[n & 1] = u;
+          mbar_arrive(&u_full[n & 1]);
+        }
+        __syncwarp();
+        if (!there) break;
+      }
     }
   } else if (warp >= 8) {
     regs_inc<kDqRegs>();
@@ -379,11 +427,17 @@ attn_window_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     const int r = qw * 32 + lane;                 // query row inside the block = TMEM lane
     const uint32_t addr = tmem_base + ((uint32_t)(qw * 32) << 16) + kColDP;
     int gi = 0;
-    each_unit([&](const BwdUnit& u) -> bool {
+    bool ok = true;
+    for (uint32_t n = 0; ok; ++n) {        // the description stays in shared memory, as in the compute warps
+      ok = mbar_wait_warp(&u_full[n & 1], (n >> 1) & 1, abort_flag);
+      if (!named_bar_and(1, 128, ok)) break;                          // one answer for the four warps, here and below
+      const volatile BwdUnit& u = s_unit[n & 1];
+      if (u.kb < 0) break;
+      const int n_it = u.n_it;
       int h = u.h0, i = u.istart;
-      for (int it = 0; it < u.n_it; ++it, ++gi) {
+      for (int it = 0; it < n_it && ok; ++it, ++gi) {
         const int q0 = (u.i0 + i) * BQ;
-        bool ok = mbar_wait_warp(dq_full, (uint32_t)(gi & 1), abort_flag);
+        ok = mbar_wait_warp(dq_full, (uint32_t)(gi & 1), abort_flag);
         tc_fence_after();
         uint32_t raw[4][32];
 #pragma unroll
@@ -403,7 +457,7 @@ attn_window_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         for (int c = 0; c < 4; ++c) {
           // the reduction that read this box two chunks ago has finished with it
           if (threadIdx.x == 8 * 32) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-          if (!named_bar_and(1, 128, ok)) { ok = false; break; }     // one answer for the four warps
+          if (!named_bar_and(1, 128, ok)) { ok = false; break; }
           uint8_t* box = sStage + (c & 1) * kStage + (size_t)r * 128;
 #pragma unroll
           for (int ch = 0; ch < 8; ++ch)
@@ -416,11 +470,11 @@ attn_window_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
           }
         }
-        if (!ok) return false;
         if (++i == u.n_i) { i = 0; ++h; }
       }
-      return true;
-    });
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&u_empty[n & 1]);
+    }
     // every reduction must have completed before the CTA exits
     if (threadIdx.x == 8 * 32) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   } else {
@@ -435,20 +489,25 @@ attn_window_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     uint8_t* srow = sS + (size_t)wg * (kTile / 2) + (size_t)r * 128;   // this warpgroup's 64 query columns = atom `wg`
     auto wait_all = [&](uint64_t* bar, uint32_t parity) { return mbar_wait_warp(bar, parity, abort_flag); };
     int gi = 0, live = 0;
-    each_unit([&](const BwdUnit& u) -> bool {
-      const int kj = u.k0 + r;
-      const bool key_off = kj >= u.Sk;
-      const bool block_off = u.k0 + BK > u.Sk;
+    // The description stays in shared memory until the unit is stored: what the loop does not need would take registers from it.
+    for (uint32_t n = 0;; ++n) {
+      if (!wait_all(&u_full[n & 1], (n >> 1) & 1)) break;
+      const volatile BwdUnit& u = s_unit[n & 1];
+      const int n_it = u.n_it, i0 = u.i0, n_i = u.n_i, k0 = u.k0, Sk = u.Sk;
+      if (u.kb < 0) break;
+      const int kj = k0 + r;
+      const bool key_off = kj >= Sk;
+      const bool block_off = k0 + BK > Sk;
       const int far = kj >= p.sinks ? kj + p.window : 0x7fffffff;      // the first query that no longer sees this key
       bool ok = true;
       int i = u.istart;
-      for (int it = 0; it < u.n_it; ++it, ++gi) {
+      for (int it = 0; it < n_it; ++it, ++gi) {
         const uint32_t par = (uint32_t)(gi & 1);
-        const int st = gi & 1, q0 = (u.i0 + i) * BQ;
+        const int st = gi & 1, q0 = (i0 + i) * BQ;
         const float4* nlse4 = reinterpret_cast<const float4*>(s_lse + st * 128 + wg * 64);
         const float4* ndlt4 = reinterpret_cast<const float4*>(s_dlt + st * 128 + wg * 64);
         // only then can a query be older than a key of this block, a key be past the end or in front of a window
-        const bool masked = q0 < u.k0 + BK || block_off || q0 + BQ - u.k0 > p.window;
+        const bool masked = q0 < k0 + BK || block_off || q0 + BQ - k0 > p.window;
         if (!wait_all(&ld_full[st], (uint32_t)((gi >> 1) & 1)) || !wait_all(s_full, par)) { ok = false; break; }
         tc_fence_after();
         float pf[64];
@@ -520,13 +579,13 @@ attn_window_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
           mbar_arrive(ds_ready);
           mbar_arrive(&ld_empty[st]);
         }
-        if (++i == u.n_i) i = 0;
+        if (++i == n_i) i = 0;
       }
-      if (ok && u.n_it > 0) ok = wait_all(all_done, (uint32_t)(live & 1));
+      if (ok && n_it > 0) ok = wait_all(all_done, (uint32_t)(live & 1));
       // ---- dK, dV of this key block
       if (ok) {
         tc_fence_after();
-        const bool row_ok = kj < u.Sk;
+        const bool row_ok = kj < Sk;
         T* dk_row = dk + (int64_t)u.bt * p.dk_sb + (int64_t)u.hk * p.dk_sh + (int64_t)(u.koff + kj) * p.dk_ss + wg * 64;
         T* dv_row = dv + (int64_t)u.bt * p.dv_sb + (int64_t)u.hk * p.dv_sh + (int64_t)(u.koff + kj) * p.dv_ss + wg * 64;
 #pragma unroll
@@ -534,7 +593,7 @@ attn_window_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             uint32_t raw[32];
-            if (u.n_it > 0) {
+            if (n_it > 0) {
               tmem_ld32(tmem_base + lane_base + (which ? kColDK : kColDV) + (uint32_t)(wg * 64 + c * 32), raw);
               tmem_ld_wait();
             } else {
@@ -544,7 +603,7 @@ attn_window_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
             if (u.partial) {
               float* dst = p.sink_ws + ((((int64_t)u.bh * p.sink_blocks + u.kb) * p.sink_chunks + u.chunk) * 2 + which) * (BK * BD) + r * BD +
                            wg * 64 + c * 32;
-              if (u.n_it > 0) {
+              if (n_it > 0) {
 #pragma unroll
                 for (int g4 = 0; g4 < 8; ++g4)
                   *reinterpret_cast<uint4*>(dst + g4 * 4) = make_uint4(raw[g4 * 4], raw[g4 * 4 + 1], raw[g4 * 4 + 2], raw[g4 * 4 + 3]);
@@ -562,24 +621,26 @@ attn_window_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
           }
         }
       }
-      if (u.n_it > 0) {
+      if (n_it > 0) {
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(acc_empty);
         ++live;
       }
-      if (p.cu_q && u.b == p.B - 1 && u.chunk == 0) {       // packed rows past the last sequence: the CTAs of a head share them
-        Vec16<T> zero;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&u_empty[n & 1]);
+      if (!ok) break;
+    }
+    if (p.cu_q) {                                    // packed rows past the last sequence: zeros, the CTAs share them
+      Vec16<T> zero;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) zero.v[e] = ToF<T>::from(0.f);
-        for (int x = u.kb * 16 + (threadIdx.x >> 4); x < p.total_k - (u.koff + u.Sk); x += p.kv_blocks * 16) {
-          const int64_t row = u.koff + u.Sk + x;
-          st16(dk + (int64_t)u.hk * p.dk_sh + row * p.dk_ss + (threadIdx.x & 15) * 8, zero);
-          st16(dv + (int64_t)u.hk * p.dv_sh + row * p.dv_ss + (threadIdx.x & 15) * 8, zero);
+      for (int e = 0; e < 8; ++e) zero.v[e] = ToF<T>::from(0.f);
+      for (int64_t row = p.cu_k[p.B] + (int)blockIdx.x * 16 + (threadIdx.x >> 4); row < p.total_k; row += gridDim.x * 16)
+        for (int y = 0; y < p.Hkv; ++y) {
+          st16(dk + (int64_t)y * p.dk_sh + row * p.dk_ss + (threadIdx.x & 15) * 8, zero);
+          st16(dv + (int64_t)y * p.dv_sh + row * p.dv_ss + (threadIdx.x & 15) * 8, zero);
         }
-      }
-      return ok;
-    });
+    }
   }
 
   tc_fence_before();
