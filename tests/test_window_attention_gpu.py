@@ -307,6 +307,21 @@ def test_refusals(bw, dev):
         assert [g.shape for g in torch.autograd.grad(o, e, torch.zeros_like(o))] == [t.shape for t in e]
 
 
+@pytest.mark.parametrize("lens,window,sinks", [([1], 7, 0), ([1, 1, 1], 300, 4), ([300], 1, 0), ([129, 1, 40], 1, 0)])
+def test_a_query_with_one_key_has_no_gradient_through_its_score(bw, dev, lens, window, sinks):
+    """The softmax over one key is constant, so the gradients of q and k are zero, exactly."""
+    from torch_musa_b200.ops import flash_attn_varlen_func
+
+    q, k, v, do = (t.to(dev) for t in inputs(torch.bfloat16, (sum(lens), 4, D), (sum(lens), 2, D), 5))
+    for t in (q, k, v):
+        t.requires_grad_()
+    cu = torch.tensor([0] + lens).cumsum(0).to(torch.int32).to(dev)
+    o = flash_attn_varlen_func(q, k, v, cu, cu, max(lens), max(lens), causal=True, window=window, sinks=sinks)
+    dq, dk, dv = torch.autograd.grad(o, (q, k, v), do)
+    assert not dq.any() and not dk.any() and torch.equal(o, v.repeat_interleave(2, 1))
+    assert torch.allclose(dv.float(), do.float().view(-1, 2, 2, D).sum(2), rtol=2.0 ** -8, atol=2.0 ** -8)
+
+
 def test_other_types_and_head_sizes_take_the_plain_way(bw, dev):
     from torch_musa_b200.ops import flash_attn_varlen_func, window_attention
 

@@ -14,6 +14,9 @@
 //     the chain K -> S^T -> P -> dS that starts afresh: K and V of the next unit have no place before the last product of this one.
 //   * Hidden scores become -inf before the exponentials, two instructions an element, instead of tests inside the loops, whose second
 //     copy of the code cost more than they did (instructions came late).
+//   * The row sums of dO O come from O as it was stored, rounded to 16 bits, as in the causal backward.  Where a query sees hundreds of keys
+//     that adds nothing beside the rounding of dS (gradients of q and k are off by 2.4e-3 of their norm in bf16, 1.7e-3 of it by their own
+//     rounding); with two keys it shows (3.7e-3).  The remainder of O, kept by the forward, would mend that for 2 x 256 bytes a row, 2 % of the time.
 //   * Packed rows that are not the sequence's own are zeros in shared memory before a product reads them: their probabilities are zero,
 //     but zero times what lies there need not be.
 // Measured (whole calls: row dots, this kernel, sums of the chunks, conversion of dQ): 32 heads x 4096, window 1024, four sinks 273 us (289
@@ -34,7 +37,7 @@ using namespace attndev;
 
 struct WindowParams {
   int B, H, Hkv, Sq, Sk;
-  float scale, scale_log2;
+  float scale, scale_log2;      // of dS; of the exponents, times log2(e)
   const float* lse;       // [B, H, Sq] natural log
   const float* delta;     // [B, H, Sq]
   float* dq;              // [B, H, Sq, 128] fp32
@@ -540,6 +543,7 @@ attn_window_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
           }
           tmem_st16(s_addr + (uint32_t)(c * 16), pk);   // over columns of S^T that this thread has read
         }
+        if (q0 == 0 && wg == 0) pf[0] = 0.f;      // the first query sees one key: its softmax is constant, and so dS is zero, not nearly zero
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
@@ -713,7 +717,7 @@ int attn_window_bwd(const b200_attn_t* a, float* dq_accum, void* dk, void* dv, f
   const int64_t* x = extra_strides;
   WindowParams p{};
   p.B = a->B; p.H = a->H; p.Hkv = a->Hkv; p.Sq = a->Sq; p.Sk = a->Sk;
-  p.scale = a->scale;
+  p.scale = a->window == 1 && a->sinks == 0 ? 0.f : a->scale;      // every query sees one key: dS is zero
   p.scale_log2 = a->scale * 1.4426950408889634f;
   p.lse = lse;
   p.delta = delta;
