@@ -120,6 +120,16 @@ def test_packed_sequences(bw, dev, dt, lens, klens, H, Hkv, window, sinks, extra
         assert bool((t[sum(n):] == 0).all())
 
 
+@pytest.mark.parametrize("sinks", [0, 5])
+@pytest.mark.parametrize("empty", ["front", "back", "spread"])
+def test_many_packed_sequences(bw, dev, empty, sinks):
+    """More sequences than a warp has lanes, dozens of them empty: where the units of work are counted."""
+    g = torch.Generator().manual_seed(1)
+    some = torch.randint(1, 40, (40,), generator=g).tolist() + [300]
+    lens = {"front": [0] * 70 + some, "back": some + [0] * 70, "spread": [n for x in some for n in (0, x, 0)]}[empty]
+    test_packed_sequences(bw, dev, torch.float16, lens, None, 2, 1, 30, sinks, 9)
+
+
 @pytest.mark.parametrize("bad", [0, 1])
 @pytest.mark.parametrize("packed", [False, True])
 def test_infinities_and_nan_stay_in_their_sequence(bw, dev, packed, bad):
