@@ -317,6 +317,37 @@ def test_refusals(bw, dev):
         assert [g.shape for g in torch.autograd.grad(o, e, torch.zeros_like(o))] == [t.shape for t in e]
 
 
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+def test_remainder_of_the_output(bw, dev, dt):
+    """Equal scores: every probability is one before the division, so only the output itself is rounded, and output + remainder is off by
+    the rounding of the remainder (u of it, u^2 of the output, 2^-25 below fp16's normal range) and by four 32-bit roundings."""
+    S, H, Hkv = 200, 4, 2
+    _, k, v, do = inputs(dt, (1, S, H, D), (1, S, Hkv, D), 6)
+    q = torch.zeros(1, S, H, D, dtype=dt)
+    p = visible(S, S, 3, 1).double()
+    vv = v[0].double().repeat_interleave(H // Hkv, 1)
+    want = torch.einsum("ij,jhd->ihd", p / p.sum(1, keepdim=True), vv)
+    bound = (torch.finfo(dt).eps / 2) ** 2 * want.abs() + 2.0 ** -22 * torch.einsum("ij,jhd->ihd", p, vv.abs()) + 2.0 ** -25
+    op, on = torch.ops.blackwell, [t.to(dev) for t in (q, k, v, do)]
+    out, lse, rest = op.window_attention_with_remainder(*on[:3], 3, 1)
+    assert bool(((out.cpu().double() + rest.cpu().double())[0] - want).abs().le(bound).all()) and bool(rest.any())
+    plain = op.window_attention(*on[:3], 3, 1)
+    assert torch.equal(plain[0], out) and torch.equal(plain[1], lse)
+    cu = torch.tensor([0, S], dtype=torch.int32).to(dev)
+    more = [torch.cat((t[0], torch.full_like(t[0, :7], float("nan")))) for t in on[:3]]
+    o2, l2, r2 = op.varlen_attention_with_remainder(*more, cu, cu, S, S, 3, 1)
+    assert torch.equal(o2[:S], out[0]) and torch.equal(r2[:S], rest[0]) and not o2[S:].any() and not r2[S:].any()
+    grads = op.window_attention_backward(on[3], *on[:3], out, lse, 3, 1, None, rest)
+    apart = op.window_attention_backward(on[3], *on[:3], out, lse, 3, 1, None, rest.transpose(1, 2).contiguous().transpose(1, 2))
+    for a, b in zip(grads[1:], apart[1:]):      # another layout of the remainder; dq depends on the order of arrival
+        assert torch.equal(a, b)
+    with pytest.raises(RuntimeError, match="remainder"):
+        op.window_attention_backward(on[3], *on[:3], out, lse, 3, 1, None, rest[:, :100])
+    for empty in ((0, S), (1, 0)):
+        e = torch.empty(*empty, H, D, dtype=dt, device=dev)
+        assert op.window_attention_with_remainder(e, e, e, 3, 1)[2].shape == e.shape
+
+
 @pytest.mark.parametrize("lens,window,sinks", [([1], 7, 0), ([1, 1, 1], 300, 4), ([300], 1, 0), ([129, 1, 40], 1, 0)])
 def test_a_query_with_one_key_has_no_gradient_through_its_score(bw, dev, lens, window, sinks):
     """The softmax over one key is constant, so the gradients of q and k are zero, exactly."""

@@ -282,41 +282,72 @@ at::Tensor bwd_workspace(b200_attn_t& a, const at::Tensor& q) {
   return ws;
 }
 
-std::tuple<at::Tensor, at::Tensor> varlen_attention(const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_,
-                                                    const at::Tensor& cu_q, const at::Tensor& cu_k, int64_t max_q,
-                                                    int64_t max_k, bool causal, std::optional<double> scale,
-                                                    std::optional<int64_t> window, int64_t sinks) {
+// What the backward under a window asks for beside the output: o + remainder is the output before it was rounded, or nearly (16 bits more).
+using WithRemainder = std::tuple<at::Tensor, at::Tensor, at::Tensor>;
+std::tuple<at::Tensor, at::Tensor> without(const WithRemainder& r) { return {std::get<0>(r), std::get<1>(r)}; }
+// o and what rounding left of it as the backward kernels take them: one layout for both.
+std::pair<at::Tensor, at::Tensor> output_pair(const char* op, const at::Tensor& out, const std::optional<at::Tensor>& remainder, const at::Tensor& q) {
+  TORCH_CHECK(out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type(), op, ": out must be like q");
+  if (!remainder.has_value() || !remainder->defined()) return {out, {}};
+  check_devices(op, q, *remainder);
+  TORCH_CHECK(remainder->sizes() == q.sizes() && remainder->scalar_type() == q.scalar_type(), op, ": remainder must be like q");
+  if (out.strides() == remainder->strides()) return {out, *remainder};
+  return {out.contiguous(), remainder->contiguous()};
+}
+
+WithRemainder varlen_forward(const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_, const at::Tensor& cu_q, const at::Tensor& cu_k,
+                             int64_t max_q, int64_t max_k, bool causal, std::optional<double> scale, std::optional<int64_t> window,
+                             int64_t sinks, bool with_remainder) {
   check_devices("varlen_attention", q_, k_, v_, cu_q, cu_k);
   if (q_.dim() == 3 && empty_window(q_, k_, window))
-    return {at::zeros(q_.sizes(), q_.options()), at::full({q_.size(1), q_.size(0)}, -INFINITY, q_.options().dtype(at::kFloat))};
+    return {at::zeros(q_.sizes(), q_.options()), at::full({q_.size(1), q_.size(0)}, -INFINITY, q_.options().dtype(at::kFloat)),
+            at::zeros(q_.sizes(), q_.options())};
   at::Tensor q = q_.stride(2) == 1 ? q_ : q_.contiguous(), k = k_.stride(2) == 1 ? k_ : k_.contiguous(),
              v = v_.stride(2) == 1 ? v_ : v_.contiguous();
   b200_attn_t a{};
   varlen_desc(a, q, k, v, cu_q, cu_k, max_q, max_k, causal, scale, window, sinks);
   at::Tensor o = at::empty({q.size(0), q.size(1), 128}, q.options());
-  at::Tensor lse = at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat));
+  at::Tensor lse = at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat)), rest;
   a.o_ss = o.stride(0); a.o_sh = o.stride(1);
+  if (with_remainder) {
+    rest = at::empty(o.sizes(), o.options());
+    a.remainder = rest.mutable_data_ptr();
+  }
   DeviceSwitch sw(q.device().index());
   int e = b200_flash_attn_fwd(&a, o.mutable_data_ptr(), lse.data_ptr<float>(), q.const_data_ptr(), k.const_data_ptr(),
                               v.const_data_ptr(), current_raw_stream(q));
   TORCH_CHECK(e != (int)cudaErrorNotSupported, "varlen_attention: unsupported strides or alignment");
   B200_KERNEL_CALL(e);
   g_native_fwd_calls.fetch_add(1, std::memory_order_relaxed);
-  return {o, lse};
+  return {o, lse, rest};
+}
+
+std::tuple<at::Tensor, at::Tensor> varlen_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& cu_q,
+                                                    const at::Tensor& cu_k, int64_t max_q, int64_t max_k, bool causal,
+                                                    std::optional<double> scale, std::optional<int64_t> window, int64_t sinks) {
+  return without(varlen_forward(q, k, v, cu_q, cu_k, max_q, max_k, causal, scale, window, sinks, false));
+}
+
+WithRemainder varlen_attention_with_remainder(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& cu_q,
+                                              const at::Tensor& cu_k, int64_t max_q, int64_t max_k, int64_t window, int64_t sinks,
+                                              std::optional<double> scale) {
+  return varlen_forward(q, k, v, cu_q, cu_k, max_q, max_k, true, scale, window, sinks, true);
 }
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor> varlen_attention_backward(
     const at::Tensor& grad_out, const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_, const at::Tensor& out,
     const at::Tensor& lse, const at::Tensor& cu_q, const at::Tensor& cu_k, int64_t max_q, int64_t max_k, bool causal,
-    std::optional<double> scale, std::optional<int64_t> window, int64_t sinks) {
+    std::optional<double> scale, std::optional<int64_t> window, int64_t sinks, const std::optional<at::Tensor>& remainder) {
   if (q_.dim() == 3 && empty_window(q_, k_, window))
     return {at::zeros(q_.sizes(), q_.options()), at::zeros(k_.sizes(), k_.options()), at::zeros(v_.sizes(), v_.options())};
   check_devices("varlen_attention_backward", grad_out, q_, k_, v_, out, lse, cu_q, cu_k);
   at::Tensor q = q_.contiguous(), k = k_.contiguous(), v = v_.contiguous(), go = grad_out.contiguous(), o = out.contiguous(),
-             l = lse.contiguous();
+             l = lse.contiguous(), rest;
   b200_attn_t a{};
   varlen_desc(a, q, k, v, cu_q, cu_k, max_q, max_k, causal, scale, window, sinks);
   if (window.has_value()) at::globalContext().alertNotDeterministic("varlen_attention_backward with a window");
+  if (window.has_value()) std::tie(o, rest) = output_pair("varlen_attention_backward", o, remainder, q);
+  if (rest.defined()) a.remainder = rest.mutable_data_ptr();
   TORCH_CHECK(l.scalar_type() == at::kFloat && l.numel() == q.size(0) * q.size(1), "varlen_attention_backward: lse must be [H, total_q]");
   a.o_ss = o.stride(0); a.o_sh = o.stride(1);
   at::Tensor dq32 = at::empty({q.size(1), q.size(0), 128}, q.options().dtype(at::kFloat));
@@ -372,32 +403,48 @@ void check_window_operands(const char* op, const at::Tensor& q, const at::Tensor
     TORCH_CHECK(t->size(0) <= INT_MAX && t->size(1) <= (1 << 30) && t->size(2) <= INT_MAX, op, ": a size of ", t->sizes(), " is not supported");
 }
 
-std::tuple<at::Tensor, at::Tensor> window_attention(const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_, int64_t window,
-                                                    int64_t sinks, std::optional<double> scale) {
+WithRemainder window_forward(const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_, int64_t window, int64_t sinks,
+                             std::optional<double> scale, bool with_remainder) {
   const char* op = "window_attention";
   check_window_operands(op, q_, k_, v_);
   check_devices(op, q_, k_, v_);
   b200_attn_t a{};
   window_desc(a, op, true, window, sinks);
   if (q_.numel() == 0 || k_.numel() == 0)
-    return {at::zeros(q_.sizes(), q_.options()), at::full({q_.size(0), q_.size(2), q_.size(1)}, -INFINITY, q_.options().dtype(at::kFloat))};
+    return {at::zeros(q_.sizes(), q_.options()), at::full({q_.size(0), q_.size(2), q_.size(1)}, -INFINITY, q_.options().dtype(at::kFloat)),
+            at::zeros(q_.sizes(), q_.options())};
   const at::Tensor q = attn_operand(q_), k = attn_operand(k_), v = attn_operand(v_);
   at::Tensor o = at::empty(q.sizes(), q.options());
-  at::Tensor lse = at::empty({q.size(0), q.size(2), q.size(1)}, q.options().dtype(at::kFloat));
+  at::Tensor lse = at::empty({q.size(0), q.size(2), q.size(1)}, q.options().dtype(at::kFloat)), rest;
   dense_window_desc(a, op, q, k, v, window, sinks, scale);
   a.o_sb = o.stride(0); a.o_sh = o.stride(2); a.o_ss = o.stride(1);
+  if (with_remainder) {
+    rest = at::empty(o.sizes(), o.options());
+    a.remainder = rest.mutable_data_ptr();
+  }
   DeviceSwitch sw(q.device().index());
   const int e = b200_flash_attn_fwd(&a, o.mutable_data_ptr(), lse.data_ptr<float>(), q.const_data_ptr(), k.const_data_ptr(),
                                     v.const_data_ptr(), current_raw_stream(q));
   TORCH_CHECK(e != (int)cudaErrorNotSupported, op, ": unsupported sizes or strides");
   B200_KERNEL_CALL(e);
   g_native_fwd_calls.fetch_add(1, std::memory_order_relaxed);
-  return {o, lse};
+  return {o, lse, rest};
+}
+
+std::tuple<at::Tensor, at::Tensor> window_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, int64_t window, int64_t sinks,
+                                                    std::optional<double> scale) {
+  return without(window_forward(q, k, v, window, sinks, scale, false));
+}
+
+WithRemainder window_attention_with_remainder(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, int64_t window, int64_t sinks,
+                                              std::optional<double> scale) {
+  return window_forward(q, k, v, window, sinks, scale, true);
 }
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor> window_attention_backward(const at::Tensor& grad_out, const at::Tensor& q_, const at::Tensor& k_,
                                                                          const at::Tensor& v_, const at::Tensor& out, const at::Tensor& lse,
-                                                                         int64_t window, int64_t sinks, std::optional<double> scale) {
+                                                                         int64_t window, int64_t sinks, std::optional<double> scale,
+                                                                         const std::optional<at::Tensor>& remainder) {
   const char* op = "window_attention_backward";
   check_window_operands(op, q_, k_, v_);
   check_devices(op, q_, k_, v_, grad_out, out, lse);
@@ -407,12 +454,14 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> window_attention_backward(const a
               op, ": grad_out and out must be like q, lse float32 [B, H, Sq]");
   if (q_.numel() == 0 || k_.numel() == 0)
     return {at::zeros(q_.sizes(), q_.options()), at::zeros(k_.sizes(), k_.options()), at::zeros(v_.sizes(), v_.options())};
-  const at::Tensor q = attn_operand(q_), k = attn_operand(k_), v = attn_operand(v_), go = attn_operand(grad_out), o = attn_operand(out);
+  const at::Tensor q = attn_operand(q_), k = attn_operand(k_), v = attn_operand(v_), go = attn_operand(grad_out);
+  const auto [o, rest] = output_pair(op, attn_operand(out), remainder, q);
   const at::Tensor l = lse.contiguous();
   const int64_t B = q.size(0), Sq = q.size(1), H = q.size(2);
   b200_attn_t a{};
   dense_window_desc(a, op, q, k, v, window, sinks, scale);
   a.o_sb = o.stride(0); a.o_sh = o.stride(2); a.o_ss = o.stride(1);
+  if (rest.defined()) a.remainder = rest.mutable_data_ptr();
   at::Tensor dq32 = at::empty({B, H, Sq, 128}, q.options().dtype(at::kFloat));
   at::Tensor delta = at::empty({B, H, Sq}, q.options().dtype(at::kFloat));
   at::Tensor gq = at::empty(q.sizes(), q.options()), gk = at::empty(k.sizes(), k.options()), gv = at::empty(v.sizes(), v.options());
@@ -452,14 +501,18 @@ namespace ops {
 
 TORCH_LIBRARY_FRAGMENT(blackwell, m) {
   m.def("varlen_attention(Tensor q, Tensor k, Tensor v, Tensor cu_seqlens_q, Tensor cu_seqlens_k, int max_seqlen_q, int max_seqlen_k, bool causal=False, float? scale=None, int? window=None, int sinks=0) -> (Tensor, Tensor)");
-  m.def("varlen_attention_backward(Tensor grad_out, Tensor q, Tensor k, Tensor v, Tensor out, Tensor lse, Tensor cu_seqlens_q, Tensor cu_seqlens_k, int max_seqlen_q, int max_seqlen_k, bool causal=False, float? scale=None, int? window=None, int sinks=0) -> (Tensor, Tensor, Tensor)");
+  m.def("varlen_attention_backward(Tensor grad_out, Tensor q, Tensor k, Tensor v, Tensor out, Tensor lse, Tensor cu_seqlens_q, Tensor cu_seqlens_k, int max_seqlen_q, int max_seqlen_k, bool causal=False, float? scale=None, int? window=None, int sinks=0, Tensor? remainder=None) -> (Tensor, Tensor, Tensor)");
+  m.def("varlen_attention_with_remainder(Tensor q, Tensor k, Tensor v, Tensor cu_seqlens_q, Tensor cu_seqlens_k, int max_seqlen_q, int max_seqlen_k, int window, int sinks=0, float? scale=None) -> (Tensor, Tensor, Tensor)");
+  m.def("window_attention_with_remainder(Tensor q, Tensor k, Tensor v, int window, int sinks=0, float? scale=None) -> (Tensor, Tensor, Tensor)");
   m.def("window_attention(Tensor q, Tensor k, Tensor v, int window, int sinks=0, float? scale=None) -> (Tensor, Tensor)");
-  m.def("window_attention_backward(Tensor grad_out, Tensor q, Tensor k, Tensor v, Tensor out, Tensor lse, int window, int sinks=0, float? scale=None) -> (Tensor, Tensor, Tensor)");
+  m.def("window_attention_backward(Tensor grad_out, Tensor q, Tensor k, Tensor v, Tensor out, Tensor lse, int window, int sinks=0, float? scale=None, Tensor? remainder=None) -> (Tensor, Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(blackwell, PrivateUse1, m) {
   m.impl("varlen_attention", TORCH_FN(varlen_attention));
   m.impl("varlen_attention_backward", TORCH_FN(varlen_attention_backward));
+  m.impl("varlen_attention_with_remainder", TORCH_FN(varlen_attention_with_remainder));
+  m.impl("window_attention_with_remainder", TORCH_FN(window_attention_with_remainder));
   m.impl("window_attention", TORCH_FN(window_attention));
   m.impl("window_attention_backward", TORCH_FN(window_attention_backward));
 }

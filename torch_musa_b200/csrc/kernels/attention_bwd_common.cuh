@@ -53,25 +53,28 @@ inline bool make_dq_map(CUtensorMap* out, float* ptr, int64_t rows) {
 // delta[b, h, q] = sum_d O[b, h, q, d] * dO[b, h, q, d], and the row of the fp32 dQ buffer is zeroed on the way.  Sixteen
 // lanes per row with 16-byte accesses, 64 consecutive rows of one (batch, head) per block, four rows in flight per lane:
 // bound by memory (2 x 256 bytes in, 512 out per row).  32 x 4096 rows: 24 us, against 30 (8-byte loads, a row per warp,
-// 64-bit divisions for its place) + 11 for the memset it replaces.
+// 64-bit divisions for its place) + 11 for the memset it replaces.  kRest: O comes with what rounding left of it.
 constexpr int kDeltaRows = 64;
-template <typename T>
+template <typename T, bool kRest = false>
 __global__ void __launch_bounds__(256) attn_delta_kernel(const T* __restrict__ o, const T* __restrict__ d_o, float* __restrict__ delta,
                                                          float* __restrict__ dq, int H, int Sq, int row_blocks, int64_t o_sb,
-                                                         int64_t o_sh, int64_t o_ss, int64_t g_sb, int64_t g_sh, int64_t g_ss) {
+                                                         int64_t o_sh, int64_t o_ss, int64_t g_sb, int64_t g_sh, int64_t g_ss,
+                                                         const T* __restrict__ rest = nullptr) {
   const int bh = (int)(blockIdx.x / row_blocks);
   const int b = bh / H, h = bh - b * H;
   const int q0 = (int)(blockIdx.x - (unsigned)bh * row_blocks) * kDeltaRows + (threadIdx.x >> 4);
   const int l16 = threadIdx.x & 15;
   const T* po = o + b * o_sb + h * o_sh + l16 * 8;
   const T* pg = d_o + b * g_sb + h * g_sh + l16 * 8;
-  Vec16<T> av[4], gv[4];
+  const T* pr = rest + b * o_sb + h * o_sh + l16 * 8;
+  Vec16<T> av[4], gv[4], rv[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int q = q0 + i * 16;
     if (q < Sq) {
       av[i] = ld16(po + q * o_ss);
       gv[i] = ld16(pg + q * g_ss);
+      if constexpr (kRest) rv[i] = ld16(pr + q * o_ss);
     }
   }
 #pragma unroll
@@ -80,7 +83,7 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(const T* __restrict__ o
     float s = 0.f;
     if (q < Sq) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) s += ToF<T>::to(av[i].v[e]) * ToF<T>::to(gv[i].v[e]);
+      for (int e = 0; e < 8; ++e) s += (kRest ? ToF<T>::to(av[i].v[e]) + ToF<T>::to(rv[i].v[e]) : ToF<T>::to(av[i].v[e])) * ToF<T>::to(gv[i].v[e]);
     }
 #pragma unroll
     for (int w = 8; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);

@@ -106,6 +106,13 @@ __device__ __forceinline__ void mul2(float& d0, float& d1, float x0, float x1, f
 }
 // the n lowest bits, for any n
 __device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u); }
+// 32 bytes at once, a whole sector: a thread that owns a row writes each of them in one piece
+__device__ __forceinline__ void st32(void* p, const uint32_t (&v)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]),
+               "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
 // A warp's walk over the units of work of packed sequences, numbered sequence after sequence: only those that exist are dealt, however
 // the lengths differ.  A lane holds one of 32 sequences at a time.
 struct UnitWalk {
@@ -153,6 +160,11 @@ template <>
 __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
   const __half2 v = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+  if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&w));
+  else return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w));
 }
 
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }

@@ -39,6 +39,7 @@ struct AttnParams {
   int total_q;
   int* status;
   int units;                  // pairs of query tiles of all (batch, head) instances
+  void* remainder;            // kWin: what rounding left of the output, laid out like it, or NULL
   int window, sinks;          // kWin: key j is visible when j <= i and (i - j < window or j < sinks)
 };
 
@@ -387,6 +388,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
       const bool w = mbar_wait(bar, parity, abort_flag);
       return __all_sync(0xffffffffu, w);
     };
+    T* const rest = kWin ? (T*)p.remainder : nullptr;
     uint32_t done = 0;                       // phases of mma_done[t] so far
     each_unit(std::true_type{}, [&](const FwdUnit& u) -> bool {
       const int qi = (2 * u.qp + t) * AQ + r;
@@ -516,19 +518,36 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
       if (ok && n_blocks > 0) {
         tc_fence_after();
         const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
-        T* orow = out + (int64_t)u.bt * p.o_sb + (int64_t)u.h * p.o_sh + (int64_t)(u.qoff + qi) * p.o_ss;
+        const int64_t at = (int64_t)u.bt * p.o_sb + (int64_t)u.h * p.o_sh + (int64_t)(u.qoff + qi) * p.o_ss;
+        T* orow = out + at;
 #pragma unroll
         for (int c = 0; c < AD / 32; ++c) {
           uint32_t raw[32];
           tmem_ld32(o_addr + (uint32_t)(c * 32), raw);
           tmem_ld_wait();
           if (qi < u.Sq) {
+            if (kWin && rest) {        // two stores of 32 bytes: 91 us for 32 heads x 4096, window 1024, 104 with four of 16 (89 without rest)
 #pragma unroll
-            for (int g8 = 0; g8 < 4; ++g8) {
-              Vec16<T> v;
+              for (int g16 = 0; g16 < 2; ++g16) {
+                uint32_t v[8], w[8];
 #pragma unroll
-              for (int e = 0; e < 8; ++e) v.v[e] = ToF<T>::from(__uint_as_float(raw[g8 * 8 + e]) * inv);
-              st16(orow + c * 32 + g8 * 8, v);
+                for (int e = 0; e < 8; ++e) {
+                  const float x0 = __uint_as_float(raw[g16 * 16 + 2 * e]) * inv, x1 = __uint_as_float(raw[g16 * 16 + 2 * e + 1]) * inv;
+                  v[e] = pack2<T>(x0, x1);
+                  const float2 r2 = unpack2<T>(v[e]);
+                  w[e] = pack2<T>(x0 - r2.x, x1 - r2.y);
+                }
+                st32(orow + c * 32 + g16 * 16, v);
+                st32(rest + at + c * 32 + g16 * 16, w);
+              }
+            } else {
+#pragma unroll
+              for (int g8 = 0; g8 < 4; ++g8) {
+                Vec16<T> v;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v.v[e] = ToF<T>::from(__uint_as_float(raw[g8 * 8 + e]) * inv);
+                st16(orow + c * 32 + g8 * 8, v);
+              }
             }
           }
         }
@@ -541,8 +560,11 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
 #pragma unroll
         for (int e = 0; e < 8; ++e) zero.v[e] = ToF<T>::from(0.f);
         if (n_blocks == 0 && qi < u.Sq) {                  // a query that sees no key
-          T* orow = out + (int64_t)u.bt * p.o_sb + (int64_t)u.h * p.o_sh + (int64_t)(u.qoff + qi) * p.o_ss;
-          for (int c = 0; c < AD; c += 8) st16(orow + c, zero);
+          const int64_t at = (int64_t)u.bt * p.o_sb + (int64_t)u.h * p.o_sh + (int64_t)(u.qoff + qi) * p.o_ss;
+          for (int c = 0; c < AD; c += 8) {
+            st16(out + at + c, zero);
+            if (rest) st16(rest + at + c, zero);
+          }
           if (p.lse) p.lse[p.cu_q ? (int64_t)u.h * p.total_q + u.qoff + qi : ((int64_t)u.b * p.H + u.h) * p.Sq + qi] = -INFINITY;
         }
       }
@@ -555,7 +577,9 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
         for (int e = 0; e < 8; ++e) zero.v[e] = ToF<T>::from(0.f);
         for (int x = p.cu_q[p.B] + blockIdx.x * 16 + (threadIdx.x >> 4); x < p.total_q; x += gridDim.x * 16)
           for (int y = 0; y < p.H; ++y) {
-            st16(out + (int64_t)y * p.o_sh + (int64_t)x * p.o_ss + (threadIdx.x & 15) * 8, zero);
+            const int64_t at = (int64_t)y * p.o_sh + (int64_t)x * p.o_ss + (threadIdx.x & 15) * 8;
+            st16(out + at, zero);
+            if (rest) st16(rest + at, zero);
             if (p.lse && (threadIdx.x & 15) == 0) p.lse[(int64_t)y * p.total_q + x] = -INFINITY;
           }
       }
@@ -630,6 +654,7 @@ extern "C" int b200_flash_attn_fwd(const b200_attn_t* a, void* out, float* lse, 
   const long long grid = (long long)a->B * a->H * p.q_pairs;
   if (grid > 2147483647ll - 1024) return (int)cudaErrorNotSupported;
   p.units = (int)grid;
+  p.remainder = a->remainder;
   p.window = a->window;
   p.sinks = a->sinks;
   auto launch = [&](auto kern, OncePerDevice& once, auto* o) -> int {
@@ -641,6 +666,8 @@ extern "C" int b200_flash_attn_fwd(const b200_attn_t* a, void* out, float* lse, 
   static OncePerDevice once[4];
   if (a->window > 0) {
     if (!a->causal || a->window > (1 << 30) || a->sinks < 0) return (int)cudaErrorNotSupported;
+    if (a->remainder && (((reinterpret_cast<uintptr_t>(a->remainder) | reinterpret_cast<uintptr_t>(out)) & 31) || a->o_sb % 16 || a->o_sh % 16 || a->o_ss % 16))
+      return (int)cudaErrorNotSupported;                                                     // stored 32 bytes at a time
     return bf16 ? launch(attn_fwd_kernel<__nv_bfloat16, true>, once[2], (__nv_bfloat16*)out)
                 : launch(attn_fwd_kernel<__half, true>, once[3], (__half*)out);
   }

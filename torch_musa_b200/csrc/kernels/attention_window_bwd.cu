@@ -14,9 +14,10 @@
 //     the chain K -> S^T -> P -> dS that starts afresh: K and V of the next unit have no place before the last product of this one.
 //   * Hidden scores become -inf before the exponentials, two instructions an element, instead of tests inside the loops, whose second
 //     copy of the code cost more than they did (instructions came late).
-//   * The row sums of dO O come from O as it was stored, rounded to 16 bits, as in the causal backward.  Where a query sees hundreds of keys
-//     that adds nothing beside the rounding of dS (gradients of q and k are off by 2.4e-3 of their norm in bf16, 1.7e-3 of it by their own
-//     rounding); with two keys it shows (3.7e-3).  The remainder of O, kept by the forward, would mend that for 2 x 256 bytes a row, 2 % of the time.
+//   * The row sums of dO O are taken with what rounding left of O, which the forward keeps for it: with few keys in a window dS is a
+//     difference of nearly equal numbers, and the rounded O alone put the gradients of q and k off by 3.7e-3 of their norm (two keys, bf16),
+//     now 2.5e-3 as with many keys: dS is rounded before its products (1.7e-3, as much as the result's own rounding).  It costs 3 % of
+//     forward and backward.
 //   * Packed rows that are not the sequence's own are zeros in shared memory before a product reads them: their probabilities are zero,
 //     but zero times what lies there need not be.
 // Measured (whole calls: row dots, this kernel, sums of the chunks, conversion of dQ): 32 heads x 4096, window 1024, four sinks 273 us (289
@@ -736,7 +737,9 @@ int attn_window_bwd(const b200_attn_t* a, float* dq_accum, void* dk, void* dv, f
   p.sink_blocks = sink_blocks(a);
   p.sink_chunks = sink_chunks(a);
   p.sink_ws = a->workspace;
-  if (!a->causal || a->window > (1 << 30) || a->sinks < 0 || (p.sink_chunks > 1 && !p.sink_ws)) return (int)cudaErrorNotSupported;
+  if (!a->causal || a->window > (1 << 30) || a->sinks < 0 || (p.sink_chunks > 1 && !p.sink_ws) ||
+      (reinterpret_cast<uintptr_t>(a->remainder) & 15))
+    return (int)cudaErrorNotSupported;
   const long long units = (long long)a->B * a->Hkv * (p.kv_blocks + p.sink_blocks * (p.sink_chunks - 1));
   if (units > 2147483647ll - 1024) return (int)cudaErrorNotSupported;
   p.units = (int)units;
@@ -744,8 +747,9 @@ int attn_window_bwd(const b200_attn_t* a, float* dq_accum, void* dk, void* dv, f
   auto launch = [&](auto kern, OncePerDevice& once, auto* gk, auto* gv) -> int {
     using T = std::remove_pointer_t<decltype(gk)>;
     if (int e = once([&] { return bwd_setup(kern); })) return e;
-    attn_delta_kernel<T><<<m.delta_grid, 256, 0, stream>>>((const T*)o, (const T*)d_o, delta, dq_accum, a->H, m.delta_rows, (int)m.row_blocks,
-                                                           a->o_sb, a->o_sh, a->o_ss, x[0], x[1], x[2]);
+    auto delta_kern = a->remainder ? attn_delta_kernel<T, true> : attn_delta_kernel<T, false>;
+    delta_kern<<<m.delta_grid, 256, 0, stream>>>((const T*)o, (const T*)d_o, delta, dq_accum, a->H, m.delta_rows, (int)m.row_blocks, a->o_sb,
+                                                 a->o_sh, a->o_ss, x[0], x[1], x[2], (const T*)a->remainder);
     kern<<<grid, kBwdThreads, kBwdSmem, stream>>>(m.q, m.k, m.v, m.d_o, m.dq, gk, gv, p);
     note_launch(2);
     if (p.sink_blocks > 0 && p.sink_chunks > 1) {

@@ -561,6 +561,8 @@ typedef struct {
   int window, sinks;
   /* backward with a window: b200_flash_attn_bwd_workspace(desc) floats of scratch (may be NULL when that is 0) */
   float* workspace;
+  /* with a window: what rounding left of out, in out's type and layout (forward: where it goes, backward: read), or NULL */
+  void* remainder;
 } b200_attn_t;
 B200_API int64_t b200_flash_attn_bwd_workspace(const b200_attn_t* desc);
 B200_API int b200_flash_attn_fwd(const b200_attn_t* desc, void* out, float* lse, const void* q, const void* k,

@@ -137,7 +137,7 @@ def _(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, causal=Fa
 
 @_reg("varlen_attention_backward")
 def _(grad_out, q, k, v, out, lse, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, causal=False, scale=None,
-      window=None, sinks=0):
+      window=None, sinks=0, remainder=None):
     return (torch.empty_like(q, memory_format=torch.contiguous_format), torch.empty_like(k, memory_format=torch.contiguous_format),
             torch.empty_like(v, memory_format=torch.contiguous_format))
 
@@ -162,8 +162,18 @@ def _(q, k, v, window, sinks=0, scale=None):
     return q.new_empty(q.shape), q.new_empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32)
 
 
+@_reg("window_attention_with_remainder")
+def _(q, k, v, window, sinks=0, scale=None):
+    return q.new_empty(q.shape), q.new_empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32), q.new_empty(q.shape)
+
+
+@_reg("varlen_attention_with_remainder")
+def _(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, window, sinks=0, scale=None):
+    return q.new_empty(q.shape), q.new_empty((q.shape[1], q.shape[0]), dtype=torch.float32), q.new_empty(q.shape)
+
+
 @_reg("window_attention_backward")
-def _(grad_out, q, k, v, out, lse, window, sinks=0, scale=None):
+def _(grad_out, q, k, v, out, lse, window, sinks=0, scale=None, remainder=None):
     return q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
 
 

@@ -381,15 +381,16 @@ def _native_attention(q, k, v) -> bool:
 class _WindowAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, window, sinks, scale):
-        out, lse = torch.ops.blackwell.window_attention(q, k, v, window, sinks, scale)
-        ctx.save_for_backward(q, k, v, out, lse)
+        out, lse, rest = torch.ops.blackwell.window_attention_with_remainder(q, k, v, window, sinks, scale)
+        ctx.save_for_backward(q, k, v, out, lse, rest)
         ctx.args = (window, sinks, scale)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_out):
-        dq, dk, dv = torch.ops.blackwell.window_attention_backward(d_out, *ctx.saved_tensors, *ctx.args)
+        *saved, rest = ctx.saved_tensors
+        dq, dk, dv = torch.ops.blackwell.window_attention_backward(d_out, *saved, *ctx.args, rest)
         return dq, dk, dv, None, None, None
 
 
@@ -421,15 +422,19 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
 class _VarlenAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, cu_q, cu_k, max_q, max_k, causal, scale, window, sinks):
-        out, lse = torch.ops.blackwell.varlen_attention(q, k, v, cu_q, cu_k, max_q, max_k, causal, scale, window, sinks)
-        ctx.save_for_backward(q, k, v, out, lse, cu_q, cu_k)
+        rest = None
+        if window is not None and any(ctx.needs_input_grad):
+            out, lse, rest = torch.ops.blackwell.varlen_attention_with_remainder(q, k, v, cu_q, cu_k, max_q, max_k, window, sinks, scale)
+        else:
+            out, lse = torch.ops.blackwell.varlen_attention(q, k, v, cu_q, cu_k, max_q, max_k, causal, scale, window, sinks)
+        ctx.save_for_backward(q, k, v, out, lse, cu_q, cu_k, rest)
         ctx.args = (max_q, max_k, causal, scale, window, sinks)
         return out
 
     @staticmethod
     def backward(ctx, d_out):
-        q, k, v, out, lse, cu_q, cu_k = ctx.saved_tensors
-        dq, dk, dv = torch.ops.blackwell.varlen_attention_backward(d_out, q, k, v, out, lse, cu_q, cu_k, *ctx.args)
+        q, k, v, out, lse, cu_q, cu_k, rest = ctx.saved_tensors
+        dq, dk, dv = torch.ops.blackwell.varlen_attention_backward(d_out, q, k, v, out, lse, cu_q, cu_k, *ctx.args, rest)
         return dq, dk, dv, None, None, None, None, None, None, None, None
 
 
