@@ -417,3 +417,30 @@ def test_two_streams_and_two_graphs(bw, dev):
                     assert float((a.double() - b.double()).abs().max()) <= float(2 ** -8 * b.double().abs().max())
                 else:
                     assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("sinks", [0, 3])
+def test_small_gradients_of_a_long_window(bw, dev, sinks):
+    """fp16, thousands of keys and an incoming gradient of 2^-10: what is rounded before the products, p (dP - delta) without the softmax
+    scale, still has most of its bits.  The formula in 64 bits with that one rounding, and that of the result, gives the error to
+    expect (as a norm); the sums of 32 bits and the output's remainder stay far below it, so twice it is the limit.  (With the scale in
+    front of the rounding it is eleven times as large.)"""
+    from torch_musa_b200.ops import window_attention
+
+    S, H, window, dt, scale = 2600, 2, 2500, torch.float16, 1 / math.sqrt(D)
+    q, k, v, do = inputs(dt, (1, S, H, D), (1, S, 1, D), 41)
+    do = (do.float() * 2.0 ** -10).to(dt)
+    seen = visible(S, S, window, sinks)
+    want, model = [torch.zeros(S, n, D, dtype=torch.float64) for n in (H, 1)], [torch.zeros(S, n, D, dtype=torch.float64) for n in (H, 1)]
+    for h in range(H):
+        qh, kh, vh, gh = q[0, :, h].double(), k[0, :, 0].double(), v[0, :, 0].double(), do[0, :, h].double()
+        p = torch.softmax((qh @ kh.T * scale).masked_fill(~seen, -math.inf), 1)
+        ds = p * (gh @ vh.T - (gh * (p @ vh)).sum(1, keepdim=True))
+        for to, x in ((want, ds), (model, ds.to(dt).double())):
+            to[0][:, h] = x @ kh * scale
+            to[1][:, 0] += x.T @ qh * scale
+    leaves = [t.to(dev).requires_grad_() for t in (q, k, v)]
+    grads = torch.autograd.grad(window_attention(*leaves, window, sinks), leaves, do.to(dev))
+    for name, got, w, m in zip(("dq", "dk"), grads, want, model):
+        expected = float((m.to(dt).double() - w).norm())
+        assert float((got[0].cpu().double() - w).norm()) <= 2 * expected, name

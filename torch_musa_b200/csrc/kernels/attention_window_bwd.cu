@@ -18,6 +18,10 @@
 //     difference of nearly equal numbers, and the rounded O alone put the gradients of q and k off by 3.7e-3 of their norm (two keys, bf16),
 //     now 2.5e-3 as with many keys: dS is rounded before its products (1.7e-3, as much as the result's own rounding).  It costs 3 % of
 //     forward and backward.
+//   * dS goes into its products without the softmax scale, which dQ and dK get in 32 bits when they leave TMEM: in fp16 its values are small
+//     under a long window, and a scale of 0.088 in front of the rounding would take three and a half bits more from them (4096 keys, dO of
+//     2^-10: dQ and dK off by 1.3e-2 of their norm with it, 1.2e-3 without).  In return fp16's largest value, 65504, bounds P (dP - delta)
+//     itself and not 0.088 of it.
 //   * Packed rows that are not the sequence's own are zeros in shared memory before a product reads them: their probabilities are zero,
 //     but zero times what lies there need not be.
 // Measured (whole calls: row dots, this kernel, sums of the chunks, conversion of dQ): 32 heads x 4096, window 1024, four sinks 273 us (289
@@ -38,7 +42,7 @@ using namespace attndev;
 
 struct WindowParams {
   int B, H, Hkv, Sq, Sk;
-  float scale, scale_log2;      // of dS; of the exponents, times log2(e)
+  float scale, scale_log2;      // of dQ and dK; of the exponents, times log2(e)
   const float* lse;       // [B, H, Sq] natural log
   const float* delta;     // [B, H, Sq]
   float* dq;              // [B, H, Sq, 128] fp32
@@ -350,8 +354,8 @@ attn_window_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       __syncwarp();
     } else if (warp == 14) {
       // ------------------------------------------------------------ lse (log2 domain, negated: an addend of the exponent) and
-      // delta (times the softmax scale, negated) of every query block; an lse of -inf switches a row off
-      // (read one block ahead, all eight loads in flight at once)
+      // delta (negated) of every query block; an lse of -inf switches a row off (read one block ahead, all eight loads in flight at
+      // once)
       int h, i, gi = 0;
       float l[4], d[4];
       auto fetch = [&](const BwdUnit& u) {
@@ -373,7 +377,7 @@ attn_window_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             s_lse[st * 128 + e * 32 + lane] = l[e] > -INFINITY ? -l[e] * 1.4426950408889634f : -INFINITY;
-            s_dlt[st * 128 + e * 32 + lane] = -d[e] * p.scale;
+            s_dlt[st * 128 + e * 32 + lane] = -d[e];
           }
           __syncwarp();
           if (lane == 0) mbar_arrive(&ld_full[st]);
@@ -450,6 +454,15 @@ attn_window_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(dq_drained);
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            float x0, x1;
+            mul2(x0, x1, __uint_as_float(raw[c][e]), __uint_as_float(raw[c][e + 1]), p.scale, p.scale);
+            raw[c][e] = __float_as_uint(x0);
+            raw[c][e + 1] = __float_as_uint(x1);
+          }
         if (q0 + r >= u.Sq) {        // a row of the next sequence or head: zero, also where this one's keys are not finite
 #pragma unroll
           for (int c = 0; c < 4; ++c)
@@ -564,8 +577,8 @@ attn_window_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
 #pragma unroll
             for (int e2 = 0; e2 < 4; e2 += 2) {
               const int e = e4 * 4 + e2, cc = c * 32 + e;
-              float t0, t1, d0, d1;
-              fma2v(t0, t1, __uint_as_float(raw[e]), __uint_as_float(raw[e + 1]), p.scale, nds[e2], nds[e2 + 1]);
+              float t0 = __uint_as_float(raw[e]), t1 = __uint_as_float(raw[e + 1]), d0, d1;
+              add2(t0, t1, nds[e2], nds[e2 + 1]);
               mul2(d0, d1, pf[cc], pf[cc + 1], t0, t1);
               pk[e >> 1] = pack2<T>(d0, d1);
             }
@@ -601,6 +614,10 @@ attn_window_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
             if (n_it > 0) {
               tmem_ld32(tmem_base + lane_base + (which ? kColDK : kColDV) + (uint32_t)(wg * 64 + c * 32), raw);
               tmem_ld_wait();
+              if (which) {
+#pragma unroll
+                for (int e = 0; e < 32; ++e) raw[e] = __float_as_uint(__uint_as_float(raw[e]) * p.scale);
+              }
             } else {
 #pragma unroll
               for (int e = 0; e < 32; ++e) raw[e] = 0u;
