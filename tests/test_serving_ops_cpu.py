@@ -1,10 +1,13 @@
 """Windowed attention, the paged cache and the verification of drafts off the device: the plain formulation against loops in 64
 bits, refusals, and the paged decoder against the model run from scratch."""
+import ctypes
 import math
+import os
 
 import pytest
 import torch
 
+import torch_musa_b200
 from torch_musa_b200 import ops
 from torch_musa_b200.models import Llama, PagedLlamaDecoder, llama_tiny_config
 from torch_musa_b200.models.decode import LlamaDecoder
@@ -294,3 +297,34 @@ def test_paged_decoder_is_unchanged_by_a_call_that_fails():
         assert dec.seq_lens.tolist() == [3, 0] and dec.lens == [3, None]
     taken, _ = dec.check(*good)
     assert dec.lens[0] == 4 + int(taken[0])
+
+
+class AttnDesc(ctypes.Structure):
+    """b200_attn_t of csrc/kernels/b200_kernels.h."""
+    _fields_ = ([(n, ctypes.c_int) for n in ("B", "H", "Hkv", "Sq", "Sk", "head_dim", "dtype", "causal")] + [("scale", ctypes.c_float)]
+                + [(f"{t}_{d}", ctypes.c_int64) for t in "qkvo" for d in ("sb", "sh", "ss")]
+                + [("cu_q", ctypes.c_void_p), ("cu_k", ctypes.c_void_p), ("total_q", ctypes.c_int), ("total_k", ctypes.c_int), ("window", ctypes.c_int),
+                   ("sinks", ctypes.c_int), ("workspace", ctypes.c_void_p), ("remainder", ctypes.c_void_p)])
+
+
+@pytest.mark.parametrize("sinks", [1, 4, 130, 4096, 2 ** 30])
+@pytest.mark.parametrize("Hkv", [1, 8, 32])
+def test_scratch_of_the_windowed_backward_is_bounded(Hkv, sinks):
+    """By the machine, not by sequences times the longest length or by the number of sinks: 1776 pairs of 64 KB."""
+    kernels = ctypes.CDLL(os.path.join(os.path.dirname(torch_musa_b200.__file__), "libb200_kernels.so"))
+    kernels.b200_flash_attn_bwd_workspace.restype = ctypes.c_int64
+    pair = 2 * 128 * 128
+
+    def floats(B, S, window, total=0):
+        d = AttnDesc(B=B, H=32, Hkv=Hkv, Sq=S, Sk=S, head_dim=128, dtype=1, causal=1, scale=1.0, total_q=total, total_k=total, window=window, sinks=sinks)
+        if total:
+            d.cu_q = d.cu_k = 1         # looked at for being there only
+        return kernels.b200_flash_attn_bwd_workspace(ctypes.byref(d))
+
+    for window in (1, 64, 128, 1024):
+        for B, S, total in ((1, 4096, 0), (1, 32768, 0), (64, 4096, 0), (64, 4096, 4096 + 63 * 100), (200, 8192, 8192 + 199 * 30), (200, 8192, 200 * 8192)):
+            n = floats(B, S, window, total)
+            assert 0 <= n <= 1776 * pair and n % pair == 0
+    assert floats(5, 128, 1) == 0 and floats(3, 100, 1, 300) == 0         # one block of queries is not cut
+    if sinks <= 128 and Hkv < 32:
+        assert floats(1, 4096, 64) >= 4 * Hkv * pair                        # long ranges of few blocks are

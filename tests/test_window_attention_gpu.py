@@ -444,3 +444,37 @@ def test_small_gradients_of_a_long_window(bw, dev, sinks):
     for name, got, w, m in zip(("dq", "dk"), grads, want, model):
         expected = float((m.to(dt).double() - w).norm())
         assert float((got[0].cpu().double() - w).norm()) <= 2 * expected, name
+
+
+@pytest.mark.parametrize("lens,H,Hkv,window,sinks", [
+    ([1500] + [40, 7, 129] * 12, 2, 1, 64, 4), ([40, 0, 129] * 12 + [1500], 2, 2, 64, 4), ([60, 1400, 3, 0, 900, 128], 4, 2, 100, 130),
+    ([300, 1300, 1], 2, 1, 64, 1000), ([260, 1300], 2, 2, 1, 5000), ([1100] * 3, 16, 16, 40, 1100)])
+def test_chunks_of_the_sinks_go_by_the_sequence(bw, dev, lens, H, Hkv, window, sinks):
+    """Long sequences among short ones, sinks over many blocks and past every end: each sequence's own number of chunks, in places that
+    follow from its first row."""
+    test_packed_sequences(bw, dev, torch.bfloat16, lens, None, H, Hkv, window, sinks, 3)
+
+
+@pytest.mark.parametrize("B,S,H,Hkv,window,sinks", [(2, 1000, 2, 1, 64, 1000), (1, 1400, 16, 16, 64, 4000), (1, 1100, 2, 2, 1, 300)])
+def test_many_sinks(bw, dev, B, S, H, Hkv, window, sinks):
+    test_dense_forward_and_gradients(bw, dev, torch.float16, B, S, S, H, Hkv, window, sinks)
+
+
+def test_scratch_does_not_grow_with_the_number_of_sequences(bw, dev):
+    """One long sequence among 199 short ones: what the backward allocates beside its results follows the rows."""
+    from torch_musa_b200.ops import flash_attn_varlen_func
+
+    lens, H, Hkv = [8192] + [20] * 199, 8, 8
+    n = sum(lens)
+    q, k, v, do = (torch.ones(n, h, D, dtype=torch.bfloat16, device=dev) for h in (H, Hkv, Hkv, H))
+    cu = torch.tensor([0] + lens).cumsum(0).to(torch.int32).to(dev)
+    for t in (q, k, v):
+        t.requires_grad_()
+    out = flash_attn_varlen_func(q, k, v, cu, cu, 8192, 8192, causal=True, window=128, sinks=4)
+    bw.synchronize()
+    bw.reset_peak_memory_stats()
+    before = bw.memory_allocated()
+    torch.autograd.grad(out, (q, k, v), do)
+    bw.synchronize()
+    results = 2 * D * n * (H + 2 * Hkv) + 4 * D * n * H + 4 * n * H          # gradients, dq and the row dots in 32 bits
+    assert bw.max_memory_allocated() - before <= results + 1776 * 2 * 4 * 128 * 128

@@ -6,8 +6,8 @@
 // fp32.  What differs:
 //   * The queries that see a block of keys are a contiguous range, window + 127 long behind the block's first key, or all that follow when
 //     it holds sinks.  A block with sinks meets many more query blocks than the others (at 4096 tokens and a window of 1024: 32 against
-//     9, times the heads of a group), so its range is cut into chunks of about the others' length; their dV and dK go to fp32 buffers
-//     that a small kernel adds up in order.
+//     9, times the heads of a group), so its range is cut into chunks of about the others' length, in each sequence by its own length;
+//     their dV and dK go to fp32 buffers that a small kernel adds up in order.
 //   * Units are short, and starting and ending a CTA cost as much as three or four pairs of blocks: a CTA stays on its SM and takes every
 //     148th unit, turning round at either end so that long and short ones even out.  The loads of a unit's queries, and the waits for its
 //     first products, run while the one before it is stored.  A warp of its own finds the units and hands them over.  What a change of units still costs, about 5 us of 27 for nine pairs, is
@@ -56,9 +56,23 @@ struct WindowParams {
   int total_q;
   int window, sinks, total_k;
   int units;                      // units of work that the CTAs share
-  int sink_blocks, sink_chunks;   // key blocks with sinks, CTAs that share the query blocks of one of them
-  float* sink_ws;                 // sink_chunks > 1: fp32 [B * Hkv][sink_blocks][sink_chunks][dV, dK][128][128]
+  int sink_blocks, sink_chunk;    // key blocks with sinks (of a long sequence), query blocks of a chunk of theirs
+  int sink_slots;                 // places of chunks; 0: no sequence has more than one
+  float* sink_ws;                 // fp32 [sink_slots][sink_blocks][Hkv][dV, dK][128][128]
 };
+
+// Query blocks of sequence b, and the chunks into which those of its sinks are cut.
+__device__ __forceinline__ int query_blocks(const WindowParams& p, int b) {
+  return p.cu_q ? min(p.q_blocks, (max(0, p.cu_q[b + 1] - p.cu_q[b]) + BQ - 1) / BQ) : p.q_blocks;
+}
+__device__ __forceinline__ int chunks_of(const WindowParams& p, int q_blocks) { return max(1, (q_blocks + p.sink_chunk - 1) / p.sink_chunk); }
+// The first of sequence b's places.  Packed sequences find theirs by their first row alone, without a sum over those in front: with
+// c = sink_chunk, n > c query blocks are at least 128 (n - 1) + 1 rows and n' = ceil(n / c) = floor((n - 1) / c) + 1 chunks, so that
+// n' <= 2 floor((n - 1) / c) <= 2 rows / (128 c), and ceil(x + y) - ceil(x) >= floor(y).
+__host__ __device__ __forceinline__ int slots_before(int64_t rows, int chunk) { return (int)((2 * rows + BQ * chunk - 1) / (BQ * chunk)); }
+__device__ __forceinline__ int first_slot(const WindowParams& p, int b) {
+  return p.cu_q ? slots_before(p.cu_q[b], p.sink_chunk) : b * chunks_of(p, p.q_blocks);
+}
 
 // The query blocks [first, end) that see key block kb.
 __device__ __forceinline__ void window_queries(const WindowParams& p, int kb, int Sq, int Sk, int q_blocks, int& first, int& end) {
@@ -87,7 +101,7 @@ constexpr int kUnitBytes = 128;          // of their descriptions, beyond the co
 struct BwdUnit {
   int kb, chunk, bh, b, hk, k0, Sq, Sk, qoff, koff, bt;
   int i0, n_i, n_it, h0, istart;      // first query block, query blocks, pairs of query block and head, where the pairs start
-  bool partial;
+  int slot;                           // of a chunk's sums; -1: the unit is the whole block
 };
 
 template <typename T>
@@ -134,7 +148,7 @@ attn_window_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int n_bh = p.B * p.Hkv, G = p.H / p.Hkv;
-  auto complete = [&](BwdUnit& u) {        // from kb, chunk, b and hk
+  auto complete = [&](BwdUnit& u, int chunks) {        // from kb, chunk, b and hk
     u.bh = u.b * p.Hkv + u.hk;
     u.k0 = u.kb * BK;
     // this instance's sequence (see the forward kernel): rows past a packed sequence's end are loaded, masked by index
@@ -142,23 +156,22 @@ attn_window_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     u.Sq = p.Sq;
     u.Sk = p.Sk;
     u.bt = u.b;
-    int q_blocks = p.q_blocks;
     if (p.cu_q) {
       u.qoff = p.cu_q[u.b];
       u.Sq = p.cu_q[u.b + 1] - u.qoff;
       u.koff = p.cu_k[u.b];
       u.Sk = p.cu_k[u.b + 1] - u.koff;
       u.bt = 0;
-      q_blocks = (u.Sq + BQ - 1) / BQ;
     }
     int end;
-    window_queries(p, u.kb, u.Sq, u.Sk, q_blocks, u.i0, end);
+    window_queries(p, u.kb, u.Sq, u.Sk, query_blocks(p, u.b), u.i0, end);
     u.n_i = end - u.i0;
     u.n_it = u.n_i * G;
     u.h0 = u.hk * G;
-    u.partial = u.kb < p.sink_blocks && p.sink_chunks > 1;
-    if (u.partial) {                                  // pairs [chunk * per, (chunk + 1) * per) of this block's
-      const int per = (u.n_it + p.sink_chunks - 1) / p.sink_chunks, from = min(u.n_it, u.chunk * per);
+    u.slot = -1;
+    if (u.kb < p.sink_blocks && chunks > 1) {         // pairs [chunk * per, (chunk + 1) * per) of this block's
+      u.slot = first_slot(p, u.b) + u.chunk;
+      const int per = (u.n_it + chunks - 1) / chunks, from = min(u.n_it, u.chunk * per);
       u.n_it = min(u.n_it, from + per) - from;
       if (u.n_i > 0) {
         u.h0 += from / u.n_i;
@@ -214,7 +227,7 @@ attn_window_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     tmem_relinquish();
   }
   auto key_blocks = [&](int b) { return min(p.kv_blocks, (max(0, p.cu_k[b + 1] - p.cu_k[b]) + BK - 1) / BK); };
-  auto sink_units = [&](int b) { return min(key_blocks(b), p.sink_blocks) * p.sink_chunks; };
+  auto sink_units = [&](int b) { return min(key_blocks(b), p.sink_blocks) * chunks_of(p, query_blocks(p, b)); };
   auto other_units = [&](int b) { return max(0, key_blocks(b) - p.sink_blocks); };
   UnitWalk walk;
   if (warp == 15 && p.cu_q) walk.take(0, 0, p.B, lane, sink_units);
@@ -405,7 +418,7 @@ attn_window_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
           u.hk = unit % p.Hkv;
           if (!in_sinks) u.kb += p.sink_blocks;
         } else {
-          const int pairs = p.sink_blocks * p.sink_chunks, bh = unit % n_bh;
+          const int pairs = p.sink_blocks * chunks_of(p, p.q_blocks), bh = unit % n_bh;
           there = unit < p.units;
           u.kb = unit / n_bh;
           u.b = bh / p.Hkv;
@@ -413,12 +426,16 @@ attn_window_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
           in_sinks = u.kb < pairs;
           if (!in_sinks) u.kb -= pairs - p.sink_blocks;
         }
-        if (in_sinks) {                       // numbers of (block, chunk) pairs
-          u.chunk = u.kb % p.sink_chunks;
-          u.kb /= p.sink_chunks;
+        if (there) {
+          const int chunks = chunks_of(p, query_blocks(p, u.b));
+          if (in_sinks) {                     // numbers of (block, chunk) pairs
+            u.chunk = u.kb % chunks;
+            u.kb /= chunks;
+          }
+          complete(u, chunks);
+        } else {
+          u.kb = -1;
         }
-        if (there) complete(u);
-        else u.kb = -1;
         if (!mbar_wait_warp(&u_empty[n & 1], ((n >> 1) & 1) ^ 1, abort_flag)) break;
         if (lane == 0) {
           s_unit[n & 1] = u;
@@ -622,8 +639,8 @@ attn_window_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
 #pragma unroll
               for (int e = 0; e < 32; ++e) raw[e] = 0u;
             }
-            if (u.partial) {
-              float* dst = p.sink_ws + ((((int64_t)u.bh * p.sink_blocks + u.kb) * p.sink_chunks + u.chunk) * 2 + which) * (BK * BD) + r * BD +
+            if (u.slot >= 0) {
+              float* dst = p.sink_ws + ((((int64_t)u.slot * p.sink_blocks + u.kb) * p.Hkv + u.hk) * 2 + which) * (BK * BD) + r * BD +
                            wg * 64 + c * 32;
               if (n_it > 0) {
 #pragma unroll
@@ -674,28 +691,37 @@ attn_window_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
   settle_abort(abort_flag, p.status);
 }
 
-// dV and dK of the blocks with sinks: the chunks' sums, added in order (the same for every run) and rounded once.  A thread owns
-// eight dimensions of a row.
+// dV and dK of the blocks with sinks of sequences that have more than one chunk: the chunks' sums, added in order (the same for every run)
+// and rounded once.  Eight blocks a place, key block and key head; a thread owns eight dimensions of a row.  Packed sequences: the
+// blocks of a sequence's first place do the work.
 template <typename T>
 __global__ void __launch_bounds__(256) attn_sink_sum_kernel(T* __restrict__ dk, T* __restrict__ dv, const WindowParams p) {
   const int which = blockIdx.y, r = (int)(blockIdx.x % 8) * 16 + (threadIdx.x >> 4), c = (threadIdx.x & 15) * 8;
-  const int unit = (int)(blockIdx.x / 8), kb = unit % p.sink_blocks, bh = unit / p.sink_blocks;
-  const int b = bh / p.Hkv, hk = bh - b * p.Hkv, kj = kb * BK + r;
-  int Sq = p.Sq, Sk = p.Sk, koff = 0, bt = b, q_blocks = p.q_blocks;
+  const int unit = (int)(blockIdx.x / 8), hk = unit % p.Hkv, kb = unit / p.Hkv % p.sink_blocks, place = unit / p.Hkv / p.sink_blocks;
+  const int kj = kb * BK + r;
+  int b = place, slot = place * chunks_of(p, p.q_blocks), Sk = p.Sk, Sq = p.Sq, koff = 0, bt = b;
   if (p.cu_q) {
-    Sq = p.cu_q[b + 1] - p.cu_q[b];
+    slot = place;
+    int above = p.B;                     // the last sequence whose places start here or before
+    b = 0;
+    while (above - b > 1) {
+      const int mid = (b + above) >> 1;
+      if (first_slot(p, mid) <= slot) b = mid; else above = mid;
+    }
+    if (first_slot(p, b) != slot) return;
     koff = p.cu_k[b];
     Sk = p.cu_k[b + 1] - koff;
+    Sq = p.cu_q[b + 1] - p.cu_q[b];
     bt = 0;
-    q_blocks = (Sq + BQ - 1) / BQ;
   }
-  if (kj >= Sk) return;
+  const int q_blocks = query_blocks(p, b), chunks = chunks_of(p, q_blocks);
+  if (chunks == 1 || kj >= Sk) return;
   int first, end;
   window_queries(p, kb, Sq, Sk, q_blocks, first, end);
-  const int n_it = (end - first) * (p.H / p.Hkv), per = (n_it + p.sink_chunks - 1) / p.sink_chunks;
+  const int n_it = (end - first) * (p.H / p.Hkv), per = (n_it + chunks - 1) / chunks;
   float s[8] = {};
-  const float* src = p.sink_ws + (((int64_t)unit * p.sink_chunks) * 2 + which) * (BK * BD) + r * BD + c;
-  for (int ch = 0; ch * per < n_it; ++ch, src += 2 * BK * BD) {
+  const float* src = p.sink_ws + ((((int64_t)slot * p.sink_blocks + kb) * p.Hkv + hk) * 2 + which) * (BK * BD) + r * BD + c;
+  for (int ch = 0; ch * per < n_it; ++ch, src += (int64_t)p.sink_blocks * p.Hkv * 2 * BK * BD) {
     const float4 x = *reinterpret_cast<const float4*>(src), y = *reinterpret_cast<const float4*>(src + 4);
     s[0] += x.x; s[1] += x.y; s[2] += x.z; s[3] += x.w;
     s[4] += y.x; s[5] += y.y; s[6] += y.z; s[7] += y.w;
@@ -707,14 +733,26 @@ __global__ void __launch_bounds__(256) attn_sink_sum_kernel(T* __restrict__ dk, 
   else st16(dv + (int64_t)bt * p.dv_sb + (int64_t)hk * p.dv_sh + (int64_t)(koff + kj) * p.dv_ss + c, o);
 }
 
-// How many CTAs share the query blocks of a key block with sinks: as many as make their ranges about as long as the others'.
-int sink_chunks(const b200_attn_t* a) {
-  if (a->window <= 0 || a->sinks <= 0) return 1;
-  const int q_blocks = (a->Sq + BQ - 1) / BQ;
-  const int others = std::min<long long>(q_blocks, (a->window + BK - 2ll) / BQ + 1);
-  return std::max(1, std::min(64, (q_blocks + others - 1) / std::max(1, others)));
+// How the query blocks of the key blocks with sinks are cut.  A chunk is about as long as what the other key blocks meet, but never so
+// short that there were more than four chunks an SM: that is enough to even the units out, and it bounds the scratch by the
+// machine (128 KB a chunk; at most 1776, 222 MB) whatever the lengths and however many sinks.  (Cut by the longest sequence for all: one
+// sequence of 8192 tokens and 199 of under 60 with 8 key heads, window 128, four sinks, took 6.4 GB and 1340
+// us, now 0.1 GB and 655; 16384 tokens, 4 heads, window 128, 4096 sinks: 1.0 GB and 970 us, now 0.1 and 445; 32 heads x 4096, window 64,
+// four sinks: 257 us, now 245.)
+struct SinkPlan {
+  int blocks, chunk, slots;
+};
+SinkPlan sink_plan(const b200_attn_t* a) {
+  SinkPlan s{0, 1, 0};
+  if (a->window <= 0 || a->sinks <= 0 || a->B <= 0 || a->Hkv <= 0 || a->Sq <= 0 || a->Sk <= 0) return s;
+  const bool packed = a->cu_seqlens_q != nullptr;
+  const long long q_blocks = (a->Sq + BQ - 1) / BQ, all = packed ? ((long long)a->total_q + BQ - 1) / BQ : a->B * q_blocks;
+  s.blocks = (std::min(a->sinks, a->Sk) + BK - 1) / BK;
+  const long long others = (a->window + BK - 2ll) / BQ + 1, even = (all * a->Hkv * s.blocks + 4 * kSMs - 1) / (4 * kSMs);
+  s.chunk = (int)std::min(q_blocks, std::max(others, even));
+  if (q_blocks > s.chunk) s.slots = packed ? slots_before(a->total_q, s.chunk) : (int)(a->B * ((q_blocks + s.chunk - 1) / s.chunk));
+  return s;
 }
-int sink_blocks(const b200_attn_t* a) { return a->window > 0 ? (std::min(a->sinks, a->Sk) + BK - 1) / BK : 0; }
 
 }  // namespace
 }  // namespace b200k
@@ -722,8 +760,8 @@ int sink_blocks(const b200_attn_t* a) { return a->window > 0 ? (std::min(a->sink
 using namespace b200k;
 
 extern "C" int64_t b200_flash_attn_bwd_workspace(const b200_attn_t* a) {
-  const int chunks = sink_chunks(a);
-  return chunks > 1 ? (int64_t)a->B * a->Hkv * sink_blocks(a) * chunks * 2 * BK * BD : 0;
+  const SinkPlan s = sink_plan(a);
+  return (int64_t)s.slots * s.blocks * a->Hkv * 2 * BK * BD;
 }
 
 namespace b200k {
@@ -751,13 +789,17 @@ int attn_window_bwd(const b200_attn_t* a, float* dq_accum, void* dk, void* dv, f
   p.window = a->window;
   p.sinks = a->sinks;
   p.total_k = a->total_k;
-  p.sink_blocks = sink_blocks(a);
-  p.sink_chunks = sink_chunks(a);
+  const SinkPlan plan = sink_plan(a);
+  p.sink_blocks = plan.blocks;
+  p.sink_chunk = plan.chunk;
+  p.sink_slots = plan.slots;
   p.sink_ws = a->workspace;
-  if (!a->causal || a->window > (1 << 30) || a->sinks < 0 || (p.sink_chunks > 1 && !p.sink_ws) ||
+  if (!a->causal || a->window > (1 << 30) || a->sinks < 0 || (plan.slots > 0 && !p.sink_ws) ||
       (reinterpret_cast<uintptr_t>(a->remainder) & 15))
     return (int)cudaErrorNotSupported;
-  const long long units = (long long)a->B * a->Hkv * (p.kv_blocks + p.sink_blocks * (p.sink_chunks - 1));
+  // of packed sequences the most there can be: only the grid follows from it, the units that exist are counted on the device
+  const long long units = (long long)a->Hkv * ((long long)a->B * p.kv_blocks + (long long)plan.slots * plan.blocks -
+                                               (p.cu_q || plan.slots == 0 ? 0ll : (long long)a->B * plan.blocks));
   if (units > 2147483647ll - 1024) return (int)cudaErrorNotSupported;
   p.units = (int)units;
   const unsigned grid = (unsigned)std::min<long long>(units, gemm_sm_count());
@@ -769,8 +811,9 @@ int attn_window_bwd(const b200_attn_t* a, float* dq_accum, void* dk, void* dv, f
                                                  a->o_sh, a->o_ss, x[0], x[1], x[2], (const T*)a->remainder);
     kern<<<grid, kBwdThreads, kBwdSmem, stream>>>(m.q, m.k, m.v, m.d_o, m.dq, gk, gv, p);
     note_launch(2);
-    if (p.sink_blocks > 0 && p.sink_chunks > 1) {
-      attn_sink_sum_kernel<T><<<dim3((unsigned)(a->B * a->Hkv * p.sink_blocks * 8), 2), 256, 0, stream>>>(gk, gv, p);
+    if (plan.slots > 0) {
+      const unsigned places = (unsigned)(p.cu_q ? plan.slots : a->B);
+      attn_sink_sum_kernel<T><<<dim3(places * (unsigned)(plan.blocks * a->Hkv * 8), 2), 256, 0, stream>>>(gk, gv, p);
       note_launch();
     }
     return (int)cudaGetLastError();
