@@ -135,6 +135,43 @@ def test_keys_of_later_tokens_do_not_reach_earlier_ones(bw, dev):
     assert not bool(torch.isfinite(got[:, 0]).any()) and bool(torch.isnan(got[:, 3]).all()) and not bool(torch.isfinite(got[:, 2]).any())
 
 
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,H,Hkv,D,window", [(1, 4, 2, 128, None), (1, 4, 4, 64, 300), (4, 8, 2, 64, None), (8, 8, 2, 128, 40), (5, 32, 4, 128, None)])
+def test_an_infinity_that_a_token_sees_comes_out(bw, dev, dt, n, H, Hkv, D, window):
+    """As in the formula: an infinity in a visible value gives an infinity of its sign, both signs or a NaN give NaN, and the other dimensions
+    keep their values.  Among the keys that all tokens see, those that some see, and with a probability of 2^-40, which
+    fp16 holds as zero."""
+    q, k, v, table, lens = case(31, [333, 60], n, H, Hkv, D, 16, dt, window, 2)
+    for b, L in enumerate(lens.tolist()):
+        for j, d, x in ((L - n - 3, 0, INF), (L - n - 20, 1, -INF), (L - n - 4, 2, INF), (L - n - 19, 2, -INF), (L - 1, 3, INF), (1, 4, -INF), (L - n, 5, NAN)):
+            v[table[b, j // 16], :, j % 16, d::16] = x
+    faint = int(lens[0]) - n - 9            # its score is -28, the others' are a few
+    q[0, :, :, 0], k[..., 0] = 8, 0
+    k[table[0, faint // 16], :, faint % 16] = 0
+    k[table[0, faint // 16], :, faint % 16, 0] = -3.5 * math.sqrt(D)
+    v[table[0, faint // 16], :, faint % 16, 6::16] = INF
+    out = paged_attention(*(t.to(dev) for t in (q, k, v, table, lens)), window=window, sinks=2).double().cpu()
+    bw.synchronize()
+    value, bound = want_attention(q, k, v, table, lens, window, 2)
+    odd = ~torch.isfinite(value)
+    assert bool(odd[..., 6::16][0].all()) and bool(torch.isinf(value[..., 0::16]).all()) and bool(torch.isnan(value[..., 2::16]).all())
+    assert torch.equal(torch.isnan(out), torch.isnan(value)) and torch.equal(out[torch.isinf(value)], value[torch.isinf(value)])
+    check(out[~odd], value[~odd], bound[~odd])
+
+
+def test_an_infinity_in_a_very_long_sequence(bw, dev):
+    """Where several clusters share the keys and a second kernel joins their parts."""
+    q, k, v, table, lens = case(32, [20000], 2, 4, 1, 64, 64, torch.float16)
+    for j, d, x in ((3, 0, INF), (19000, 1, -INF), (700, 2, INF), (15000, 2, -INF), (12345, 3, NAN), (19999, 4, INF)):
+        v[table[0, j // 64], :, j % 64, d] = x
+    out = paged_attention(*(t.to(dev) for t in (q, k, v, table, lens))).cpu().double()
+    value, bound = want_attention(q, k, v, table, lens)
+    odd = ~torch.isfinite(value)
+    assert int(odd.sum()) == 4 * (4 + 5) and torch.equal(out[torch.isinf(value)], value[torch.isinf(value)])
+    assert torch.equal(torch.isnan(out), torch.isnan(value))
+    check(out[~odd], value[~odd], bound[~odd])
+
+
 def test_strides_scale_and_slices(bw, dev):
     q, k, v, table, lens = case(3, [130, 47], 2, 4, 2, 128, 32, torch.float16)
     want = paged_attention(*(t.to(dev) for t in (q, k, v, table, lens)), softmax_scale=0.2)

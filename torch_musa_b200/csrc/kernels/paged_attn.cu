@@ -127,6 +127,47 @@ __device__ __forceinline__ bool not_finite(uint32_t w) {
   return (w & e) == e || (w & (e << 16)) == (e << 16);
 }
 
+// The sums of an output that are NaN although no score is: an infinity met a probability that 16 bits hold as zero, or the remainder of one,
+// which may be zero or negative.  What the softmax gives follows from the values that the token sees alone, its probabilities are
+// positive: an infinity for those of one sign, NaN where there are both signs or a NaN.  v: four dimensions of the key head's pool.
+// With finite values nobody comes here.  What its being there costs is the compiler's choice of registers: 16 sequences with 20 rows a key
+// head, D 64, 15.0 us where it was 14.5; four rows or D 128 within 1 % (a second pass over the keys by the warp that
+// found a NaN: 2 to 9 %).
+template <typename T>
+__device__ __noinline__ float4 settle_infinities(float4 sums, const T* vp, const PagedParams& p, int b, int hk, int i, int d) {
+  const int pos = min(max(__ldg(p.lens + b), 0), p.table_width * p.page_size) - p.n + i, from = p.window > 0 ? max(0, pos - p.window + 1) : 0;
+  const int* table = p.table + b * p.table_sb;
+  const T* v = vp + hk * p.v_sh + d;
+  constexpr uint32_t kExp = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+  uint32_t found[4] = {};              // 1: +inf, 2: -inf, 4: NaN
+  for (int k0 = 0; k0 <= pos; k0 += kPageRows) {
+    if (k0 + kPageRows <= from && k0 >= p.sinks) continue;
+    const int index = p.by_page(k0), page = __ldg(table + index);
+    if ((unsigned)page >= (unsigned)p.num_pages) continue;
+    const T* rows = v + page * p.v_sp + (k0 - index * p.page_size) * p.v_sr;
+    for (int r = 0; r < kPageRows; ++r) {
+      const int j = k0 + r;
+      if (j > pos || (j < from && j >= p.sinks)) continue;
+      const uint2 w = *reinterpret_cast<const uint2*>(rows + r * p.v_sr);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t x = ((e < 2 ? w.x : w.y) >> (e & 1) * 16) & 0xffffu;
+        if ((x & kExp) == kExp) found[e] |= (x & 0x7fffu) != kExp ? 4u : (x >> 15 ? 2u : 1u);
+      }
+    }
+  }
+  float o[4] = {sums.x, sums.y, sums.z, sums.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (o[e] != o[e] && (found[e] == 1u || found[e] == 2u)) o[e] = found[e] == 1u ? INFINITY : -INFINITY;
+  return make_float4(o[0], o[1], o[2], o[3]);
+}
+// whether settle_infinities has to be asked
+__device__ __forceinline__ bool unsettled(const float (&v)[4], float sum) {
+  const float any = (v[0] + v[1]) + (v[2] + v[3]);        // NaN where one is (or infinities of both signs: asked in vain)
+  return any != any && sum == sum;
+}
+
 // One CTA: one row group (up to 8 * NT rows = new tokens x query heads of a key head) of one (sequence, key head), one of several
 // contiguous shares of the visible keys.  A share is cut into steps of 16 keys (32 when D is 64 and the rows few) that the four warps take in turn;
 // each warp runs its own online softmax, the warps join through shared memory and the CTAs of a cluster through distributed shared
@@ -151,7 +192,7 @@ __device__ __forceinline__ bool not_finite(uint32_t w) {
 // away from the page's.
 template <typename T, int D, int NT, bool kDense>
 __global__ void __launch_bounds__(kPagedWarps * 32, NT * D <= 256 ? 3 : 2)
-paged_attn_kernel(T* __restrict__ out, const T* __restrict__ q, const T* __restrict__ kp, const T* __restrict__ vp, const PagedParams p) {
+paged_attn_kernel(T* __restrict__ out, const T* __restrict__ q, const T* __restrict__ kp, const T* __restrict__ vp, const __grid_constant__ PagedParams p) {
   constexpr int kRows = 8 * NT, kHalves = D == 64 && NT <= 2 ? 2 : 1, kKeys = kHalves * kPageRows, kHalf = kPageRows * D * 2;
   constexpr int kStageBytes = 2 * kHalves * kHalf, kStages = kWarpRing / kStageBytes;
   constexpr int kPad = D + 4;            // floats of a row of a part: the four lanes' rows then lie in different banks
@@ -493,7 +534,7 @@ paged_attn_kernel(T* __restrict__ out, const T* __restrict__ q, const T* __restr
       }
     }
   __syncthreads();
-  auto store = [&](int r, int d, const float (&v)[4], float sum, float top) {
+  auto store = [&](int r, int d, float (&v)[4], float sum, float top) {
     if (p.outer > 1) {
       float* dst = p.parts + ((((int64_t)b * p.Hkv + hk) * rows_all + r0 + r) * p.outer + outer) * (D + 4);
       *reinterpret_cast<float4*>(dst + d) = make_float4(v[0], v[1], v[2], v[3]);
@@ -501,10 +542,14 @@ paged_attn_kernel(T* __restrict__ out, const T* __restrict__ q, const T* __restr
       return;
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;       // no key: zeros
+    const int i = p.by_heads(r0 + r), h = hk * G + r0 + r - i * G;
+    if (unsettled(v, sum)) {
+      const float4 x = settle_infinities<T>(make_float4(v[0], v[1], v[2], v[3]), vp, p, b, hk, i, d);
+      v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+    }
     T o4[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) o4[e] = ToF<T>::from(sum == 0.f ? 0.f : v[e] * inv);
-    const int i = p.by_heads(r0 + r), h = hk * G + r0 + r - i * G;
     *reinterpret_cast<uint2*>(out + (((int64_t)b * p.n + i) * p.H + h) * D + d) = *reinterpret_cast<const uint2*>(o4);
   };
   for (int x = threadIdx.x; x < rows * (D / 4); x += kPagedWarps * 32) {       // the CTA's sum, over warp 0's part
@@ -516,7 +561,7 @@ paged_attn_kernel(T* __restrict__ out, const T* __restrict__ q, const T* __restr
       v.x += y.x; v.y += y.y; v.z += y.z; v.w += y.w;
     }
     if (split == 1) {
-      const float v4[4] = {v.x, v.y, v.z, v.w};
+      float v4[4] = {v.x, v.y, v.z, v.w};
       store(r, d, v4, s_sum[r], s_top[r]);
     } else {
       *reinterpret_cast<float4*>(part + r * kPad + d) = v;
@@ -566,7 +611,7 @@ paged_attn_kernel(T* __restrict__ out, const T* __restrict__ q, const T* __restr
 
 // Joins the clusters' parts of a row: a thread owns four dimensions of one row.
 template <typename T, int D>
-__global__ void __launch_bounds__(128) paged_join_kernel(T* __restrict__ out, const PagedParams p) {
+__global__ void __launch_bounds__(128) paged_join_kernel(T* __restrict__ out, const T* __restrict__ vp, const __grid_constant__ PagedParams p) {
   const int G = p.H / p.Hkv, rows_all = p.n * G;
   const int64_t x = (int64_t)blockIdx.x * 128 + threadIdx.x, row = x / (D / 4);
   if (row >= (int64_t)p.B * p.Hkv * rows_all) return;
@@ -582,7 +627,11 @@ __global__ void __launch_bounds__(128) paged_join_kernel(T* __restrict__ out, co
     v[0] += y.x * f; v[1] += y.y * f; v[2] += y.z * f; v[3] += y.w * f;
   }
   const int64_t unit = row / rows_all;
-  const int r = (int)(row - unit * rows_all), i = p.by_heads(r), h = (int)(unit % p.Hkv) * G + r - i * G;
+  const int r = (int)(row - unit * rows_all), i = p.by_heads(r), hk = (int)(unit % p.Hkv), h = hk * G + r - i * G;
+  if (unsettled(v, sum)) {
+    const float4 x = settle_infinities<T>(make_float4(v[0], v[1], v[2], v[3]), vp, p, (int)(unit / p.Hkv), hk, i, d);
+    v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+  }
   T o4[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) o4[e] = ToF<T>::from(sum == 0.f ? 0.f : v[e] / sum);
@@ -737,7 +786,7 @@ int launch_paged(const PagedPlan& plan, void* out, const void* q, const void* kp
   note_launch();
   if (plan.outer == 1) return 0;
   const long long threads = (long long)p.B * p.Hkv * p.n * (p.H / p.Hkv) * (D / 4);
-  paged_join_kernel<T, D><<<(unsigned)((threads + 127) / 128), 128, 0, stream>>>((T*)out, p);
+  paged_join_kernel<T, D><<<(unsigned)((threads + 127) / 128), 128, 0, stream>>>((T*)out, (const T*)vp, p);
   B200K_LAUNCH_RET();
 }
 
