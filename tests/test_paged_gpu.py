@@ -121,6 +121,21 @@ def test_other_types_and_head_sizes_take_the_plain_way(bw, dev):
         assert float((a.cpu() - b).abs().max()) <= 2.0 ** -20      # products of values below 4, each side rounded in 32 bits
 
 
+def test_infinities_the_plain_way(bw, dev):
+    """fp32, several tokens at once: the same pattern of infinities and NaN as off the device."""
+    q, k, v, table, lens = case(22, [40, 23], 3, 4, 2, 64, 16, torch.float32, 9, 1)
+    hidden = torch.isinf(v)
+    for b, L in enumerate(lens.tolist()):
+        for j, d, x in ((L - 1, 0, INF), (L - 11, 1, -INF), (L - 3, 2, NAN), (L - 3, 3, INF), (L - 1, 3, -INF)):
+            v[table[b, j // 16], :, j % 16, d] = x
+    out = paged_attention(*(t.to(dev) for t in (q, k, v, table, lens)), window=9, sinks=1).cpu()
+    there = table.clamp(0, k.shape[0] - 1)           # off the device an entry that nobody asks for may be anything, too
+    want = paged_attention(q, k, v, there, lens, window=9, sinks=1)
+    odd = ~torch.isfinite(want)
+    assert bool(hidden.any()) and bool(odd.any()) and torch.equal(out[odd].nan_to_num(7.0), want[odd].nan_to_num(7.0))
+    assert float((out[~odd] - want[~odd]).abs().max()) <= 2.0 ** -18     # sums of at most 40 products of values below 8, in 32 bits on either side
+
+
 def test_keys_of_later_tokens_do_not_reach_earlier_ones(bw, dev):
     """n tokens at once with infinities and NaN in the newest keys and values, and in those that only the oldest token still sees."""
     n, window = 4, 50

@@ -102,6 +102,29 @@ def test_paged_attention_reads_only_what_is_seen():
     assert bool((ops.paged_attention(q, kp, vp, table[:, :0], lens * 0) == 0).all())
 
 
+@pytest.mark.parametrize("n,window", [(1, None), (3, None), (4, 6)])
+def test_infinities_reach_the_tokens_that_see_them(n, window):
+    """An infinity or NaN in the newest values and in those that only the oldest token still sees: other tokens are as without it, the
+    ones that see it get what the loop's softmax gives."""
+    q, kp, vp, table, lens = paged_case(5, [50, 20], n)
+    clean = ops.paged_attention(q, kp, vp, table, lens, window)
+    for b, L in enumerate(lens.tolist()):
+        oldest = 0 if window is None else L - n - window + 1
+        for j, d, x in ((L - 1, 0, math.inf), (L - 1, 1, math.nan), (oldest, 2, -math.inf), (L - n, 3, math.inf), (L - n, 4, -math.inf), (oldest, 4, math.inf)):
+            vp[table[b, j // 16], :, j % 16, d] = x
+    out = ops.paged_attention(q, kp, vp, table, lens, window)
+    for b, L in enumerate(lens.tolist()):
+        number, row = table[b].long()[torch.arange(L) // 16], torch.arange(L) % 16
+        pos, j = L - n + torch.arange(n)[:, None], torch.arange(L)[None]
+        seen = j <= pos if window is None else (j <= pos) & (pos - j < window)
+        for h in range(4):
+            want = loop_attention(q[b, :, h], kp[number, h // 2, row], vp[number, h // 2, row], seen)
+            odd = ~torch.isfinite(want)
+            assert torch.equal(out[b, :, h].double()[odd].nan_to_num(7.0), want[odd].nan_to_num(7.0)) and int(odd.sum()) >= 4
+            assert torch.allclose(out[b, :, h].double()[~odd], want[~odd], rtol=0, atol=64 * U * 8)
+    assert n == 1 or torch.equal(out[:, 0, :, 0], clean[:, 0, :, 0])          # the first token does not see the last key
+
+
 @pytest.mark.parametrize("packed", [False, True])
 def test_paged_rope_cache(packed):
     lens, news = [20, 3, 0, 17], [3, 3, 3, 3] if not packed else [4, 3, 0, 1]

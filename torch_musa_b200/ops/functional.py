@@ -575,7 +575,15 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     x = x.masked_fill(~seen, float("-inf"))
     top = x.amax(-1, keepdim=True)
     x = torch.exp(x - top.masked_fill(top == float("-inf"), 0))
-    out = (x @ rows(v_pages)) / x.sum(-1, keepdim=True).clamp_min(torch.finfo(torch.float32).tiny)
+    v = rows(v_pages)
+    odd = ~torch.isfinite(v)
+    if n == 1 or (not _on_device(q) and not bool(odd.any())):
+        out = x @ v
+    else:            # an infinity or NaN reaches the tokens that see it and no others: zero times it would be NaN
+        weight = (x > 0).float()
+        high, low, nan = (weight @ t.float() > 0 for t in (v == math.inf, v == -math.inf, v != v))
+        out = (x @ v.masked_fill(odd, 0)).masked_fill(high, math.inf).masked_fill(low, -math.inf).masked_fill(nan | (high & low), math.nan)
+    out = out / x.sum(-1, keepdim=True).clamp_min(torch.finfo(torch.float32).tiny)
     return out.permute(0, 3, 1, 2, 4).reshape(B, n, H, D).to(q.dtype)
 
 
