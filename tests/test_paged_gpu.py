@@ -439,6 +439,17 @@ def test_verify_drafts(bw, dev, dt, B, n, V, drafts):
     assert torch.equal(got[0].cpu(), want[0]) and torch.equal(got[1].cpu(), want[1])
 
 
+@pytest.mark.parametrize("V", [5, 700, 32000])
+def test_random_numbers_outside_their_range(bw, dev, V):
+    """Each draws a token: what is below zero or NaN counts as zero, from one on it is the last token with weight."""
+    us = [-1.0, -INF, NAN, -0.0, 0.0, 1.0, 7.0, INF]
+    p = torch.rand(1, 1, V, generator=torch.Generator().manual_seed(V))
+    p[..., 0] = p[..., -1] = 0
+    args = p.expand(len(us), 1, V).contiguous(), torch.zeros(len(us), 0, dtype=torch.long), torch.tensor(us)[:, None]
+    got, want = verify_drafts(*(t.to(dev) for t in args)), verify_drafts(*args)
+    assert got[1].flatten().tolist() == want[1].flatten().tolist() == [1] * 5 + [V - 2] * 3 and not got[0].any()
+
+
 def test_verify_drafts_edges(bw, dev):
     """Random numbers of 0 and just below 1, rows without weight, NaN, views."""
     top = 1 - 2.0 ** -24

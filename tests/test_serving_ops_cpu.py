@@ -214,6 +214,13 @@ def test_verify_drafts_where_nothing_is_left():
         ops.verify_drafts(p, torch.tensor([[0, 1]]), torch.zeros(1, 2))
 
 
+def test_random_numbers_outside_their_range():
+    """Below zero or NaN: as zero, and never a token without weight.  From one on: the last token with weight."""
+    p = torch.tensor([[[0.0, 0.25, 0.5, 0.25, 0.0]]])
+    for u, token in ((-1.0, 1), (-math.inf, 1), (math.nan, 1), (0.0, 1), (1 - 2 ** -24, 3), (1.0, 3), (7.0, 3), (math.inf, 3)):
+        assert ops.verify_drafts(p, torch.zeros(1, 0, dtype=torch.long), torch.tensor([[u]]))[1].tolist() == [[token]], u
+
+
 def test_verified_drafts_follow_the_target():
     """On a grid of random numbers the outcomes have exactly the target's probabilities (to the grid's step)."""
     p, q = torch.tensor([0.5, 0.25, 0.25]), torch.tensor([0.25, 0.5, 0.25])

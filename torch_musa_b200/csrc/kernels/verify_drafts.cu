@@ -3,8 +3,9 @@
 // Drafted token x_i (i < n) with draft probability q_i(x_i) is taken while u_i q_i(x_i) < p_i(x_i), u_i given in [0, 1); a
 // draft without probabilities counts as certain (q = 1 at its token, 0 elsewhere).  At the first refusal r one token is drawn
 // from the residual max(p_r - q_r, 0), after n taken drafts from p_n: the smallest j whose running sum of weights exceeds
-// u_n times their total.  The products of two inputs are exact in 64 bits and the sums are held there, so that the outcome does
-// not depend on how the vocabulary is split.
+// u_n times their total (u_n below zero or NaN counts as zero; from one on, the last j with a weight).  Products of two inputs are
+// exact in 64 bits and the sums are held there.  Their order follows the split of the vocabulary, so the outcome depends on it where
+// the limit lies within the sums' rounding, 2^-53 of the total for each addition, of a running sum.
 //
 // One cluster per sequence.  Every CTA of it finds r by itself (n small loads) and adds up its contiguous share of the row, a
 // contiguous piece per warp; the pieces' sums cross the cluster through distributed shared memory, and the one warp in whose piece
@@ -62,7 +63,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_drafts_kernel(int64_t* 
   const int64_t x = r < p.n ? tok[r] : -1;
   const bool refused = x >= 0 && x < p.V;       // otherwise the draft ends here: the target's own distribution
   const T* qrow = refused && draft ? draft + b * p.q_sb + r * p.q_sn : nullptr;
-  const double un = (double)u[p.n];
+  const double un = u[p.n] > 0.f ? (double)u[p.n] : 0.0;       // below zero or NaN: zero, so that some piece always has the limit
   // this warp's piece of the row, a whole number of its loads long
   const int pieces = p.split * kVerifyWarps, piece = rank * kVerifyWarps + warp;
   const int per = ((p.V + pieces - 1) / pieces + kStep - 1) / kStep * kStep;

@@ -596,7 +596,8 @@ def verify_drafts(target_probs: torch.Tensor, draft_tokens: torch.Tensor, unifor
     ``uniforms`` float32 [B, n + 1] in [0, 1), ``draft_probs`` [B, n, V] or None for drafts that were certain (a greedy
     draft).  Draft i is taken while ``uniforms[i] * draft_probs[i, x_i] < target_probs[i, x_i]``; at the first refusal r one
     token is drawn from ``max(target_probs[r] - draft_probs[r], 0)``, after n taken drafts from ``target_probs[n]``: the first
-    token at which the running sum exceeds ``uniforms[n]`` times the whole.  A draft outside the vocabulary (-1, say) ends a
+    token at which the running sum exceeds ``uniforms[n]`` times the whole (a number below zero or NaN counts as zero there, from one on
+    it is the last token that has weight).  A draft outside the vocabulary (-1, say) ends a
     sequence's draft early: the token there is drawn from the target's row.  Sums are held in 64 bits.
 
     Returns ``(taken [B], tokens [B, n + 1])``, both int64: the taken drafts, the drawn token, then -1.  Where a row has no
@@ -623,7 +624,9 @@ def verify_drafts(target_probs: torch.Tensor, draft_tokens: torch.Tensor, unifor
         w = torch.where(refused[:, None], less, w)
     w = torch.where(w > 0, w, 0.0)
     total = w.cumsum(1)
-    token = (total > u[:, n:] * total[:, -1:]).long().argmax(1)
+    past = (w > 0) & (total > torch.where(u[:, n:] > 0, u[:, n:], 0.0) * total[:, -1:])
+    last = ((w > 0) * torch.arange(V, device=x.device)).amax(1)
+    token = torch.where(past.any(1), past.long().argmax(1), last)
     token = torch.where(total[:, -1] > 0, token, -1)
     i = torch.arange(n1, device=x.device)
     drafts = torch.cat((x, x.new_full((B, 1), -1)), 1)
