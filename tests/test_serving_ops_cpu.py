@@ -221,6 +221,16 @@ def test_random_numbers_outside_their_range():
         assert ops.verify_drafts(p, torch.zeros(1, 0, dtype=torch.long), torch.tensor([[u]]))[1].tolist() == [[token]], u
 
 
+@pytest.mark.parametrize("tokens,uniforms,draft", [(torch.int32, torch.float32, torch.float32), (torch.long, torch.float64, torch.float32),
+                                                   (torch.long, torch.float32, torch.bfloat16)])
+def test_verify_drafts_refuses_other_types(tokens, uniforms, draft):
+    """The same calls as on the device."""
+    p, x, u, q = verify_case(1, 2, 3, 11)
+    ops.verify_drafts(p, x, u, q)
+    with pytest.raises(RuntimeError, match="must be"):
+        ops.verify_drafts(p, x.to(tokens), u.to(uniforms), q.to(draft))
+
+
 def test_verified_drafts_follow_the_target():
     """On a grid of random numbers the outcomes have exactly the target's probabilities (to the grid's step)."""
     p, q = torch.tensor([0.5, 0.25, 0.25]), torch.tensor([0.25, 0.5, 0.25])

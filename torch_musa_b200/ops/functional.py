@@ -593,7 +593,7 @@ def verify_drafts(target_probs: torch.Tensor, draft_tokens: torch.Tensor, unifor
     distributed as if it were sampled from the target alone.
 
     ``target_probs`` [B, n + 1, V] (the rows for the n drafted tokens and the one after them), ``draft_tokens`` int64 [B, n],
-    ``uniforms`` float32 [B, n + 1] in [0, 1), ``draft_probs`` [B, n, V] or None for drafts that were certain (a greedy
+    ``uniforms`` float32 [B, n + 1] in [0, 1), ``draft_probs`` [B, n, V] in the type of ``target_probs`` or None for drafts that were certain (a greedy
     draft).  Draft i is taken while ``uniforms[i] * draft_probs[i, x_i] < target_probs[i, x_i]``; at the first refusal r one
     token is drawn from ``max(target_probs[r] - draft_probs[r], 0)``, after n taken drafts from ``target_probs[n]``: the first
     token at which the running sum exceeds ``uniforms[n]`` times the whole (a number below zero or NaN counts as zero there, from one on
@@ -609,6 +609,8 @@ def verify_drafts(target_probs: torch.Tensor, draft_tokens: torch.Tensor, unifor
     n, x, u = n1 - 1, draft_tokens, uniforms.double()
     if tuple(x.shape) != (B, n) or tuple(u.shape) != (B, n1) or (draft_probs is not None and tuple(draft_probs.shape) != (B, n, V)):
         raise RuntimeError("verify_drafts: draft_tokens [B, n], uniforms [B, n + 1] and draft_probs [B, n, V] expected")
+    if x.dtype != torch.long or uniforms.dtype != torch.float32 or (draft_probs is not None and draft_probs.dtype != target_probs.dtype):
+        raise RuntimeError("verify_drafts: draft_tokens must be int64, uniforms float32 and draft_probs of target_probs' type")
     known = (x >= 0) & (x < V)
     at = x.clamp(0, V - 1)[..., None]
     p = target_probs[:, :n].gather(2, at).squeeze(2).double()
