@@ -535,3 +535,19 @@ def test_decoder_captured_step_and_checked_drafts(bw, dev, window, sinks):
     went_in = c.step()
     assert all(int(went_in[s]) == int(out[s, taken[s]]) for s in range(3)) and full
     bw.synchronize()
+
+
+def test_decoder_is_unchanged_by_drafts_that_are_refused(bw, dev):
+    from torch_musa_b200.models import Llama, LlamaConfig, PagedLlamaDecoder
+
+    cfg = LlamaConfig(vocab_size=64, dim=256, n_layers=1, n_heads=4, n_kv_heads=2, ffn_dim=256, max_seq_len=64)
+    torch.manual_seed(0)
+    d = PagedLlamaDecoder(Llama(cfg).to(torch.bfloat16).eval().to(dev), sequences=2, pages=6, page_size=16, device=dev)
+    d.add([torch.arange(15)])
+    drafts, uniforms = torch.zeros(2, 2, dtype=torch.long, device=dev), torch.zeros(2, 3, device=dev)
+    for bad in ((drafts.int(), uniforms), (drafts.cpu(), uniforms), (drafts, uniforms.cpu()), (drafts, uniforms, torch.zeros(2, 2, 64))):
+        with pytest.raises(ValueError):
+            d.check(*bad)
+        assert d.seq_lens.tolist() == [15, 0] and d.lens == [15, None] and len(d.free) == 5
+    taken, _ = d.check(drafts, uniforms)
+    assert d.seq_lens.tolist() == [16 + int(taken[0]), 0] and d.lens == [16 + int(taken[0]), None]

@@ -368,3 +368,42 @@ def test_scratch_of_the_windowed_backward_is_bounded(Hkv, sinks):
     assert floats(5, 128, 1) == 0 and floats(3, 100, 1, 300) == 0         # one block of queries is not cut
     if sinks <= 128 and Hkv < 32:
         assert floats(1, 4096, 64) >= 4 * Hkv * pair                        # long ranges of few blocks are
+
+
+@pytest.mark.parametrize("call,where", [("step", "first layer"), ("step", "head"), ("check", "first layer"), ("check", "head"), ("check", "verification")])
+def test_paged_decoder_after_a_step_that_failed_halfway(monkeypatch, call, where):
+    """The model or the verification raises when the lengths are already raised: lengths, pages and tokens are as before, and the next call
+    goes on as if nothing had been."""
+    model = Llama(llama_tiny_config(vocab_size=61)).eval()
+    prompts = [torch.arange(15), torch.arange(16), torch.arange(3)]
+    dec, other = (PagedLlamaDecoder(model, sequences=4, pages=9, page_size=16, max_len=48) for _ in range(2))
+    dec.add(prompts), other.add(prompts)
+    args = () if call == "step" else (torch.full((4, 2), 5), torch.full((4, 3), 0.5))
+    before = dec.seq_lens.tolist(), list(dec.lens), sorted(dec.free), dec.tokens.tolist(), [dict(p) for p in dec._pages]
+
+    def fails(*_args, **_kw):
+        raise RuntimeError("out of memory, say")
+
+    with monkeypatch.context() as m:
+        if where == "verification":
+            m.setattr("torch_musa_b200.models.paged_decode.BF.verify_drafts", fails)
+        else:
+            m.setattr(model.layers[0].ffn if where == "first layer" else model.lm_head, "forward", fails)
+        with pytest.raises(RuntimeError, match="say"):
+            getattr(dec, call)(*args)
+    assert (dec.seq_lens.tolist(), list(dec.lens), sorted(dec.free), dec.tokens.tolist(), [dict(p) for p in dec._pages]) == before
+    for _ in range(3):
+        a, b = getattr(dec, call)(*args), getattr(other, call)(*args)
+        for x, y in ((a, b),) if call == "step" else zip(a, b):
+            assert torch.equal(x[:3], y[:3])
+        assert torch.equal(dec.tokens[:3], other.tokens[:3]) and dec.lens == other.lens == [n or None for n in dec.seq_lens.tolist()]
+
+
+def test_paged_decoder_refuses_drafts_of_another_type():
+    dec = PagedLlamaDecoder(Llama(llama_tiny_config(vocab_size=61)).eval(), sequences=1, pages=4, page_size=16, max_len=48)
+    dec.add([torch.arange(4)])
+    with pytest.raises(ValueError, match="int64"):
+        dec.check(torch.zeros(1, 2, dtype=torch.int32), torch.zeros(1, 3))
+    with pytest.raises(ValueError, match="the decoder is on cpu"):
+        dec.check(torch.zeros(1, 2, dtype=torch.long), torch.zeros(1, 3, device="meta"))
+    assert dec.seq_lens.tolist() == dec.lens == [4] and len(dec.free) == 3

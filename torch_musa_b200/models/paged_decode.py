@@ -44,8 +44,9 @@ class PagedLlamaDecoder:
         self._graph = None
 
     # ------------------------------------------------------------------ pages
-    def _reserve(self, slots: Sequence[int], new: int) -> None:
-        """Pages for ``new`` more tokens of each slot; pages that no later token can see go back to the pool."""
+    def _reserve(self, slots: Sequence[int], new: int) -> List[Tuple[int, int]]:
+        """Pages for ``new`` more tokens of each slot; pages that no later token can see go back to the pool.  Returns what
+        ``_give_up`` takes back."""
         size, changed = self.page_size, False
         wanted = []
         for b in slots:
@@ -66,6 +67,13 @@ class PagedLlamaDecoder:
             changed = True
         if changed:
             self.block_table.copy_(self._table)
+        return wanted
+
+    def _give_up(self, reserved: Sequence[Tuple[int, int]]) -> None:
+        """After a step that failed: its new pages are free again, the device's lengths are the host's."""
+        for b, i in reserved:
+            self.free.append(self._pages[b].pop(i))
+        self.seq_lens.copy_(torch.tensor([n or 0 for n in self.lens], dtype=torch.int32))
 
     def remove(self, slot: int) -> None:
         """Ends the sequence in ``slot``: its pages and the slot are free again."""
@@ -161,12 +169,16 @@ class PagedLlamaDecoder:
     def step(self) -> torch.Tensor:
         """Decodes one greedy token for every slot in use; returns the tokens that went into the cache, [B] (a copy)."""
         used = [b for b in range(self.B) if self.lens[b] is not None]
-        self._reserve(used, 1)
+        reserved = self._reserve(used, 1)
         went_in = self.tokens[:, 0].clone()
-        if self._graph is not None:
-            self._graph.replay()
-        else:
-            self._step()
+        try:
+            if self._graph is not None:
+                self._graph.replay()
+            else:
+                self._step()
+        except Exception:
+            self._give_up(reserved)
+            raise
         for b in used:
             self.lens[b] += 1
         return went_in
@@ -175,25 +187,35 @@ class PagedLlamaDecoder:
     def check(self, drafts: torch.Tensor, uniforms: torch.Tensor, draft_probs: Optional[torch.Tensor] = None,
               temperature: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor]:
         """Verifies ``drafts`` [B, n] (what a draft model proposes after ``tokens``) in one pass over n + 1 tokens per slot, as
-        ``ops.verify_drafts`` does with the model's probabilities at ``temperature``.  The caches keep the taken tokens only,
-        ``tokens`` becomes the drawn ones.  Returns (taken [B], tokens [B, n + 1]); rows of slots not in use mean nothing."""
+        ``ops.verify_drafts`` does with the model's probabilities (float32) at ``temperature``: ``drafts`` are int64, ``uniforms`` and
+        ``draft_probs`` float32, all on the decoder's device.  The caches keep the taken tokens only, ``tokens`` becomes the drawn
+        ones.  Returns (taken [B], tokens [B, n + 1]); rows of slots not in use mean nothing.  A call that fails changes nothing."""
         if temperature <= 0:
             raise ValueError(f"temperature must be positive, got {temperature}")
         n = drafts.shape[-1]
-        if (tuple(drafts.shape) != (self.B, n) or tuple(uniforms.shape) != (self.B, n + 1) or uniforms.dtype != torch.float32
+        if (tuple(drafts.shape) != (self.B, n) or drafts.dtype != torch.long
+                or tuple(uniforms.shape) != (self.B, n + 1) or uniforms.dtype != torch.float32
                 or (draft_probs is not None and (tuple(draft_probs.shape) != (self.B, n, self.cfg.vocab_size)
                                                  or draft_probs.dtype != torch.float32))):
-            raise ValueError("drafts [sequences, n], float32 uniforms [sequences, n + 1] and float32 draft_probs "
+            raise ValueError("int64 drafts [sequences, n], float32 uniforms [sequences, n + 1] and float32 draft_probs "
                              "[sequences, n, vocabulary] expected")
+        for t in (drafts, uniforms, draft_probs):
+            if t is not None and t.device != self.seq_lens.device:
+                raise ValueError(f"the decoder is on {self.seq_lens.device}, an argument on {t.device}")
         used = [b for b in range(self.B) if self.lens[b] is not None]
-        self._reserve(used, n + 1)
-        self.seq_lens.add_(self.active * (n + 1))
-        inputs = torch.cat((self.tokens, drafts.clamp(0, self.cfg.vocab_size - 1)), 1)
-        logits = self.model.lm_head(self._new_tokens(inputs)).float()
-        taken, out = BF.verify_drafts(torch.softmax(logits / temperature, -1), drafts, uniforms, draft_probs)
-        self.seq_lens.sub_(self.active * (n - taken).to(torch.int32))
-        self.tokens.copy_(out.gather(1, taken[:, None]).clamp_min(0))
-        for b, t in zip(range(self.B), taken.tolist()):
+        reserved = self._reserve(used, n + 1)
+        try:
+            self.seq_lens.add_(self.active * (n + 1))
+            inputs = torch.cat((self.tokens, drafts.clamp(0, self.cfg.vocab_size - 1)), 1)
+            logits = self.model.lm_head(self._new_tokens(inputs)).float()
+            taken, out = BF.verify_drafts(torch.softmax(logits / temperature, -1), drafts, uniforms, draft_probs)
+            drawn, counts = out.gather(1, taken[:, None]).clamp_min(0), taken.tolist()
+            self.seq_lens.sub_(self.active * (n - taken).to(torch.int32))
+        except Exception:
+            self._give_up(reserved)
+            raise
+        self.tokens.copy_(drawn)
+        for b, t in enumerate(counts):
             if self.lens[b] is not None:
                 self.lens[b] += t + 1
         return taken, out
