@@ -478,3 +478,39 @@ def test_scratch_does_not_grow_with_the_number_of_sequences(bw, dev):
     bw.synchronize()
     results = 2 * D * n * (H + 2 * Hkv) + 4 * D * n * H + 4 * n * H          # gradients, dq and the row dots in 32 bits
     assert bw.max_memory_allocated() - before <= results + 1776 * 2 * 4 * 128 * 128
+
+
+@pytest.mark.parametrize("sinks", [0, 2])
+@pytest.mark.parametrize("which", ["q", "k", "v", "do"])
+def test_reach_of_what_is_not_finite_within_a_sequence(bw, dev, which, sinks):
+    """A NaN at place 300, block 2 of a sequence of eight blocks, window 4.  Queries of blocks 2 and 3 see keys of block 2, and queries of
+    block 2 see keys of blocks 1 and 2 (and the sinks' block 0): nothing else changes.  (dq is a sum of at most three blocks in any order,
+    as in the test of two sequences above.)"""
+    from torch_musa_b200.ops import window_attention
+
+    S, H, at, dt = 1000, 2, 300, torch.bfloat16
+    clean = dict(zip(("q", "k", "v", "do"), inputs(dt, (1, S, H, D), (1, S, H, D), 51)))
+    dirty = {n: t.clone() for n, t in clean.items()}
+    dirty[which][0, at] = math.nan
+
+    def run(x):
+        leaves = [x[n].to(dev).requires_grad_() for n in ("q", "k", "v")]
+        o = window_attention(*leaves, 4, sinks)
+        return dict(zip(("o", "dq", "dk", "dv"), (t.detach().cpu()[0].float() for t in (o, *torch.autograd.grad(o, leaves, x["do"].to(dev))))))
+
+    want, got = run(clean), run(dirty)
+    place = torch.arange(S) // 128
+    by_key = {"o": (place == 2) | (place == 3), "dq": (place == 2) | (place == 3), "dk": place == 2, "dv": place == 2}
+    by_query = {"o": place == 2, "dq": place == 2, "dk": (place == 1) | (place == 2) | ((place == 0) & (sinks > 0)),
+                "dv": (place == 1) | (place == 2) | ((place == 0) & (sinks > 0))}
+    for n in want:
+        rows = (by_key if which in ("k", "v") else by_query)[n].clone()
+        if n in ("dk", "dv") and which in ("k", "v"):      # a query that has become NaN reaches the keys of its own blocks
+            rows |= by_query[n] | (place == 3)
+        a, b = want[n][~rows], got[n][~rows]
+        if n == "dq":
+            assert bool(((a - b).abs() <= 2.0 ** -7 * a.abs() + 2.0 ** -18 * a.abs().max()).all())
+        else:
+            assert torch.equal(a, b), n
+    seen = {"q": ("o", at), "k": ("o", at), "v": ("o", at + 3), "do": ("dv", at - 3)}[which]
+    assert bool(got[seen[0]][seen[1]].isnan().all())

@@ -401,8 +401,11 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     returns [B, Sq, H, D], zeros for a query that sees no key.  On the blackwell device with D = 128 and bf16 / fp16 the
     tensor-core kernels skip the blocks of keys outside the mask, in both directions; otherwise it is
     ``scaled_dot_product_attention`` with the mask.  There the gradient of ``q`` is summed in 32 bits in the order in which
-    blocks of keys arrive, which ``torch.use_deterministic_algorithms`` refuses, and a key or value that is not finite
-    reaches every query that shares a block of 128 keys with it, whether it sees it or not."""
+    blocks of keys arrive, which ``torch.use_deterministic_algorithms`` refuses, and what is not finite reaches further than the mask:
+    queries and keys are taken in blocks of 128 from the start of a sequence, and where any query of a block sees any key of another,
+    an infinity or NaN in a value of the one reaches the outputs and gradients of all queries of the other, one in a key the
+    gradients of all of them, one in a query or an incoming gradient those of all keys.  Other blocks, heads, sequences and batches
+    are not reached.  A call that is to be differentiated keeps a second tensor like the output: what rounding left of it."""
     _check_window(True, window, sinks, softmax_scale)
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3] or k.shape[2] == 0 or q.shape[2] % k.shape[2]:
         raise ValueError(f"window_attention: q [B, Sq, H, D] and k, v [B, Sk, Hkv, D] with Hkv a divisor of H expected, got "
