@@ -551,3 +551,13 @@ def test_decoder_is_unchanged_by_drafts_that_are_refused(bw, dev):
         assert d.seq_lens.tolist() == [15, 0] and d.lens == [15, None] and len(d.free) == 5
     taken, _ = d.check(drafts, uniforms)
     assert d.seq_lens.tolist() == [16 + int(taken[0]), 0] and d.lens == [16 + int(taken[0]), None]
+
+
+def test_an_expanded_pool_is_read_but_not_written(bw, dev):
+    q, k, v, table, lens = (t.to(dev) for t in case(33, [40], 1, 4, 2, 64, 16, torch.bfloat16))
+    cos, sin = (t.to(dev) for t in precompute_rope_cache(64, 64))
+    new, one = q[:, 0], k[:, :1]
+    assert torch.equal(paged_attention(q, one.expand_as(k), v, table, lens), paged_attention(q, one.repeat(1, 2, 1, 1), v, table, lens))
+    for pools in ((one.expand_as(k), v), (k, v[:1].expand_as(v))):
+        with pytest.raises(RuntimeError, match="single memory location"):
+            paged_rope_cache(new, new[:, :2], new[:, 2:], cos, sin, *pools, table, lens)

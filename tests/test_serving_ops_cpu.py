@@ -407,3 +407,12 @@ def test_paged_decoder_refuses_drafts_of_another_type():
     with pytest.raises(ValueError, match="the decoder is on cpu"):
         dec.check(torch.zeros(1, 2, dtype=torch.long), torch.zeros(1, 3, device="meta"))
     assert dec.seq_lens.tolist() == dec.lens == [4] and len(dec.free) == 3
+
+
+def test_paged_rope_cache_refuses_an_expanded_pool():
+    _, kp, vp, table, lens = paged_case(8, [20], 1)
+    cos, sin = ops.precompute_rope_cache(32, 16)
+    x = torch.randn(1, 4, 16)
+    for k, v in ((kp[:, :1].expand_as(kp), vp), (kp, vp[:1].expand_as(vp))):
+        with pytest.raises(RuntimeError, match="single memory location"):
+            ops.paged_rope_cache(x, x[:, :2], x[:, 2:], cos, sin, k, v, table, lens)

@@ -7,6 +7,7 @@
 #include "core/DeviceAssert.h"
 
 #include <ATen/Functions.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/core/grad_mode.h>
 #include <torch/library.h>
 
@@ -118,6 +119,8 @@ at::Tensor paged_rope_cache(const at::Tensor& q_, const at::Tensor& k_, const at
   TORCH_CHECK((q_.scalar_type() == at::kBFloat16 || q_.scalar_type() == at::kHalf) && (D == 64 || D == 128) && k_.scalar_type() == q_.scalar_type() &&
                   v_.scalar_type() == q_.scalar_type(), op, ": bf16 / fp16 with head_dim 64 or 128");
   check_pools(op, k_pages, v_pages, D, q_.scalar_type());
+  at::assert_no_internal_overlap(k_pages);      // an expanded pool: heads or pages would be written over one another
+  at::assert_no_internal_overlap(v_pages);
   TORCH_CHECK(k_pages.size(1) == Hkv && H > 0, op, ": the pools have ", k_pages.size(1), " kv heads, k has ", Hkv);
   TORCH_CHECK(cos.scalar_type() == at::kFloat && sin.scalar_type() == at::kFloat && cos.dim() == 2 && cos.size(1) == D / 2 && cos.size(0) > 0 &&
                   sin.sizes() == cos.sizes() && cos.is_contiguous() && sin.is_contiguous(), op,

@@ -495,10 +495,12 @@ def paged_rope_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: tor
     [positions, D / 2].  Returns the rotated queries.  Tokens past the last sequence or before position 0 are padding:
     zeros come back for them and nothing is written.  A page number outside the pool or a position outside the tables is
     reported by the next ``synchronize()`` (the row is not written; the last angle is used).  Sequences do not
-    share the pages that they write."""
+    share the pages that they write, and the pools are not expanded tensors."""
     if _paged_native(q):
         return torch.ops.blackwell.paged_rope_cache(q, k, v, cos, sin, k_pages, v_pages, block_table, seq_lens, cu_seqlens)
     _no_grad_inputs("paged_rope_cache", q, k, v)
+    if any(n > 1 and stride == 0 for pool in (k_pages, v_pages) for n, stride in zip(pool.shape, pool.stride())):
+        raise RuntimeError("paged_rope_cache: an expanded pool cannot be written, more than one element refers to a single memory location")
     T, B, page = q.shape[0], seq_lens.shape[0], k_pages.shape[2]
     t = torch.arange(T, device=q.device)
     if cu_seqlens is None:
