@@ -514,3 +514,23 @@ def test_reach_of_what_is_not_finite_within_a_sequence(bw, dev, which, sinks):
             assert torch.equal(a, b), n
     seen = {"q": ("o", at), "k": ("o", at), "v": ("o", at + 3), "do": ("dv", at - 3)}[which]
     assert bool(got[seen[0]][seen[1]].isnan().all())
+
+
+def test_second_order_of_packed_sequences_is_refused(bw, dev):
+    """As of a dense batch, instead of a gradient with a part missing; the first order with a graph is as without."""
+    from torch_musa_b200.ops import flash_attn_varlen_func
+
+    q, k, v, do = (t.to(dev) for t in inputs(torch.bfloat16, (40, 2, D), (40, 1, D)))
+    for t in (q, k, v):
+        t.requires_grad_()
+    cu = torch.tensor([0, 15, 40], dtype=torch.int32).to(dev)
+    out = flash_attn_varlen_func(q, k, v, cu, cu, 25, 25, causal=True, window=8, sinks=1)
+    plain = torch.autograd.grad(out, (k, v), do, retain_graph=True)
+    grads = torch.autograd.grad(out, (k, v), do, create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(plain, grads))
+    with pytest.raises(RuntimeError):           # no graph behind them: the incoming gradient is a constant
+        grads[0].float().sum().backward()
+    out = flash_attn_varlen_func(q, k, v, cu, cu, 25, 25, causal=True, window=8, sinks=1)
+    grads = torch.autograd.grad(out.float().square().sum(), (k, v), create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        grads[0].float().sum().backward()

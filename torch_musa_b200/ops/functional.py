@@ -441,6 +441,10 @@ class _VarlenAttention(torch.autograd.Function):
         return dq, dk, dv, None, None, None, None, None, None, None, None
 
 
+class _VarlenWindowAttention(_VarlenAttention):
+    backward = staticmethod(torch.autograd.function.once_differentiable(_VarlenAttention.backward))
+
+
 def flash_attn_varlen_func(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens_q: torch.Tensor,
                            cu_seqlens_k: torch.Tensor, max_seqlen_q: int, max_seqlen_k: int,
                            softmax_scale: Optional[float] = None, causal: bool = False,
@@ -454,8 +458,9 @@ def flash_attn_varlen_func(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu
     ``window_attention``, and rows past the last sequence then get zeros, in the gradients too."""
     _check_window(causal, window, sinks, softmax_scale)
     if _native_attention(q, k, v):
-        return _VarlenAttention.apply(q, k, v, cu_seqlens_q.to(torch.int32), cu_seqlens_k.to(torch.int32),
-                                      int(max_seqlen_q), int(max_seqlen_k), bool(causal), softmax_scale, window, int(sinks))
+        attention = _VarlenAttention if window is None else _VarlenWindowAttention
+        return attention.apply(q, k, v, cu_seqlens_q.to(torch.int32), cu_seqlens_k.to(torch.int32),
+                               int(max_seqlen_q), int(max_seqlen_k), bool(causal), softmax_scale, window, int(sinks))
     cq, ck = cu_seqlens_q.tolist(), cu_seqlens_k.tolist()
     rep = q.shape[1] // k.shape[1]
     outs = []
