@@ -69,7 +69,10 @@ __device__ __forceinline__ int chunks_of(const WindowParams& p, int q_blocks) { 
 // The first of sequence b's places.  Packed sequences find theirs by their first row alone, without a sum over those in front: with
 // c = sink_chunk, n > c query blocks are at least 128 (n - 1) + 1 rows and n' = ceil(n / c) = floor((n - 1) / c) + 1 chunks, so that
 // n' <= 2 floor((n - 1) / c) <= 2 rows / (128 c), and ceil(x + y) - ceil(x) >= floor(y).
-__host__ __device__ __forceinline__ int slots_before(int64_t rows, int chunk) { return (int)((2 * rows + BQ * chunk - 1) / (BQ * chunk)); }
+__host__ __device__ __forceinline__ int slots_before(int rows, int chunk) {
+  const unsigned c = BQ / 2 * (unsigned)chunk;
+  return (int)(((unsigned)rows + c - 1) / c);
+}
 __device__ __forceinline__ int first_slot(const WindowParams& p, int b) {
   return p.cu_q ? slots_before(p.cu_q[b], p.sink_chunk) : b * chunks_of(p, p.q_blocks);
 }
@@ -692,28 +695,29 @@ attn_window_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
 }
 
 // dV and dK of the blocks with sinks of sequences that have more than one chunk: the chunks' sums, added in order (the same for every run)
-// and rounded once.  Eight blocks a place, key block and key head; a thread owns eight dimensions of a row.  Packed sequences: the
-// blocks of a sequence's first place do the work.
+// and rounded once.  Eight blocks a sequence, key block and key head; a thread owns eight dimensions of a row.  Where there are more packed
+// sequences than places, the blocks go by places, and those of a sequence's first one do its work.
 template <typename T>
 __global__ void __launch_bounds__(256) attn_sink_sum_kernel(T* __restrict__ dk, T* __restrict__ dv, const WindowParams p) {
   const int which = blockIdx.y, r = (int)(blockIdx.x % 8) * 16 + (threadIdx.x >> 4), c = (threadIdx.x & 15) * 8;
-  const int unit = (int)(blockIdx.x / 8), hk = unit % p.Hkv, kb = unit / p.Hkv % p.sink_blocks, place = unit / p.Hkv / p.sink_blocks;
-  const int kj = kb * BK + r;
-  int b = place, slot = place * chunks_of(p, p.q_blocks), Sk = p.Sk, Sq = p.Sq, koff = 0, bt = b;
+  const int unit = (int)(blockIdx.x / 8), kb = unit / p.Hkv, hk = unit - kb * p.Hkv, kj = kb * BK + r;
+  int b = (int)blockIdx.z, Sk = p.Sk, Sq = p.Sq, koff = 0, bt = b;
   if (p.cu_q) {
-    slot = place;
-    int above = p.B;                     // the last sequence whose places start here or before
-    b = 0;
-    while (above - b > 1) {
-      const int mid = (b + above) >> 1;
-      if (first_slot(p, mid) <= slot) b = mid; else above = mid;
+    if (p.sink_slots < p.B) {            // the last sequence whose places start here or before
+      int above = p.B;
+      b = 0;
+      while (above - b > 1) {
+        const int mid = (b + above) >> 1;
+        if (first_slot(p, mid) <= (int)blockIdx.z) b = mid; else above = mid;
+      }
+      if (first_slot(p, b) != (int)blockIdx.z) return;
     }
-    if (first_slot(p, b) != slot) return;
     koff = p.cu_k[b];
     Sk = p.cu_k[b + 1] - koff;
     Sq = p.cu_q[b + 1] - p.cu_q[b];
     bt = 0;
   }
+  const int slot = first_slot(p, b);
   const int q_blocks = query_blocks(p, b), chunks = chunks_of(p, q_blocks);
   if (chunks == 1 || kj >= Sk) return;
   int first, end;
@@ -735,10 +739,10 @@ __global__ void __launch_bounds__(256) attn_sink_sum_kernel(T* __restrict__ dk, 
 
 // How the query blocks of the key blocks with sinks are cut.  A chunk is about as long as what the other key blocks meet, but never so
 // short that there were more than four chunks an SM: that is enough to even the units out, and it bounds the scratch by the
-// machine (128 KB a chunk; at most 1776, 222 MB) whatever the lengths and however many sinks.  (Cut by the longest sequence for all: one
-// sequence of 8192 tokens and 199 of under 60 with 8 key heads, window 128, four sinks, took 6.4 GB and 1340
-// us, now 0.1 GB and 655; 16384 tokens, 4 heads, window 128, 4096 sinks: 1.0 GB and 970 us, now 0.1 and 445; 32 heads x 4096, window 64,
-// four sinks: 257 us, now 245.)
+// machine (128 KB a chunk; at most 1776, 222 MB) whatever the lengths and however many sinks.  Cut by the longest sequence for all, one
+// sequence of 8192 tokens and 199 of under 60 (8 key heads, window 128, four sinks) took 6.4 GB and 1340 us, now 0.1 GB and 620; 16384
+// tokens with 4 heads, window 128 and 4096 sinks 1.0 GB and 970 us, now 0.1 GB and 440; 32 heads x 4096, window 64, four sinks 257 us,
+// now 241.
 struct SinkPlan {
   int blocks, chunk, slots;
 };
@@ -812,8 +816,8 @@ int attn_window_bwd(const b200_attn_t* a, float* dq_accum, void* dk, void* dv, f
     kern<<<grid, kBwdThreads, kBwdSmem, stream>>>(m.q, m.k, m.v, m.d_o, m.dq, gk, gv, p);
     note_launch(2);
     if (plan.slots > 0) {
-      const unsigned places = (unsigned)(p.cu_q ? plan.slots : a->B);
-      attn_sink_sum_kernel<T><<<dim3(places * (unsigned)(plan.blocks * a->Hkv * 8), 2), 256, 0, stream>>>(gk, gv, p);
+      const unsigned z = (unsigned)std::min(plan.slots, a->B);
+      attn_sink_sum_kernel<T><<<dim3((unsigned)(plan.blocks * a->Hkv * 8), 2, z), 256, 0, stream>>>(gk, gv, p);
       note_launch();
     }
     return (int)cudaGetLastError();
