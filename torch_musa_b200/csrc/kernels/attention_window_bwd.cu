@@ -10,22 +10,23 @@
 //     their dV and dK go to fp32 buffers that a small kernel adds up in order.
 //   * Units are short, and starting and ending a CTA cost as much as three or four pairs of blocks: a CTA stays on its SM and takes every
 //     148th unit, turning round at either end so that long and short ones even out.  The loads of a unit's queries, and the waits for its
-//     first products, run while the one before it is stored.  A warp of its own finds the units and hands them over.  What a change of units still costs, about 5 us of 27 for nine pairs, is
-//     the chain K -> S^T -> P -> dS that starts afresh: K and V of the next unit have no place before the last product of this one.
+//     first products, run while the one before it is stored.  A warp of its own finds the units and hands them over.  What a change of
+//     units still costs, about 5 us of 27 for nine pairs, is the chain K -> S^T -> P -> dS that starts afresh: K and V of the next unit have
+//     no place before the last product of this one.
 //   * Hidden scores become -inf before the exponentials, two instructions an element, instead of tests inside the loops, whose second
 //     copy of the code cost more than they did (instructions came late).
 //   * The row sums of dO O are taken with what rounding left of O, which the forward keeps for it: with few keys in a window dS is a
 //     difference of nearly equal numbers, and the rounded O alone put the gradients of q and k off by 3.7e-3 of their norm (two keys, bf16),
-//     now 2.5e-3 as with many keys: dS is rounded before its products (1.7e-3, as much as the result's own rounding).  It costs 3 % of
-//     forward and backward.
+//     now 2.5e-3 as with many keys: dS is rounded before its products (1.7e-3, as much as the result's own rounding).  It costs 4.5 % of
+//     forward and backward at a window of 1024 (348 -> 364 us, 32 heads x 4096), 6 % at 256 and below.
 //   * dS goes into its products without the softmax scale, which dQ and dK get in 32 bits when they leave TMEM: in fp16 its values are small
 //     under a long window, and a scale of 0.088 in front of the rounding would take three and a half bits more from them (4096 keys, dO of
 //     2^-10: dQ and dK off by 1.3e-2 of their norm with it, 1.2e-3 without).  In return fp16's largest value, 65504, bounds P (dP - delta)
 //     itself and not 0.088 of it.
 //   * Packed rows that are not the sequence's own are zeros in shared memory before a product reads them: their probabilities are zero,
 //     but zero times what lies there need not be.
-// Measured (whole calls: row dots, this kernel, sums of the chunks, conversion of dQ): 32 heads x 4096, window 1024, four sinks 273 us (289
-// with a CTA per unit); with 8 key heads 260 us.  Tried and not kept: cutting the list of pairs into 148 equal shares, so that units are
+// Measured (whole calls: row dots, this kernel, sums of the chunks, conversion of dQ): 32 heads x 4096, window 1024, four sinks 277 us
+// (247 without sinks; a CTA per unit took 15 more); with 8 key heads 269 us.  Tried and not kept: cutting the list of pairs into 148 equal shares, so that units are
 // cut anywhere (32 heads x 4096: 484 us; neighbouring CTAs no longer read the same rows, and twice as many units begin afresh).
 //
 // Parity: no counterpart in the reference (its vendor flash backward takes a causal flag only: reference
@@ -739,7 +740,7 @@ __global__ void __launch_bounds__(256) attn_sink_sum_kernel(T* __restrict__ dk, 
 
 // How the query blocks of the key blocks with sinks are cut.  A chunk is about as long as what the other key blocks meet, but never so
 // short that there were more than four chunks an SM: that is enough to even the units out, and it bounds the scratch by the
-// machine (128 KB a chunk; at most 1776, 222 MB) whatever the lengths and however many sinks.  Cut by the longest sequence for all, one
+// machine (128 KB a chunk; at most 1776, 222 MiB) whatever the lengths and however many sinks.  Cut by the longest sequence for all, one
 // sequence of 8192 tokens and 199 of under 60 (8 key heads, window 128, four sinks) took 6.4 GB and 1340 us, now 0.1 GB and 620; 16384
 // tokens with 4 heads, window 128 and 4096 sinks 1.0 GB and 970 us, now 0.1 GB and 440; 32 heads x 4096, window 64, four sinks 257 us,
 // now 241.

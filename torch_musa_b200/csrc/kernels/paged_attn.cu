@@ -183,8 +183,10 @@ __device__ __forceinline__ bool unsettled(const float (&v)[4], float sum) {
 // What bounds it: memory, where the batch fills the machine -- 32 sequences of 1100 to 2048 keys with 32 key heads: 126 us, 830 MB read once,
 // 6.6 TB/s, warps waiting for their copies (long scoreboard 5.3 of 10.9 clocks an instruction); two of 50001 to 65536 keys with 8 key heads:
 // 82 us, 5.8 TB/s, on 384 of 444 places.  Where it is small, the way from the launch through length, table and keys to the joins: 3.4 us
-// for 32 keys, 5.1 for 500.  With several tokens at once, issue: 20 rows a key head, D 64, take 190 instructions for 16 keys (4 KB), so
-// 16 sequences, window 1024, five tokens take 14.3 us where one token takes 8.5.
+// for 32 keys, 5.1 for 500.  With several tokens at once the same chain, longer: 16 sequences, 8 key heads, D 64, 20 rows a key head take 5.9 us
+// for 8 keys (3.9 with four rows), 7.8 once two CTAs have to join (5.1), and 6.2 us more for each thousand keys (33 MB, out of the L2 cache;
+// 3.3 with four rows).  Three or four warps a scheduler issue 0.34 instructions a clock; they wait for one another's results (1.8
+// clocks an instruction), for copies (1.2) and at barriers (1.0).
 // On the way here (us, the first two of these cases): a warp per row and scalar products 2262 / 72680; the tensor core with operands
 // copied piece by piece into a lane's own slots 181 / 156 (600, then 400 instructions for 16 keys); whole rows and ldmatrix 127 / 93; keys as
 // the long side of the products 124 / 82, and D 64 with four rows a key head, 64 sequences of up to 4000 keys, 62 -> 50.
