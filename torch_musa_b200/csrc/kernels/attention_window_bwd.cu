@@ -26,8 +26,9 @@
 //   * Packed rows that are not the sequence's own are zeros in shared memory before a product reads them: their probabilities are zero,
 //     but zero times what lies there need not be.
 // Measured (whole calls: row dots, this kernel, sums of the chunks, conversion of dQ): 32 heads x 4096, window 1024, four sinks 277 us
-// (247 without sinks; a CTA per unit took 15 more); with 8 key heads 269 us.  Tried and not kept: cutting the list of pairs into 148 equal shares, so that units are
-// cut anywhere (32 heads x 4096: 484 us; neighbouring CTAs no longer read the same rows, and twice as many units begin afresh).
+// (247 without sinks; a CTA per unit took 15 more); with 8 key heads 269 us.  Tried and not kept: cutting the list of pairs into 148 equal
+// shares, so that units are cut anywhere (32 heads x 4096: 484 us; neighbouring CTAs no longer read the same rows, and twice as many
+// units begin afresh).
 //
 // Parity: no counterpart in the reference (its vendor flash backward takes a causal flag only: reference
 // torch_musa/csrc/aten/ops/attention/mudnn/SDP.cpp:678-845).

@@ -135,7 +135,8 @@ __device__ __forceinline__ bool not_finite(uint32_t w) {
 // found a NaN: 2 to 9 %).
 template <typename T>
 __device__ __noinline__ float4 settle_infinities(float4 sums, const T* vp, const PagedParams& p, int b, int hk, int i, int d) {
-  const int pos = min(max(__ldg(p.lens + b), 0), p.table_width * p.page_size) - p.n + i, from = p.window > 0 ? max(0, pos - p.window + 1) : 0;
+  const int pos = min(max(__ldg(p.lens + b), 0), p.table_width * p.page_size) - p.n + i;
+  const int from = p.window > 0 ? max(0, pos - p.window + 1) : 0;
   const int* table = p.table + b * p.table_sb;
   const T* v = vp + hk * p.v_sh + d;
   constexpr uint32_t kExp = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
@@ -194,7 +195,8 @@ __device__ __forceinline__ bool unsettled(const float (&v)[4], float sum) {
 // away from the page's.
 template <typename T, int D, int NT, bool kDense>
 __global__ void __launch_bounds__(kPagedWarps * 32, NT * D <= 256 ? 3 : 2)
-paged_attn_kernel(T* __restrict__ out, const T* __restrict__ q, const T* __restrict__ kp, const T* __restrict__ vp, const __grid_constant__ PagedParams p) {
+paged_attn_kernel(T* __restrict__ out, const T* __restrict__ q, const T* __restrict__ kp, const T* __restrict__ vp,
+                  const __grid_constant__ PagedParams p) {
   constexpr int kRows = 8 * NT, kHalves = D == 64 && NT <= 2 ? 2 : 1, kKeys = kHalves * kPageRows, kHalf = kPageRows * D * 2;
   constexpr int kStageBytes = 2 * kHalves * kHalf, kStages = kWarpRing / kStageBytes;
   constexpr int kPad = D + 4;            // floats of a row of a part: the four lanes' rows then lie in different banks
@@ -613,7 +615,8 @@ paged_attn_kernel(T* __restrict__ out, const T* __restrict__ q, const T* __restr
 
 // Joins the clusters' parts of a row: a thread owns four dimensions of one row.
 template <typename T, int D>
-__global__ void __launch_bounds__(128) paged_join_kernel(T* __restrict__ out, const T* __restrict__ vp, const __grid_constant__ PagedParams p) {
+__global__ void __launch_bounds__(128) paged_join_kernel(T* __restrict__ out, const T* __restrict__ vp,
+                                                         const __grid_constant__ PagedParams p) {
   const int G = p.H / p.Hkv, rows_all = p.n * G;
   const int64_t x = (int64_t)blockIdx.x * 128 + threadIdx.x, row = x / (D / 4);
   if (row >= (int64_t)p.B * p.Hkv * rows_all) return;

@@ -603,12 +603,12 @@ def verify_drafts(target_probs: torch.Tensor, draft_tokens: torch.Tensor, unifor
     distributed as if it were sampled from the target alone.
 
     ``target_probs`` [B, n + 1, V] (the rows for the n drafted tokens and the one after them), ``draft_tokens`` int64 [B, n],
-    ``uniforms`` float32 [B, n + 1] in [0, 1), ``draft_probs`` [B, n, V] in the type of ``target_probs`` or None for drafts that were certain (a greedy
-    draft).  Draft i is taken while ``uniforms[i] * draft_probs[i, x_i] < target_probs[i, x_i]``; at the first refusal r one
-    token is drawn from ``max(target_probs[r] - draft_probs[r], 0)``, after n taken drafts from ``target_probs[n]``: the first
-    token at which the running sum exceeds ``uniforms[n]`` times the whole (a number below zero or NaN counts as zero there, from one on
-    it is the last token that has weight).  A draft outside the vocabulary (-1, say) ends a
-    sequence's draft early: the token there is drawn from the target's row.  Sums are held in 64 bits.
+    ``uniforms`` float32 [B, n + 1] in [0, 1), ``draft_probs`` [B, n, V] in the type of ``target_probs`` or None for drafts that
+    were certain (a greedy draft).  Draft i is taken while ``uniforms[i] * draft_probs[i, x_i] < target_probs[i, x_i]``;
+    at the first refusal r one token is drawn from ``max(target_probs[r] - draft_probs[r], 0)``, after n taken drafts from
+    ``target_probs[n]``: the first token at which the running sum exceeds ``uniforms[n]`` times the whole (a number below
+    zero or NaN counts as zero there, from one on it is the last token that has weight).  A draft outside the vocabulary
+    (-1, say) ends a sequence's draft early: the token there is drawn from the target's row.  Sums are held in 64 bits.
 
     Returns ``(taken [B], tokens [B, n + 1])``, both int64: the taken drafts, the drawn token, then -1.  Where a row has no
     weight at all (zeros or NaN) the drawn token is -1."""
